@@ -556,7 +556,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(KVT) == 2 ? 4 : 2) void attn_rows_k
         KvLoad<KVT>::unpack(rkb[slot], kvb);
         KvLoad<KVT>::unpack(rva[slot], vva);
         KvLoad<KVT>::unpack(rvb[slot], vvb);
-        // packed fp32 multiply-adds (v_pk_fma_f32: two lanes of arithmetic per instruction): element pairs (e, e + 1)
+        // the library is built without packed fp32 instructions (Makefile): these are pairs of scalar multiply-adds over elements (e, e + 1)
         // of both keys; the per-key dot product is the sum of an even and an odd chain
         f32x2 da = {0.f, 0.f}, db = {0.f, 0.f};
 #pragma unroll
