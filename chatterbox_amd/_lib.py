@@ -68,6 +68,38 @@ class HiftInfo(C.Structure):
                                          "device", "reserved_")] + [("weight_bytes", C.c_int64)]
 
 
+class PagedCache(C.Structure):
+    """t3mi_paged_cache (a struct's fields in its order: the operators fill them by position)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("block_table", C.c_void_p),
+                ("table_stride", C.c_int64)] + [(n, C.c_int32) for n in ("n_seqs", "max_pages", "n_pages", "page_size", "kv_heads", "head_dim",
+                                                                        "dtype", "device")]
+
+
+class AppendArgs(C.Structure):
+    """t3mi_append_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "q", "q_out")] + \
+               [(n, C.c_int64 * 2) for n in ("k_stride", "v_stride", "q_stride", "q_out_stride")] + \
+               [("cos", C.c_void_p), ("sin", C.c_void_p), ("rope_stride", C.c_int64), ("positions", C.c_void_p), ("seq", C.c_void_p)] + \
+               [(n, C.c_int32) for n in ("rows", "q_heads", "rope_len", "dtype")]
+
+
+class AttentionArgs(C.Structure):
+    """t3mi_attention_args"""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64 * 2), ("out_stride", C.c_int64 * 2), ("lengths", C.c_void_p),
+                ("starts", C.c_void_p), ("seq", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("scale", C.c_float)] + \
+               [(n, C.c_int32) for n in ("rows", "q_heads", "q_dtype", "out_dtype", "length_add", "max_length")]
+
+
+class LogitsArgs(C.Structure):
+    """t3mi_logits_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "uncond", "out")] + [(n, C.c_int64) for n in ("logits_stride", "uncond_stride", "out_stride")] + \
+               [("tokens", C.c_void_p), ("n_tokens", C.c_void_p), ("tokens_stride", C.c_int64)] + \
+               [(n, C.c_void_p) for n in ("repetition_each", "frequency_each", "presence_each", "bias_ids", "bias_values")] + \
+               [("bias_ids_stride", C.c_int64), ("bias_values_stride", C.c_int64), ("allowed", C.c_void_p), ("allowed_stride", C.c_int64)] + \
+               [(n, C.c_float) for n in ("cfg_weight", "repetition", "frequency", "presence")] + \
+               [(n, C.c_int32) for n in ("rows", "vocab", "dtype", "token_cap", "n_bias", "device")]
+
+
 class KStat(C.Structure):
     _fields_ = [("name", C.c_char * 32), ("launches", C.c_int32), ("total_us", C.c_float),
                 ("bytes", C.c_double)]
@@ -132,6 +164,10 @@ SYMBOLS = {
     "t3mi_hift_close": (C.c_int, [_H]),
     "t3mi_hift_get_info": (C.c_int, [_H, C.POINTER(HiftInfo)]),
     "t3mi_hift_inference": (C.c_int, [_H, C.c_int, _FP, _FP, _FP, _FP, C.c_int, _FP, _FP, _FP, _FP]),
+    "t3mi_paged_append": (C.c_int, [C.POINTER(PagedCache), C.POINTER(AppendArgs), C.c_void_p]),
+    "t3mi_paged_attention_workspace": (C.c_int, [C.POINTER(PagedCache), C.POINTER(AttentionArgs), C.POINTER(C.c_size_t)]),
+    "t3mi_paged_attention": (C.c_int, [C.POINTER(PagedCache), C.POINTER(AttentionArgs), C.c_void_p]),
+    "t3mi_process_logits": (C.c_int, [C.POINTER(LogitsArgs), C.c_void_p]),
     "t3mi_cfm_solve": (C.c_int, [_H, C.c_int, _FP, _FP, _FP, _FP, _FP, C.c_int, C.c_double, C.c_int, _FP, _FP]),
 }
 

@@ -1,0 +1,181 @@
+// t3mi C ABI: the serving operators on caller-owned device tensors (include/t3mi.h).  Argument checks and launches; no state.
+#include "t3mi.h"
+
+#include <hip/hip_runtime_api.h>
+
+#include <string>
+
+#include "ops_kernels.hpp"
+
+int t3mi_set_error(int code, const std::string& msg);   // t3mi.cpp
+
+namespace {
+
+int bad(const char* where, const char* what) { return t3mi_set_error(T3MI_ERR_ARG, std::string(where) + ": " + what); }
+
+// the operators' device, for the length of a call; the caller's current device afterwards
+struct OnDevice {
+    int before = -1, device;
+    hipError_t err;
+    explicit OnDevice(int d) : device(d) {
+        err = hipGetDevice(&before);
+        if (err == hipSuccess && before != device) err = hipSetDevice(device);
+    }
+    ~OnDevice() {
+        if (before >= 0 && before != device) (void)hipSetDevice(before);
+    }
+};
+
+int done(const char* where, hipError_t e) {
+    if (e == hipSuccess) return T3MI_OK;
+    return t3mi_set_error(T3MI_ERR_HIP, std::string(where) + ": " + hipGetErrorString(e));
+}
+
+bool is_type(int t) { return t == T3MI_W_F32 || t == T3MI_W_BF16; }
+bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool at4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+bool step16(int64_t s, int dtype) { return s >= 0 && ((s * (dtype == T3MI_W_BF16 ? 2 : 4)) & 15) == 0; }
+template <int N> bool steps16(const int64_t (&s)[N], int dtype) {
+    for (int i = 0; i < N; ++i)
+        if (!step16(s[i], dtype)) return false;
+    return true;
+}
+
+int take_cache(const char* where, const t3mi_paged_cache* c, t3k::PagedCache& o) {
+    if (!c) return bad(where, "null cache");
+    if (!c->k || !c->v || !c->block_table) return bad(where, "the cache has a null pointer");
+    if (!is_type(c->dtype)) return bad(where, "cache dtype must be T3MI_W_F32 or T3MI_W_BF16");
+    if (c->head_dim != 64 && c->head_dim != 128) return bad(where, "head_dim must be 64 or 128");
+    if (c->kv_heads <= 0 || c->n_seqs <= 0 || c->max_pages <= 0 || c->n_pages <= 0) return bad(where, "cache extents must be positive");
+    if (c->page_size <= 0 || c->page_size > 65536 || (c->page_size & (c->page_size - 1))) return bad(where, "page_size must be a power of two, at most 65536");
+    if ((int64_t)c->max_pages * c->page_size > 0x7FFFFF00LL) return bad(where, "a sequence may have at most 2^31 - 256 keys");
+    if (!at16(c->k) || !at16(c->v) || !steps16(c->k_stride, c->dtype) || !steps16(c->v_stride, c->dtype))
+        return bad(where, "cache addresses and strides must be multiples of 16 bytes");
+    if (!at4(c->block_table) || c->table_stride < 0) return bad(where, "bad block table");
+    o.k = c->k; o.v = c->v;
+    o.kp = c->k_stride[0]; o.ks = c->k_stride[1]; o.kh = c->k_stride[2];
+    o.vp = c->v_stride[0]; o.vs = c->v_stride[1]; o.vh = c->v_stride[2];
+    o.table = c->block_table; o.table_stride = c->table_stride;
+    o.n_seqs = c->n_seqs; o.max_pages = c->max_pages; o.n_pages = c->n_pages;
+    o.page_shift = __builtin_ctz((unsigned)c->page_size);
+    o.kv_heads = c->kv_heads; o.head_dim = c->head_dim; o.bf16 = c->dtype == T3MI_W_BF16;
+    return T3MI_OK;
+}
+
+int take_attention(const char* where, const t3mi_paged_cache* cache, const t3mi_attention_args* a, t3k::PagedAttnArgs& o) {
+    int rc = take_cache(where, cache, o.c);
+    if (rc) return rc;
+    if (!a) return bad(where, "null arguments");
+    if (a->rows < 0 || a->q_heads <= 0 || a->q_heads % cache->kv_heads) return bad(where, "q_heads must be a positive multiple of kv_heads");
+    if (!is_type(a->q_dtype) || !is_type(a->out_dtype)) return bad(where, "dtypes must be T3MI_W_F32 or T3MI_W_BF16");
+    if (a->q_dtype == T3MI_W_BF16 && cache->dtype != T3MI_W_BF16) return bad(where, "bf16 queries need a bf16 cache");
+    if (a->max_length < 0 || (a->length_add != 0 && a->length_add != 1)) return bad(where, "max_length must be >= 0, length_add 0 or 1");
+    if ((int64_t)a->rows * a->q_heads > 0x1000000LL) return bad(where, "at most 2^24 (row, head) pairs a call");
+    if (!(a->scale == a->scale) || a->scale - a->scale != 0.f) return bad(where, "scale must be finite");
+    if (a->rows && (!a->q || !a->out || !a->lengths)) return bad(where, "null pointer");
+    if (!at16(a->q) || !at16(a->out) || !steps16(a->q_stride, a->q_dtype) || !steps16(a->out_stride, a->out_dtype))
+        return bad(where, "q and out: addresses and strides must be multiples of 16 bytes");
+    if (!a->seq && a->rows > cache->n_seqs) return bad(where, "more rows than sequences (seq says which row belongs to which)");
+    o.q = a->q; o.out = a->out;
+    o.qr = a->q_stride[0]; o.qh = a->q_stride[1]; o.outr = a->out_stride[0]; o.outh = a->out_stride[1];
+    o.lengths = a->lengths; o.starts = a->starts; o.seq = a->seq;
+    o.scale = a->scale; o.rows = a->rows; o.q_heads = a->q_heads;
+    o.q_bf16 = a->q_dtype == T3MI_W_BF16; o.out_bf16 = a->out_dtype == T3MI_W_BF16;
+    const int64_t most = (int64_t)cache->max_pages * cache->page_size;
+    o.max_length = (int)(a->max_length > 0 && a->max_length < most ? a->max_length : most);
+    o.length_add = a->length_add;
+    return T3MI_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int t3mi_paged_append(const t3mi_paged_cache* cache, const t3mi_append_args* a, void* stream) {
+    const char* me = "t3mi_paged_append";
+    t3k::PagedAppendArgs o;
+    int rc = take_cache(me, cache, o.c);
+    if (rc) return rc;
+    if (!a) return bad(me, "null arguments");
+    if (a->rows < 0) return bad(me, "rows must be >= 0");
+    if (!is_type(a->dtype)) return bad(me, "dtype must be T3MI_W_F32 or T3MI_W_BF16");
+    if ((a->q != nullptr) != (a->q_out != nullptr)) return bad(me, "q and q_out go together");
+    if (a->q && a->q_heads <= 0) return bad(me, "q_heads must be positive");
+    if ((a->cos != nullptr) != (a->sin != nullptr)) return bad(me, "cos and sin go together");
+    if (a->cos && (a->rope_len <= 0 || a->rope_stride < 0)) return bad(me, "bad rotation tables");
+    if (a->rows && (!a->k || !a->v || !a->positions)) return bad(me, "null pointer");
+    if (!at16(a->k) || !at16(a->v) || !at16(a->q) || !at16(a->q_out) || !steps16(a->k_stride, a->dtype) || !steps16(a->v_stride, a->dtype) ||
+        (a->q && (!steps16(a->q_stride, a->dtype) || !steps16(a->q_out_stride, a->dtype))))
+        return bad(me, "k, v, q and q_out: addresses and strides must be multiples of 16 bytes");
+    if (!at4(a->cos) || !at4(a->sin)) return bad(me, "rotation tables must be aligned to 4 bytes");
+    if (a->q && a->q == a->q_out && (a->q_stride[0] != a->q_out_stride[0] || a->q_stride[1] != a->q_out_stride[1]))
+        return bad(me, "q_out may be q only with the same strides");
+    if (!a->seq && a->rows > cache->n_seqs) return bad(me, "more rows than sequences (seq says which row belongs to which)");
+    if ((int64_t)a->rows * ((a->q ? a->q_heads : 0) + 2LL * cache->kv_heads) > 0x10000000LL) return bad(me, "at most 2^28 (row, head) pairs a call");
+    if (a->rows == 0) return T3MI_OK;
+    o.k = a->k; o.v = a->v; o.q = a->q; o.q_out = a->q_out;
+    o.kr = a->k_stride[0]; o.kh = a->k_stride[1]; o.vr = a->v_stride[0]; o.vh = a->v_stride[1];
+    o.qr = a->q_stride[0]; o.qh = a->q_stride[1]; o.qor = a->q_out_stride[0]; o.qoh = a->q_out_stride[1];
+    o.cos = a->cos; o.sin = a->sin; o.rope_stride = a->rope_stride; o.rope_len = a->rope_len;
+    o.positions = a->positions; o.seq = a->seq; o.rows = a->rows; o.q_heads = a->q ? a->q_heads : 0; o.in_bf16 = a->dtype == T3MI_W_BF16;
+    OnDevice dev(cache->device);
+    if (dev.err != hipSuccess) return done(me, dev.err);
+    return done(me, t3k::launch_paged_append(o, (hipStream_t)stream));
+}
+
+int t3mi_paged_attention_workspace(const t3mi_paged_cache* cache, const t3mi_attention_args* args, size_t* bytes) {
+    const char* me = "t3mi_paged_attention_workspace";
+    if (!bytes) return bad(me, "null result");
+    t3k::PagedAttnArgs o;
+    int rc = take_attention(me, cache, args, o);
+    if (rc) return rc;
+    *bytes = 0;
+    return T3MI_OK;
+}
+
+int t3mi_paged_attention(const t3mi_paged_cache* cache, const t3mi_attention_args* args, void* stream) {
+    const char* me = "t3mi_paged_attention";
+    t3k::PagedAttnArgs o;
+    int rc = take_attention(me, cache, args, o);
+    if (rc) return rc;
+    if (o.rows == 0) return T3MI_OK;
+    OnDevice dev(cache->device);
+    if (dev.err != hipSuccess) return done(me, dev.err);
+    return done(me, t3k::launch_paged_attention(o, (hipStream_t)stream));
+}
+
+int t3mi_process_logits(const t3mi_logits_args* a, void* stream) {
+    const char* me = "t3mi_process_logits";
+    if (!a) return bad(me, "null arguments");
+    if (a->rows < 0 || a->rows > 65535 || a->vocab <= 0) return bad(me, "rows must be 0..65535, vocab positive");
+    if (!is_type(a->dtype)) return bad(me, "dtype must be T3MI_W_F32 or T3MI_W_BF16");
+    if (a->rows && (!a->logits || !a->out)) return bad(me, "null logits or out");
+    const uintptr_t low = a->dtype == T3MI_W_BF16 ? 1u : 3u;
+    if (((reinterpret_cast<uintptr_t>(a->logits) | reinterpret_cast<uintptr_t>(a->uncond) | reinterpret_cast<uintptr_t>(a->out)) & low) != 0)
+        return bad(me, "logits must be aligned to their elements");
+    if (a->logits_stride < 0 || a->uncond_stride < 0 || a->tokens_stride < 0 || a->bias_ids_stride < 0 || a->bias_values_stride < 0 || a->allowed_stride < 0)
+        return bad(me, "strides must be >= 0");
+    if (a->rows > 1 && a->out_stride < a->vocab) return bad(me, "the rows of out must not overlap");
+    if (a->out == a->logits && a->rows > 1 && a->out_stride != a->logits_stride) return bad(me, "out may be logits only with the same stride");
+    if (a->tokens && (!a->n_tokens || a->token_cap < 0 || a->token_cap > 1048575)) return bad(me, "tokens need n_tokens and a token_cap of 0..1048575");
+    if (a->n_bias < 0 || a->n_bias > 4094 || (a->n_bias > 0 && (!a->bias_ids || !a->bias_values))) return bad(me, "n_bias must be 0..4094, with ids and values");
+    if (!a->repetition_each && !(a->repetition > 0.f)) return bad(me, "repetition must be > 0");
+    if (!at4(a->tokens) || !at4(a->n_tokens) || !at4(a->bias_ids) || !at4(a->bias_values) || !at4(a->allowed) || !at4(a->repetition_each) ||
+        !at4(a->frequency_each) || !at4(a->presence_each))
+        return bad(me, "arrays must be aligned to 4 bytes");
+    if (a->rows == 0) return T3MI_OK;
+    t3k::LogitsArgs o;
+    o.logits = a->logits; o.uncond = a->uncond; o.out = a->out;
+    o.lr = a->logits_stride; o.ur = a->uncond_stride; o.outr = a->out_stride;
+    o.bf16 = a->dtype == T3MI_W_BF16; o.rows = a->rows; o.vocab = a->vocab; o.cfg_weight = a->cfg_weight;
+    o.tokens = a->tokens; o.n_tokens = a->n_tokens; o.tr = a->tokens_stride; o.cap = a->token_cap;
+    o.repetition = a->repetition_each; o.frequency = a->frequency_each; o.presence = a->presence_each;
+    o.repetition_s = a->repetition; o.frequency_s = a->frequency; o.presence_s = a->presence;
+    o.bias_ids = a->bias_ids; o.bias_values = a->bias_values; o.br = a->bias_ids_stride; o.bvr = a->bias_values_stride; o.n_bias = a->n_bias;
+    o.allowed = a->allowed; o.ar = a->allowed_stride;
+    OnDevice dev(a->device);
+    if (dev.err != hipSuccess) return done(me, dev.err);
+    return done(me, t3k::launch_process_logits(o, (hipStream_t)stream));
+}
+
+}  // extern "C"

@@ -349,6 +349,109 @@ int t3mi_hift_get_info(const t3mi_hift* m, t3mi_hift_info* info);
 int t3mi_hift_inference(t3mi_hift* m, int T, const float* mel, const float* phase, const float* noise, const float* cache_source,
                         int cache_len, float* audio, float* source_out, float* f0_out, float* device_ms);
 
+/* ---- serving operators on the caller's device tensors ---------------------------------------------------------------------
+ * What a serving loop of its own needs beside the sessions above (which call the same kernels: t3mi_set_paged_kv,
+ * t3mi_set_logit_rules): a key-value cache in pages shared by many sequences, and the rules a logits row goes through before it is
+ * sampled.  The reference has no counterpart (its caches are contiguous, R/llama_traced.R:274-297; its sampling tail knows the
+ * repetition penalty alone, R/t3.R:529-537).  Every pointer in the structs is device memory of GPU `device`; the calls enqueue on
+ * `stream` (a hipStream_t, NULL = the default stream), allocate nothing, wait for nothing and may be captured into a graph.  What
+ * the host can see is checked (T3MI_ERR_ARG); what lives in device memory -- lengths, positions, page numbers, token ids -- is
+ * checked by the kernels, which never read or write outside what the struct describes.  Rows of tensors may have any strides
+ * whose last dimension is contiguous; addresses and strides are multiples of 16 bytes except where noted.  Element types:
+ * T3MI_W_F32 / T3MI_W_BF16; all sums and softmax statistics are fp32. */
+
+/* One layer's keys and values in pages: element (page, slot, head, i) of the keys is k[page * k_stride[0] + slot * k_stride[1] +
+ * head * k_stride[2] + i] (strides in elements).  Key j of sequence s is in page block_table[s * table_stride + j / page_size],
+ * slot j % page_size.  An entry outside 0..n_pages-1 names no page: keys there are absent. */
+typedef struct t3mi_paged_cache {
+    void* k;
+    void* v;
+    int64_t k_stride[3], v_stride[3];
+    const int32_t* block_table;  /* [n_seqs, max_pages]                                      */
+    int64_t table_stride;
+    int32_t n_seqs, max_pages, n_pages;
+    int32_t page_size;           /* a power of two, 1..65536                                 */
+    int32_t kv_heads;
+    int32_t head_dim;            /* 64 or 128                                                */
+    int32_t dtype, device;
+} t3mi_paged_cache;
+
+/* Append: row r's key and value go to position positions[r] of sequence seq[r] (NULL: sequence r).  With cos / sin ([rope_len, >=
+ * head_dim / 2] fp32, 4-byte aligned) keys and queries are rotated by their position's angle on the way, element i with element
+ * i + head_dim / 2 (apply_rotary_pos_emb, R/llama.R:155-188): (a, b) -> (a cos - b sin, b cos + a sin); the rotated queries go to
+ * q_out (may be q itself, with the same strides).  A row whose position is negative, beyond the tables or on no page is skipped: neither
+ * the cache nor its q_out row is written.  No two rows of a call may name the same place. */
+typedef struct t3mi_append_args {
+    const void* k;               /* [rows, kv_heads, head_dim], type dtype; strides (row, head) */
+    const void* v;
+    const void* q;               /* [rows, q_heads, head_dim] or NULL                        */
+    void* q_out;
+    int64_t k_stride[2], v_stride[2], q_stride[2], q_out_stride[2];
+    const float* cos;            /* both NULL: no rotation                                   */
+    const float* sin;
+    int64_t rope_stride;
+    const int32_t* positions;    /* [rows]                                                   */
+    const int32_t* seq;          /* [rows] or NULL                                           */
+    int32_t rows, q_heads, rope_len;
+    int32_t dtype;               /* of k, v, q and q_out; the cache has its own              */
+} t3mi_append_args;
+int t3mi_paged_append(const t3mi_paged_cache* cache, const t3mi_append_args* args, void* stream);
+
+/* Attention of one new token per row: out[r, h] = sum_j softmax_j(scale * q[r, h] . k_j) v_j over the keys j in [starts[r],
+ * lengths[r] + length_add) of sequence seq[r], head h reading key head h / (q_heads / kv_heads).  Row r of a prompt's queries attends
+ * causally when lengths[r] is its position and length_add 1.  A row with no key is written as zeros, a row whose length is negative is left as it
+ * was (padding of a batch); lengths beyond the block table end there.  Types: q fp32 over an fp32 or bf16 cache, q bf16 over a bf16
+ * cache; out fp32 or bf16. */
+typedef struct t3mi_attention_args {
+    const void* q;               /* [rows, q_heads, head_dim]; strides (row, head)           */
+    void* out;
+    int64_t q_stride[2], out_stride[2];
+    const int32_t* lengths;      /* [rows]                                                   */
+    const int32_t* starts;       /* [rows] or NULL                                           */
+    const int32_t* seq;          /* [rows] or NULL                                           */
+    void* workspace;             /* at least what t3mi_paged_attention_workspace says; one call in flight at a time */
+    size_t workspace_bytes;
+    float scale;
+    int32_t rows, q_heads;       /* q_heads: a multiple of kv_heads                          */
+    int32_t q_dtype, out_dtype;
+    int32_t length_add;          /* 0 or 1                                                   */
+    int32_t max_length;          /* about the longest length, for planning alone (0: the table's); longer rows are still right */
+} t3mi_attention_args;
+int t3mi_paged_attention_workspace(const t3mi_paged_cache* cache, const t3mi_attention_args* args, size_t* bytes);
+int t3mi_paged_attention(const t3mi_paged_cache* cache, const t3mi_attention_args* args, void* stream);
+
+/* Rules on logits, row by row, in this order, in fp32, rounded once to dtype:
+ *   z = l + cfg_weight (l - u)                     with uncond rows u (the guidance of R/t3.R:518-524)
+ *   z += bias_values[i]                            where bias_ids[i] names the token (the last i that does; ids outside 0..vocab-1 name none)
+ *   z = z / repetition (z > 0) or z * repetition   where the token occurs among tokens[r, 0 .. n_tokens[r]) (sign-aware, R/t3.R:1699-1708)
+ *   z -= frequency * occurrences + presence        likewise
+ *   z = -inf                                       where bit (t & 31) of allowed[r, t >> 5] is 0, whatever z was
+ * A row whose mask allows nothing is all -inf.  Row strides are in elements; 0 shares one bias list or mask among the rows.  out may
+ * be logits.  Addresses are aligned to their elements only. */
+typedef struct t3mi_logits_args {
+    const void* logits;          /* [rows, vocab]                                            */
+    const void* uncond;          /* [rows, vocab] or NULL                                    */
+    void* out;
+    int64_t logits_stride, uncond_stride, out_stride;
+    const int32_t* tokens;       /* [rows, token_cap] or NULL: no penalties                  */
+    const int32_t* n_tokens;     /* [rows]                                                   */
+    int64_t tokens_stride;
+    const float* repetition_each;   /* [rows] each, or NULL: the scalar below                */
+    const float* frequency_each;
+    const float* presence_each;
+    const int32_t* bias_ids;     /* [rows, n_bias] or NULL                                   */
+    const float* bias_values;
+    int64_t bias_ids_stride, bias_values_stride;
+    const uint32_t* allowed;     /* [rows, >= ceil(vocab / 32)] or NULL                      */
+    int64_t allowed_stride;
+    float cfg_weight, repetition, frequency, presence;
+    int32_t rows, vocab, dtype;
+    int32_t token_cap;           /* at most 1048575                                          */
+    int32_t n_bias;              /* at most 4094                                             */
+    int32_t device;
+} t3mi_logits_args;
+int t3mi_process_logits(const t3mi_logits_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
