@@ -58,6 +58,8 @@ int take_cache(const char* where, const t3mi_paged_cache* c, t3k::PagedCache& o)
     o.table = c->block_table; o.table_stride = c->table_stride;
     o.n_seqs = c->n_seqs; o.max_pages = c->max_pages; o.n_pages = c->n_pages;
     o.page_shift = __builtin_ctz((unsigned)c->page_size);
+    // (the attention kernel addresses a tile of 32 slots by 32-bit offsets)
+    if (c->k_stride[1] > (1 << 24) || c->v_stride[1] > (1 << 24)) return bad(where, "slot strides may be at most 2^24 elements");
     o.kv_heads = c->kv_heads; o.head_dim = c->head_dim; o.bf16 = c->dtype == T3MI_W_BF16;
     return T3MI_OK;
 }
@@ -130,6 +132,9 @@ int t3mi_paged_attention_workspace(const t3mi_paged_cache* cache, const t3mi_att
     int rc = take_attention(me, cache, args, o);
     if (rc) return rc;
     *bytes = 0;
+    if (o.rows == 0) return T3MI_OK;
+    t3k::plan_paged_attention(o);
+    *bytes = t3k::paged_attention_workspace(o);
     return T3MI_OK;
 }
 
@@ -139,6 +144,11 @@ int t3mi_paged_attention(const t3mi_paged_cache* cache, const t3mi_attention_arg
     int rc = take_attention(me, cache, args, o);
     if (rc) return rc;
     if (o.rows == 0) return T3MI_OK;
+    t3k::plan_paged_attention(o);
+    const size_t need = t3k::paged_attention_workspace(o);
+    if (need > 0 && (!args->workspace || !at16(args->workspace) || args->workspace_bytes < need))
+        return bad(me, "the workspace is smaller than t3mi_paged_attention_workspace says, or not aligned to 16 bytes");
+    o.ws = static_cast<float*>(args->workspace);
     OnDevice dev(cache->device);
     if (dev.err != hipSuccess) return done(me, dev.err);
     return done(me, t3k::launch_paged_attention(o, (hipStream_t)stream));

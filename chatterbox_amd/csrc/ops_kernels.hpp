@@ -46,6 +46,11 @@ struct PagedAttnArgs {
     const int* seq = nullptr;     // [rows] block-table row, or nullptr: identity
     float scale = 1.f;
     int rows = 0, q_heads = 0, q_bf16 = 0, out_bf16 = 0, max_length = 0, length_add = 0;
+    // filled by plan_paged_attention
+    int n_split = 1;              // blocks a row's keys are shared by at most
+    int min_tiles = 1;            // 32-key tiles that are worth a block
+    int waves = 4;                // waves of a block
+    float* ws = nullptr;          // n_split > 1: [rows * q_heads * n_split] partial results of head_dim floats, then as many (max, sum)
 };
 
 struct LogitsArgs {
@@ -73,6 +78,9 @@ struct LogitsArgs {
 
 // all launches are asynchronous on `s`, on the current device
 hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s);
+// how a call is cut into blocks, from its sizes and types alone; the workspace that takes
+void plan_paged_attention(PagedAttnArgs& a);
+size_t paged_attention_workspace(const PagedAttnArgs& a);
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s);
 hipError_t launch_process_logits(const LogitsArgs& a, hipStream_t s);
 

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "ops_kernels.hpp"
 
@@ -76,35 +77,406 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
     }
 }
 
-// one wave per (row, query head): keys one after the other, a running maximum and sum (the softmax in one pass)
-template <typename QT, typename KV, typename OT>
-__global__ __launch_bounds__(64) void paged_attention_kernel(PagedAttnArgs a) {
-    const int row = blockIdx.x / a.q_heads, h = blockIdx.x % a.q_heads, lane = threadIdx.x;
-    const int hk = h / (a.q_heads / a.c.kv_heads), per = a.c.head_dim >> 6;
-    int n = a.lengths[row];
-    if (n < 0) return;
-    n += a.length_add;
-    const long long most = (long long)a.c.max_pages << a.c.page_shift;
-    if (n > most) n = (int)most;
-    const int s = a.seq ? a.seq[row] : row;
-    if (s < 0 || s >= a.c.n_seqs) n = 0;
-    const int first = a.starts ? max(a.starts[row], 0) : 0;
-    float q[2] = {0.f, 0.f}, acc[2] = {0.f, 0.f}, m = -INFINITY, l = 0.f;
-    for (int e = 0; e < per; ++e) q[e] = load1<QT>(a.q, row * a.qr + h * a.qh + e * 64 + lane);
-    for (int j = first; j < n; ++j) {
-        const int page = page_of(a.c, s, j);
-        if (page < 0) continue;
-        const int slot = j & ((1 << a.c.page_shift) - 1);
-        float dot = 0.f;
-        for (int e = 0; e < per; ++e) dot += q[e] * load1<KV>(a.c.k, page * a.c.kp + slot * a.c.ks + hk * a.c.kh + e * 64 + lane);
-        for (int o = 32; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
-        dot *= a.scale;
-        const float mn = fmaxf(m, dot), ref = mn > -INFINITY ? mn : 0.f, keep = expf(m - ref), p = expf(dot - ref);
-        l = l * keep + p;
-        for (int e = 0; e < per; ++e) acc[e] = acc[e] * keep + p * load1<KV>(a.c.v, page * a.c.vp + slot * a.c.vs + hk * a.c.vh + e * 64 + lane);
-        m = mn;
+// four neighbouring results of a head: the weighted sum over the sum of weights, zero where no key was seen
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void store_out(const PagedAttnArgs& a, int row, int h, int d, f32x4 o, float sum) {
+    const long long at = (long long)row * a.outr + (long long)h * a.outh + d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = sum == 0.f ? 0.f : o[i] / sum;
+    if (a.out_bf16) {
+        const uint2 w = {(unsigned)to_bf16(o[0]) | (unsigned)to_bf16(o[1]) << 16, (unsigned)to_bf16(o[2]) | (unsigned)to_bf16(o[3]) << 16};
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = w;
+    } else {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + at) = o;
     }
-    for (int e = 0; e < per; ++e) store1<OT>(a.out, row * a.outr + h * a.outh + e * 64 + lane, l > 0.f ? acc[e] / l : 0.f);
+}
+
+// ---- attention -----------------------------------------------------------------------------------------------------------------
+// o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(x_j - max x),  x_j = scale log2(e) q . k_j.  Bound: every live key and value is read once from
+// HBM (4 G flop for each pair of elements, G query heads to a key head: far below the matrix rate), so the kernel is built around loads.
+// A wave takes 32 keys at a time of one key head for up to 16 of its query heads:
+//   S^T = K Q^T   (A: 16 keys x head_dim, straight from memory to the registers the matrix instruction takes; B: the queries, resident)
+//   O^T += V^T P  (B: the 8 weights a lane holds after the softmax are already its operand: lane (query n, group g) has keys 4 g + i of both
+//                  16-key tiles, and the sum over keys may run in any order; A: a lane loads D / 16 neighbouring values of each of
+//                  these 8 keys -- whole rows of the cache to an instruction -- and turns the 8 x D/16 block in its registers)
+// so neither K nor V passes through LDS.  The next 32 keys are requested as soon as their registers are free: keys after the first
+// product, values after the second, one tile in flight per wave all the time.  Waves of a block take every nw-th tile and meet in LDS;
+// blocks of a row (split) leave (max, sum, weighted sum) in the workspace for paged_join_kernel.
+// Types: bf16 operands go to the bf16 matrix instruction.  An fp32 query over a bf16 cache is cut into three bf16 parts of 8 significant
+// bits each, which hold it exactly, and so are the weights when the result is fp32; a bf16 result rounds each weight to bf16 (the
+// result is rounded as coarsely).  An fp32 cache uses the exact fp32 matrix instruction.  Sums, maxima and products: fp32.
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+// over the four 16-lane groups of a wave (lanes n, n + 16, n + 32, n + 48), by register swaps
+template <typename F> __device__ __forceinline__ float over_groups(float x, F f) {
+    const unsigned u = __float_as_uint(x);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned w = __float_as_uint(f(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    const auto b = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float group_max(float x) { return over_groups(x, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ float group_sum(float x) { return over_groups(x, [](float a, float b) { return a + b; }); }
+
+// the leading 8 significant bits of x; what is left over is x - lead(x), exactly
+__device__ __forceinline__ float lead(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
+
+// eight floats as PARTS bf16 vectors: rounded (1), or cut into three parts that hold them exactly (3)
+template <int PARTS> __device__ __forceinline__ void to_parts(const float (&x)[8], bf16x8 (&o)[PARTS]) {
+    if constexpr (PARTS == 1) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[0][j] = (__bf16)x[j];
+    } else {
+        float r[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = x[j];
+#pragma unroll
+        for (int s = 0; s < PARTS; ++s) {
+            u32x4 w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = __builtin_amdgcn_perm(__float_as_uint(r[2 * j + 1]), __float_as_uint(r[2 * j]), 0x07060302u);
+                if (s + 1 < PARTS) {
+                    r[2 * j] -= lead(r[2 * j]);
+                    r[2 * j + 1] -= lead(r[2 * j + 1]);
+                }
+            }
+            o[s] = __builtin_bit_cast(bf16x8, w);
+        }
+    }
+}
+
+// which keys of a row a block works on: key tiles [t0, t1) of 32, shared by `active` blocks of at most `per` tiles each
+struct RowPlan {
+    int first, len, t0, t1, per, active;
+};
+__device__ __forceinline__ RowPlan plan_row(const PagedAttnArgs& a, int row, int s) {
+    RowPlan p;
+    long long n = (long long)a.lengths[row] + a.length_add;
+    const long long most = (long long)a.c.max_pages << a.c.page_shift;
+    n = n > most ? most : n;
+    p.first = a.starts ? max(a.starts[row], 0) : 0;
+    p.len = (s < 0 || s >= a.c.n_seqs) ? 0 : (int)n;
+    p.t0 = p.first >> 5;
+    p.t1 = (p.len + 31) >> 5;
+    const int tiles = p.len > p.first ? p.t1 - p.t0 : 0;
+    if (tiles == 0) p.t1 = p.t0;
+    const int want = min(a.n_split, (tiles + a.min_tiles - 1) / a.min_tiles);
+    p.per = want > 0 ? (tiles + want - 1) / want : 1;
+    p.active = tiles > 0 ? (tiles + p.per - 1) / p.per : 1;
+    return p;
+}
+
+// QB, KB: bf16 queries, bf16 cache.  PAGES 0: pages of 32 keys and more (a tile lies in one), 1: of 4, 8, 16, 2: of 1, 2.
+// PARTS: bf16 parts of a weight (bf16 cache only).
+template <bool QB, bool KB, int D, int PAGES, int PARTS>
+__global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) float sm[];
+    constexpr int EB = KB ? 2 : 4;                  // bytes of a cache element
+    constexpr int KC = KB ? D / 32 : D / 16;        // 16-byte pieces of a key to a lane
+    constexpr int VL = KB ? 1 : D / 64;             // loads of a value to a lane: D / 16 bf16 in one, or 4 floats of each 64
+    constexpr int NT = D / 16;                      // 16 x 16 tiles of O^T
+    constexpr int QS = QB ? 1 : 3;
+    using VT = std::conditional_t<KB && D == 64, u32x2, u32x4>;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
+    const int group = a.q_heads / a.c.kv_heads, gt = (group + 15) >> 4;
+    const unsigned split = blockIdx.x % (unsigned)a.n_split;
+    unsigned pair = blockIdx.x / (unsigned)a.n_split;
+    const int q16 = (int)(pair % (unsigned)gt);
+    pair /= (unsigned)gt;
+    const int hk = (int)(pair % (unsigned)a.c.kv_heads), row = (int)(pair / (unsigned)a.c.kv_heads);
+    if (a.lengths[row] < 0) return;
+    const int seq = a.seq ? a.seq[row] : row;
+    const RowPlan rp = plan_row(a, row, seq);
+    if ((int)split >= rp.active) return;
+    const int gn = min(16, group - q16 * 16);       // live query heads of this block
+    const int h0 = hk * group + q16 * 16;
+    const int t_begin = rp.t0 + (int)split * rp.per, t_end = min(rp.t1, t_begin + rp.per);
+
+    // queries: lane (n, g) holds, for piece c, elements 32 c + 8 g + j (bf16 cache) or 16 c + 4 g + i (fp32 cache) of head n
+    bf16x8 qb[KB ? QS : 1][KB ? KC : 1];
+    f32x4 qf[KB ? 1 : KC];
+    {
+        const bool live = n < gn;
+        const long long qo = row * a.qr + (long long)(h0 + (live ? n : 0)) * a.qh;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            if constexpr (QB) {
+                u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + qo + 32 * c + 8 * g);
+                if (!live) w = u32x4{0u, 0u, 0u, 0u};
+                qb[0][c] = __builtin_bit_cast(bf16x8, w);
+            } else if constexpr (KB) {
+                const float* qp = static_cast<const float*>(a.q) + qo + 32 * c + 8 * g;
+                const f32x4 lo = *reinterpret_cast<const f32x4*>(qp), hi = *reinterpret_cast<const f32x4*>(qp + 4);
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { x[j] = live ? lo[j] : 0.f; x[4 + j] = live ? hi[j] : 0.f; }
+                bf16x8 o[3];
+                to_parts<3>(x, o);
+#pragma unroll
+                for (int s = 0; s < QS; ++s) qb[s][c] = o[s];
+            } else {
+                f32x4 w = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + qo + 16 * c + 4 * g);
+                if (!live) w = f32x4{0.f, 0.f, 0.f, 0.f};
+                qf[c] = w;
+            }
+        }
+    }
+
+    // byte offsets of this lane inside a tile: keys 16 t + n, piece g; values of keys 16 t + 4 g + i, elements D / 16 * n (or 4 n)
+    const unsigned ksb = (unsigned)a.c.ks * EB, vsb = (unsigned)a.c.vs * EB;
+    const char* kbase = static_cast<const char*>(a.c.k) + (long long)hk * a.c.kh * EB;
+    const char* vbase = static_cast<const char*>(a.c.v) + (long long)hk * a.c.vh * EB;
+    const int* trow = a.c.table + (long long)(seq < 0 || seq >= a.c.n_seqs ? 0 : seq) * a.c.table_stride;
+    const int in_page = (1 << a.c.page_shift) - 1;
+    constexpr int NP = PAGES == 0 ? 1 : (PAGES == 1 ? 4 : 10);   // page numbers of a tile: one; K and V of both 16s; K of both, V of 8 keys
+    // key of page number x of tile t (clamped to the row's last: entries past it may hold anything)
+    auto key_of = [&](int t, int x) {
+        int k = t * 32;
+        if (PAGES == 1) k += x < 2 ? 16 * x + n : 16 * (x - 2) + 4 * g;
+        if (PAGES == 2) k += x < 2 ? 16 * x + n : 16 * ((x - 2) >> 2) + 4 * g + ((x - 2) & 3);
+        return PAGES == 0 ? k : min(k, rp.len - 1);
+    };
+    int ids[NP];
+    auto ask = [&](int t) {
+#pragma unroll
+        for (int x = 0; x < NP; ++x) ids[x] = trow[key_of(t, x) >> a.c.page_shift];
+    };
+    u32x4 kr[2][KC];
+    VT vr[8][VL];
+    // what the loads of a tile need: page numbers clamped into the pool, and whether they were in it
+    struct Pages { int id[NP]; bool ok; };
+    auto settle = [&]() {
+        Pages p;
+        p.ok = true;
+#pragma unroll
+        for (int x = 0; x < NP; ++x) {
+            const bool in = ids[x] >= 0 && ids[x] < a.c.n_pages;
+            p.id[x] = in ? ids[x] : 0;
+            p.ok &= in;
+        }
+        return p;
+    };
+    auto load_k = [&](int t, const Pages& p) {
+        if constexpr (PAGES == 0) {
+            const char* base = kbase + ((long long)p.id[0] * a.c.kp + (long long)((t * 32) & in_page) * a.c.ks) * EB;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int c = 0; c < KC; ++c) kr[u][c] = *reinterpret_cast<const u32x4*>(base + (unsigned)((16 * u + n) * ksb + 64 * c + 16 * g));
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int slot = key_of(t, u) & in_page;
+                const char* base = kbase + ((long long)p.id[u] * a.c.kp + (long long)slot * a.c.ks) * EB + 16 * g;
+#pragma unroll
+                for (int c = 0; c < KC; ++c) kr[u][c] = *reinterpret_cast<const u32x4*>(base + 64 * c);
+            }
+        }
+    };
+    auto load_v = [&](int t, const Pages& p) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (PAGES == 0) {
+                const char* base = vbase + ((long long)p.id[0] * a.c.vp + (long long)((t * 32) & in_page) * a.c.vs) * EB;
+#pragma unroll
+                for (int h = 0; h < VL; ++h)
+                    vr[j][h] = *reinterpret_cast<const VT*>(base + (unsigned)((16 * (j >> 2) + 4 * g + (j & 3)) * vsb + 256 * h + (unsigned)sizeof(VT) * n));
+            } else {
+                const int x = PAGES == 1 ? 2 + (j >> 2) : 2 + j;
+                const int key = min(t * 32 + 16 * (j >> 2) + 4 * g + (j & 3), rp.len - 1);
+                // (PAGES 1: keys 4 g .. 4 g + 3 share a page; a clamped key may not, and then only its slot has to be inside)
+                const int slot = key & in_page;
+                const char* base = vbase + ((long long)p.id[x] * a.c.vp + (long long)slot * a.c.vs) * EB + sizeof(VT) * n;
+#pragma unroll
+                for (int h = 0; h < VL; ++h) vr[j][h] = *reinterpret_cast<const VT*>(base + 256 * h);
+            }
+        }
+    };
+
+    f32x4 acc[NT];
+#pragma unroll
+    for (int e = 0; e < NT; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    const float scale2 = a.scale * 1.4426950408889634f;
+    int t = t_begin + wave;
+    if (t < t_end) {
+        // page numbers are asked for one tile before the loads that need them, so that nothing waits for them
+        ask(t);
+        Pages pg = settle();
+        ask(min(t + nw, t_end - 1));
+        load_k(t, pg);
+        load_v(t, pg);
+        while (true) {
+            const int t_next = min(t + nw, t_end - 1);   // (past the end: a tile that is asked for again, from L2, and not used)
+            f32x4 s[2];
+            s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (KB) {
+#pragma unroll
+                for (int part = QS - 1; part >= 0; --part)   // small parts first
+#pragma unroll
+                    for (int c = 0; c < KC; ++c)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[u][c]), qb[part][c], s[u], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, kr[u][c])[i], qf[c][i], s[u], 0, 0, 0);
+            }
+            const Pages next = settle();
+            ask(min(t + 2 * nw, t_end - 1));
+            load_k(t_next, next);
+            // softmax: x = scores in units of log2, keys 32 t + 16 u + 4 g + i of head n
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = s[j >> 2][j & 3] * scale2;
+            const bool whole = t * 32 >= rp.first && t * 32 + 32 <= rp.len;
+            bool all_in = true;
+            if constexpr (PAGES == 0) all_in = pg.ok;
+            else all_in = __builtin_amdgcn_ballot_w64(!pg.ok) == 0;
+            if (!(whole && all_in)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int key = t * 32 + 16 * (j >> 2) + 4 * g + (j & 3);
+                    bool live = key >= rp.first && key < rp.len;
+                    if (!all_in) {
+                        const int id = key < rp.len ? trow[key >> a.c.page_shift] : -1;
+                        live = live && id >= 0 && id < a.c.n_pages;
+                    }
+                    p[j] = live ? p[j] : -INFINITY;
+#pragma unroll
+                    for (int h = 0; h < VL; ++h)
+#pragma unroll
+                        for (int w = 0; w < (int)(sizeof(VT) / 4); ++w) vr[j][h][w] = live ? vr[j][h][w] : 0u;   // what is there may be NaN
+                }
+            }
+            float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+            mx = fmaxf(m, group_max(mx));
+            const float ref = mx > -INFINITY ? mx : 0.f;
+            if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
+                const float keep = __builtin_amdgcn_exp2f(m - ref);
+                l *= keep;
+#pragma unroll
+                for (int e = 0; e < NT; ++e) acc[e] *= keep;
+                m = mx;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(p[j] - ref);
+            l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            if constexpr (KB) {
+                bf16x8 pb[PARTS];
+                to_parts<PARTS>(p, pb);
+#pragma unroll
+                for (int e = 0; e < NT; ++e) {
+                    u32x4 w;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        w[j] = __builtin_amdgcn_perm(vr[2 * j + 1][0][e >> 1], vr[2 * j][0][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
+                    const bf16x8 av = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+                    for (int part = PARTS - 1; part >= 0; --part) acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, pb[part], acc[e], 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int e = 0; e < NT; ++e)
+                        acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[j][e >> 2][e & 3]), p[j], acc[e], 0, 0, 0);
+            }
+            load_v(t_next, next);
+            t += nw;
+            if (t >= t_end) break;
+            pg = next;
+        }
+    }
+    l = group_sum(l);
+
+    // the waves meet in LDS: maxima and sums [nw][16], then the weighted sums [nw][gn][D].  Lane (n, g) holds for head n the elements of
+    // row 4 g + i of tile e: D / 16 (4 g + i) + e with a bf16 cache, 64 (e / 4) + 4 (4 g + i) + e % 4 with an fp32 one
+    float* sm_m = sm;
+    float* sm_l = sm + nw * 16;
+    float* sm_o = sm + nw * 32;
+    if (lane < 16) {
+        sm_m[wave * 16 + n] = m;
+        sm_l[wave * 16 + n] = l;
+    }
+    __syncthreads();
+    float top = -INFINITY;
+    for (int w = 0; w < nw; ++w) top = fmaxf(top, sm_m[w * 16 + n]);
+    if (n < gn) {
+        const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.f;
+        float* o = sm_o + (wave * gn + n) * D;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < NT; e += 4) {
+                const f32x4 v = f32x4{acc[e][i], acc[e + 1][i], acc[e + 2][i], acc[e + 3][i]} * f;
+                const int at = KB ? NT * (4 * g + i) + e : 64 * (e >> 2) + 4 * (4 * g + i);
+                *reinterpret_cast<f32x4*>(o + at) = v;
+            }
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < gn * (D / 4); x += blockDim.x) {
+        const int hn = x / (D / 4), d4 = (x % (D / 4)) * 4;
+        float big = -INFINITY, sum = 0.f;
+        for (int w = 0; w < nw; ++w) big = fmaxf(big, sm_m[w * 16 + hn]);
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < nw; ++w) {
+            const float mw = sm_m[w * 16 + hn];
+            sum += mw > -INFINITY ? sm_l[w * 16 + hn] * __builtin_amdgcn_exp2f(mw - big) : 0.f;
+            o += *reinterpret_cast<const f32x4*>(sm_o + (w * gn + hn) * D + d4);
+        }
+        if (rp.active > 1) {
+            const long long part = ((long long)row * a.q_heads + h0 + hn) * a.n_split + split;
+            *reinterpret_cast<f32x4*>(a.ws + part * D + d4) = o;
+            if (d4 == 0) *reinterpret_cast<float2*>(a.ws + (long long)a.rows * a.q_heads * a.n_split * D + part * 2) = float2{big, sum};
+        } else {
+            store_out(a, row, h0 + hn, d4, o, sum);
+        }
+    }
+}
+
+// one block per (row, query head): the row's partial results joined in a fixed order
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
+    constexpr int LP = D / 4, NS = 256 / LP;        // threads of a partial, partials at a time
+    __shared__ __attribute__((aligned(16))) float sm_o[NS][D];
+    __shared__ float sm_l[NS];
+    const int row = blockIdx.x / a.q_heads, h = blockIdx.x % a.q_heads, tid = threadIdx.x;
+    if (a.lengths[row] < 0) return;
+    const RowPlan rp = plan_row(a, row, a.seq ? a.seq[row] : row);
+    if (rp.active <= 1) return;
+    const long long part = (long long)blockIdx.x * a.n_split;
+    const float* ml = a.ws + (long long)a.rows * a.q_heads * a.n_split * D + part * 2;
+    float big = -INFINITY;
+    for (int s = 0; s < rp.active; ++s) big = fmaxf(big, ml[2 * s]);
+    const int sub = tid / LP, d4 = (tid % LP) * 4;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+#pragma unroll 4
+    for (int s = sub; s < rp.active; s += NS) {
+        const float2 x = *reinterpret_cast<const float2*>(ml + 2 * s);
+        const float f = x.x > -INFINITY ? __builtin_amdgcn_exp2f(x.x - big) : 0.f;
+        o += *reinterpret_cast<const f32x4*>(a.ws + (part + s) * D + d4) * f;
+        sum += x.y * f;
+    }
+    *reinterpret_cast<f32x4*>(&sm_o[sub][d4]) = o;
+    if (d4 == 0) sm_l[sub] = sum;
+    __syncthreads();
+    if (sub == 0) {
+        for (int x = 1; x < NS; ++x) {
+            o += *reinterpret_cast<const f32x4*>(&sm_o[x][d4]);
+            sum += sm_l[x];
+        }
+        store_out(a, row, h, d4, o, sum);
+    }
 }
 
 }  // namespace
@@ -120,18 +492,53 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <typename QT, typename KV>
-static void launch_attention_o(const PagedAttnArgs& a, hipStream_t s) {
-    const dim3 grid((unsigned)(a.rows * a.q_heads)), block(64);
-    if (a.out_bf16) hipLaunchKernelGGL((paged_attention_kernel<QT, KV, uint16_t>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((paged_attention_kernel<QT, KV, float>), grid, block, 0, s, a);
+namespace {
+
+template <bool QB, bool KB, int D, int PARTS>
+void launch_attention_p(const PagedAttnArgs& a, unsigned blocks, unsigned threads, size_t lds, hipStream_t s) {
+    const dim3 grid(blocks), block(threads);
+    if (a.c.page_shift >= 5) hipLaunchKernelGGL((paged_attention_kernel<QB, KB, D, 0, PARTS>), grid, block, lds, s, a);
+    else if (a.c.page_shift >= 2) hipLaunchKernelGGL((paged_attention_kernel<QB, KB, D, 1, PARTS>), grid, block, lds, s, a);
+    else hipLaunchKernelGGL((paged_attention_kernel<QB, KB, D, 2, PARTS>), grid, block, lds, s, a);
+}
+template <int D>
+void launch_attention_d(const PagedAttnArgs& a, unsigned blocks, unsigned threads, size_t lds, hipStream_t s) {
+    if (!a.c.bf16) launch_attention_p<false, false, D, 1>(a, blocks, threads, lds, s);
+    else if (a.q_bf16 && a.out_bf16) launch_attention_p<true, true, D, 1>(a, blocks, threads, lds, s);
+    else if (a.q_bf16) launch_attention_p<true, true, D, 3>(a, blocks, threads, lds, s);
+    else if (a.out_bf16) launch_attention_p<false, true, D, 1>(a, blocks, threads, lds, s);
+    else launch_attention_p<false, true, D, 3>(a, blocks, threads, lds, s);
+    if (a.n_split > 1) hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)(a.rows * a.q_heads)), dim3(256), 0, s, a);
+}
+
+}  // namespace
+
+void plan_paged_attention(PagedAttnArgs& a) {
+    const int group = a.q_heads / a.c.kv_heads;
+    const long long pairs = (long long)a.rows * a.c.kv_heads * ((group + 15) / 16);
+    const int tiles = (a.max_length + 31) / 32;
+    a.waves = 4;
+    a.min_tiles = 2 * a.waves;
+    long long n = (2048 + pairs - 1) / pairs;
+    n = n > 128 ? 128 : n;
+    const long long most = (tiles + a.min_tiles - 1) / a.min_tiles;
+    a.n_split = (int)(n < most ? n : most);
+    if (a.n_split < 1) a.n_split = 1;
+}
+
+size_t paged_attention_workspace(const PagedAttnArgs& a) {
+    return a.n_split <= 1 ? 0 : (size_t)a.rows * a.q_heads * a.n_split * (a.c.head_dim + 2) * 4;
 }
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s) {
-    if (a.rows <= 0 || (long long)a.rows * a.q_heads > 0x7FFFFFFFLL) return hipErrorInvalidValue;
-    if (a.q_bf16) launch_attention_o<uint16_t, uint16_t>(a, s);
-    else if (a.c.bf16) launch_attention_o<float, uint16_t>(a, s);
-    else launch_attention_o<float, float>(a, s);
+    const int group = a.q_heads / a.c.kv_heads;
+    const long long blocks = (long long)a.rows * a.c.kv_heads * ((group + 15) / 16) * a.n_split;
+    if (a.rows <= 0 || a.n_split < 1 || a.min_tiles < 1 || a.waves < 1 || a.waves > 4 || blocks > 0x7FFFFFFFLL) return hipErrorInvalidValue;
+    if (a.n_split > 1 && a.ws == nullptr) return hipErrorInvalidValue;
+    const size_t lds = (size_t)a.waves * (32 + (size_t)(group < 16 ? group : 16) * a.c.head_dim) * 4;
+    if (a.c.head_dim == 64) launch_attention_d<64>(a, (unsigned)blocks, 64u * a.waves, lds, s);
+    else if (a.c.head_dim == 128) launch_attention_d<128>(a, (unsigned)blocks, 64u * a.waves, lds, s);
+    else return hipErrorInvalidValue;
     return hipGetLastError();
 }
 
