@@ -113,7 +113,7 @@ int t3mi_paged_append(const t3mi_paged_cache* cache, const t3mi_append_args* a, 
     if (a->q && a->q == a->q_out && (a->q_stride[0] != a->q_out_stride[0] || a->q_stride[1] != a->q_out_stride[1]))
         return bad(me, "q_out may be q only with the same strides");
     if (!a->seq && a->rows > cache->n_seqs) return bad(me, "more rows than sequences (seq says which row belongs to which)");
-    if ((int64_t)a->rows * ((a->q ? a->q_heads : 0) + 2LL * cache->kv_heads) > 0x10000000LL) return bad(me, "at most 2^28 (row, head) pairs a call");
+    if ((int64_t)a->rows * ((a->q ? a->q_heads : 0) + 2LL * cache->kv_heads) > 0x8000000LL) return bad(me, "at most 2^27 (row, head) pairs a call");
     if (a->rows == 0) return T3MI_OK;
     o.k = a->k; o.v = a->v; o.q = a->q; o.q_out = a->q_out;
     o.kr = a->k_stride[0]; o.kh = a->k_stride[1]; o.vr = a->v_stride[0]; o.vh = a->v_stride[1];

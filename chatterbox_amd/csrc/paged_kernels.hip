@@ -18,13 +18,36 @@ __device__ __forceinline__ uint16_t to_bf16(float f) {
 }
 __device__ __forceinline__ float from_bf16(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }
 
-template <typename T> __device__ __forceinline__ float load1(const void* p, long long i) {
-    if constexpr (sizeof(T) == 2) return from_bf16(static_cast<const uint16_t*>(p)[i]);
-    else return static_cast<const float*>(p)[i];
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));   // sixteen bytes at a float's address
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+// N neighbouring values as floats: 16 bytes of the type that comes in (N = 4 floats or 8 bf16), any type going out
+template <typename T, int N> __device__ __forceinline__ void load_row(const void* p, long long at, float (&x)[N]) {
+    if constexpr (sizeof(T) == 2) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+    } else {
+        const f32x4 w = *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = w[i];
+    }
 }
-template <typename T> __device__ __forceinline__ void store1(void* p, long long i, float v) {
-    if constexpr (sizeof(T) == 2) static_cast<uint16_t*>(p)[i] = to_bf16(v);
-    else static_cast<float*>(p)[i] = v;
+template <typename T, int N> __device__ __forceinline__ void store_row(void* p, long long at, const float (&x)[N]) {
+    if constexpr (sizeof(T) == 2) {
+        unsigned w[N / 2];
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) w[i] = (unsigned)to_bf16(x[2 * i]) | (unsigned)to_bf16(x[2 * i + 1]) << 16;
+        uint16_t* o = static_cast<uint16_t*>(p) + at;
+        if constexpr (N == 8) *reinterpret_cast<u32x4*>(o) = u32x4{w[0], w[1], w[2], w[3]};
+        else *reinterpret_cast<u32x2*>(o) = u32x2{w[0], w[1]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<f32x4*>(static_cast<float*>(p) + at + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+    }
 }
 
 // page of key j of sequence s, or -1: outside the table, or an entry that names no page of the pool
@@ -35,50 +58,63 @@ __device__ __forceinline__ int page_of(const PagedCache& c, int s, int j) {
     return p >= 0 && p < c.n_pages ? p : -1;
 }
 
-// one thread per element pair (i, i + head_dim / 2) of a head of q, k or v:  (a, b) -> (a cos - b sin, b cos + a sin)
-template <typename IN, typename KV>
+// A thread takes 16 bytes of the first half of a head of q, k or v and the 16 bytes that turn with them in the second half:
+// (a, b) -> (a cos - b sin, b cos + a sin) in fp32, rounded once.  Bound: every value is read and written once; the angles come from
+// L2 (the heads of a row share them), so the kernel is a copy with a permutation of rows.
+template <typename IN, typename KV, int D>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
-    const int half = a.c.head_dim >> 1;
-    const int heads = (a.q ? a.q_heads : 0) + 2 * a.c.kv_heads;
-    const long long per_row = (long long)heads * half, total = per_row * a.rows;
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (idx >= total) return;
-    const int row = (int)(idx / per_row), rem = (int)(idx % per_row);
-    int head = rem / half;
-    const int i = rem % half;
-    const int pos = a.positions[row], s = a.seq ? a.seq[row] : row;
+    constexpr int N = 16 / sizeof(IN), H = D / 2, UN = H / N;   // values of a piece, of a half, pieces of a half
+    const unsigned heads = (unsigned)(a.q_heads + 2 * a.c.kv_heads);
+    const unsigned idx = blockIdx.x * 256u + threadIdx.x;
+    const unsigned hr = idx / UN;
+    const int i = (int)(idx % UN) * N;
+    const unsigned row = hr / heads;
+    if (row >= (unsigned)a.rows) return;
+    int head = (int)(hr - row * heads);
+    const int pos = a.positions[row], s = a.seq ? a.seq[row] : (int)row;
     if (pos < 0 || s < 0 || s >= a.c.n_seqs || (a.cos && pos >= a.rope_len)) return;
     const int page = page_of(a.c, s, pos);
     if (page < 0) return;
     const int slot = pos & ((1 << a.c.page_shift) - 1);
-    const bool is_v = head >= heads - a.c.kv_heads;
-    float c = 1.f, sn = 0.f;
-    if (a.cos && !is_v) {
-        c = a.cos[pos * a.rope_stride + i];
-        sn = a.sin[pos * a.rope_stride + i];
-    }
-    const int qn = a.q ? a.q_heads : 0;
-    if (head < qn) {
-        const long long o = row * a.qr + head * a.qh + i, w = row * a.qor + head * a.qoh + i;
-        const float x = load1<IN>(a.q, o), y = load1<IN>(a.q, o + half);
-        store1<IN>(a.q_out, w, x * c - y * sn);
-        store1<IN>(a.q_out, w + half, y * c + x * sn);
-    } else if (!is_v) {
-        head -= qn;
-        const long long o = row * a.kr + head * a.kh + i, w = page * a.c.kp + slot * a.c.ks + head * a.c.kh + i;
-        const float x = load1<IN>(a.k, o), y = load1<IN>(a.k, o + half);
-        store1<KV>(a.c.k, w, x * c - y * sn);
-        store1<KV>(a.c.k, w + half, y * c + x * sn);
-    } else {
-        head -= qn + a.c.kv_heads;
+    float x[N], y[N];
+    if (head >= a.q_heads + a.c.kv_heads) {
+        head -= a.q_heads + a.c.kv_heads;
         const long long o = row * a.vr + head * a.vh + i, w = page * a.c.vp + slot * a.c.vs + head * a.c.vh + i;
-        store1<KV>(a.c.v, w, load1<IN>(a.v, o));
-        store1<KV>(a.c.v, w + half, load1<IN>(a.v, o + half));
+        load_row<IN, N>(a.v, o, x);
+        load_row<IN, N>(a.v, o + H, y);
+        store_row<KV, N>(a.c.v, w, x);
+        store_row<KV, N>(a.c.v, w + H, y);
+        return;
+    }
+    const bool is_q = head < a.q_heads;
+    if (!is_q) head -= a.q_heads;
+    const long long o = is_q ? row * a.qr + head * a.qh + i : row * a.kr + head * a.kh + i;
+    load_row<IN, N>(is_q ? a.q : a.k, o, x);
+    load_row<IN, N>(is_q ? a.q : a.k, o + H, y);
+    if (a.cos) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+            const f32x4 c = *reinterpret_cast<const f32x4u*>(a.cos + pos * a.rope_stride + i + e), sn = *reinterpret_cast<const f32x4u*>(a.sin + pos * a.rope_stride + i + e);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float p = x[e + k], r = y[e + k];
+                x[e + k] = p * c[k] - r * sn[k];
+                y[e + k] = r * c[k] + p * sn[k];
+            }
+        }
+    }
+    if (is_q) {
+        const long long w = row * a.qor + head * a.qoh + i;
+        store_row<IN, N>(a.q_out, w, x);
+        store_row<IN, N>(a.q_out, w + H, y);
+    } else {
+        const long long w = page * a.c.kp + slot * a.c.ks + head * a.c.kh + i;
+        store_row<KV, N>(a.c.k, w, x);
+        store_row<KV, N>(a.c.k, w + H, y);
     }
 }
 
 // four neighbouring results of a head: the weighted sum over the sum of weights, zero where no key was seen
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void store_out(const PagedAttnArgs& a, int row, int h, int d, f32x4 o, float sum) {
     const long long at = (long long)row * a.outr + (long long)h * a.outh + d;
 #pragma unroll
@@ -105,10 +141,6 @@ __device__ __forceinline__ void store_out(const PagedAttnArgs& a, int row, int h
 // Types: bf16 operands go to the bf16 matrix instruction.  An fp32 query over a bf16 cache is cut into three bf16 parts of 8 significant
 // bits each, which hold it exactly, and so are the weights when the result is fp32; a bf16 result rounds each weight to bf16 (the
 // result is rounded as coarsely).  An fp32 cache uses the exact fp32 matrix instruction.  Sums, maxima and products: fp32.
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 // over the four 16-lane groups of a wave (lanes n, n + 16, n + 32, n + 48), by register swaps
 template <typename F> __device__ __forceinline__ float over_groups(float x, F f) {
@@ -481,15 +513,24 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
 
 }  // namespace
 
-hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
-    const long long total = (long long)a.rows * ((a.q ? a.q_heads : 0) + 2 * a.c.kv_heads) * (a.c.head_dim / 2);
-    if (a.rows <= 0 || (total + 255) / 256 > 0x7FFFFFFFLL) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)((total + 255) / 256)), block(256);
-    if (a.in_bf16 && a.c.bf16) hipLaunchKernelGGL((paged_append_kernel<uint16_t, uint16_t>), grid, block, 0, s, a);
-    else if (a.in_bf16) hipLaunchKernelGGL((paged_append_kernel<uint16_t, float>), grid, block, 0, s, a);
-    else if (a.c.bf16) hipLaunchKernelGGL((paged_append_kernel<float, uint16_t>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((paged_append_kernel<float, float>), grid, block, 0, s, a);
+namespace {
+
+template <typename IN, typename KV> hipError_t launch_append_t(const PagedAppendArgs& a, hipStream_t s) {
+    const long long threads = (long long)a.rows * (a.q_heads + 2 * a.c.kv_heads) * (a.c.head_dim / 2) * (long long)sizeof(IN) / 16;
+    if (threads > 0xFFFFFF00LL) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
+    if (a.c.head_dim == 64) hipLaunchKernelGGL((paged_append_kernel<IN, KV, 64>), grid, block, 0, s, a);
+    else if (a.c.head_dim == 128) hipLaunchKernelGGL((paged_append_kernel<IN, KV, 128>), grid, block, 0, s, a);
+    else return hipErrorInvalidValue;
     return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
+    if (a.rows <= 0 || (a.q == nullptr) != (a.q_heads == 0)) return hipErrorInvalidValue;
+    if (a.in_bf16) return a.c.bf16 ? launch_append_t<uint16_t, uint16_t>(a, s) : launch_append_t<uint16_t, float>(a, s);
+    return a.c.bf16 ? launch_append_t<float, uint16_t>(a, s) : launch_append_t<float, float>(a, s);
 }
 
 namespace {
