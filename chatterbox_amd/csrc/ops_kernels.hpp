@@ -48,8 +48,10 @@ struct PagedAttnArgs {
     int rows = 0, q_heads = 0, q_bf16 = 0, out_bf16 = 0, max_length = 0, length_add = 0;
     // filled by plan_paged_attention
     int n_split = 1;              // blocks a row's keys are shared by at most
-    int min_tiles = 1;            // 32-key tiles that are worth a block
+    int tile_shift = 5;           // keys of a tile: 32, or 16 (fp32 cache)
+    int min_tiles = 1;            // tiles that are worth a block
     int waves = 4;                // waves of a block
+    int head_waves = 1;           // neighbouring key heads of a block (waves / head_waves share the keys of each)
     float* ws = nullptr;          // n_split > 1: [rows * q_heads * n_split] partial results of head_dim floats, then as many (max, sum)
 };
 

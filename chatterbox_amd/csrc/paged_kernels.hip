@@ -2,6 +2,7 @@
 // attention of new tokens' query rows over the pages.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -181,7 +182,9 @@ template <int PARTS> __device__ __forceinline__ void to_parts(const float (&x)[8
     }
 }
 
-// which keys of a row a block works on: key tiles [t0, t1) of 32, shared by `active` blocks of at most `per` tiles each
+constexpr int kMaxSplit = 64;      // blocks that share a row's keys at most
+
+// which keys of a row a block works on: key tiles [t0, t1) of 1 << tile_shift, shared by `active` blocks of at most `per` tiles each
 struct RowPlan {
     int first, len, t0, t1, per, active;
 };
@@ -192,8 +195,8 @@ __device__ __forceinline__ RowPlan plan_row(const PagedAttnArgs& a, int row, int
     n = n > most ? most : n;
     p.first = a.starts ? max(a.starts[row], 0) : 0;
     p.len = (s < 0 || s >= a.c.n_seqs) ? 0 : (int)n;
-    p.t0 = p.first >> 5;
-    p.t1 = (p.len + 31) >> 5;
+    p.t0 = p.first >> a.tile_shift;
+    p.t1 = (p.len + (1 << a.tile_shift) - 1) >> a.tile_shift;
     const int tiles = p.len > p.first ? p.t1 - p.t0 : 0;
     if (tiles == 0) p.t1 = p.t0;
     const int want = min(a.n_split, (tiles + a.min_tiles - 1) / a.min_tiles);
@@ -202,32 +205,38 @@ __device__ __forceinline__ RowPlan plan_row(const PagedAttnArgs& a, int row, int
     return p;
 }
 
-// QB, KB: bf16 queries, bf16 cache.  PAGES 0: pages of 32 keys and more (a tile lies in one), 1: of 4, 8, 16, 2: of 1, 2.
-// PARTS: bf16 parts of a weight (bf16 cache only).
-template <bool QB, bool KB, int D, int PAGES, int PARTS>
-__global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttnArgs a) {
+// QB, KB: bf16 queries, bf16 cache.  TK: keys of a tile, 32 or (fp32 cache) 16.  PAGES 0: pages of TK keys and more (a tile lies in one),
+// 1: smaller ones of 4 keys and more, 2: of 1, 2.  PARTS: bf16 parts of a weight (bf16 cache only).
+template <bool QB, bool KB, int D, int TK, int PAGES, int PARTS>
+__global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) float sm[];
     constexpr int EB = KB ? 2 : 4;                  // bytes of a cache element
     constexpr int KC = KB ? D / 32 : D / 16;        // 16-byte pieces of a key to a lane
     constexpr int VL = KB ? 1 : D / 64;             // loads of a value to a lane: D / 16 bf16 in one, or 4 floats of each 64
     constexpr int NT = D / 16;                      // 16 x 16 tiles of O^T
     constexpr int QS = QB ? 1 : 3;
+    constexpr int U = TK / 16, J = 4 * U;           // 16-key halves of a tile, weights to a lane
+    static_assert(TK == 32 || (TK == 16 && !KB), "the bf16 product takes 32 keys");
     using VT = std::conditional_t<KB && D == 64, u32x2, u32x4>;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    // waves: head_waves neighbouring key heads, and kw shares of each one's keys
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
-    const int group = a.q_heads / a.c.kv_heads, gt = (group + 15) >> 4;
+    const int hw = a.head_waves, wh = wave % hw, wk = wave / hw, kw = nw / hw;
+    const int group = a.q_heads / a.c.kv_heads, gt = (group + 15) >> 4, hg = (a.c.kv_heads + hw - 1) / hw;
     const unsigned split = blockIdx.x % (unsigned)a.n_split;
     unsigned pair = blockIdx.x / (unsigned)a.n_split;
     const int q16 = (int)(pair % (unsigned)gt);
     pair /= (unsigned)gt;
-    const int hk = (int)(pair % (unsigned)a.c.kv_heads), row = (int)(pair / (unsigned)a.c.kv_heads);
+    const int hk0 = (int)(pair % (unsigned)hg) * hw, row = (int)(pair / (unsigned)hg);
     if (a.lengths[row] < 0) return;
     const int seq = a.seq ? a.seq[row] : row;
     const RowPlan rp = plan_row(a, row, seq);
     if ((int)split >= rp.active) return;
-    const int gn = min(16, group - q16 * 16);       // live query heads of this block
+    const int gn = min(16, group - q16 * 16);       // live query heads of a key head in this block
+    const bool idle = hk0 + wh >= a.c.kv_heads;     // (a wave past the last key head: no tile, nothing stored)
+    const int hk = idle ? a.c.kv_heads - 1 : hk0 + wh;
     const int h0 = hk * group + q16 * 16;
-    const int t_begin = rp.t0 + (int)split * rp.per, t_end = min(rp.t1, t_begin + rp.per);
+    const int t_begin = rp.t0 + (int)split * rp.per, t_end = idle ? t_begin : min(rp.t1, t_begin + rp.per);
 
     // queries: lane (n, g) holds, for piece c, elements 32 c + 8 g + j (bf16 cache) or 16 c + 4 g + i (fp32 cache) of head n
     bf16x8 qb[KB ? QS : 1][KB ? KC : 1];
@@ -265,12 +274,12 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttnArgs a) {
     const char* vbase = static_cast<const char*>(a.c.v) + (long long)hk * a.c.vh * EB;
     const int* trow = a.c.table + (long long)(seq < 0 || seq >= a.c.n_seqs ? 0 : seq) * a.c.table_stride;
     const int in_page = (1 << a.c.page_shift) - 1;
-    constexpr int NP = PAGES == 0 ? 1 : (PAGES == 1 ? 4 : 10);   // page numbers of a tile: one; K and V of both 16s; K of both, V of 8 keys
+    constexpr int NP = PAGES == 0 ? 1 : (PAGES == 1 ? 2 * U : U + J);   // page numbers of a tile: one; K and V of each 16; K of each 16, V of each key
     // key of page number x of tile t (clamped to the row's last: entries past it may hold anything)
     auto key_of = [&](int t, int x) {
-        int k = t * 32;
-        if (PAGES == 1) k += x < 2 ? 16 * x + n : 16 * (x - 2) + 4 * g;
-        if (PAGES == 2) k += x < 2 ? 16 * x + n : 16 * ((x - 2) >> 2) + 4 * g + ((x - 2) & 3);
+        int k = t * TK;
+        if (PAGES == 1) k += x < U ? 16 * x + n : 16 * (x - U) + 4 * g;
+        if (PAGES == 2) k += x < U ? 16 * x + n : 16 * ((x - U) >> 2) + 4 * g + ((x - U) & 3);
         return PAGES == 0 ? k : min(k, rp.len - 1);
     };
     int ids[NP];
@@ -278,8 +287,8 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttnArgs a) {
 #pragma unroll
         for (int x = 0; x < NP; ++x) ids[x] = trow[key_of(t, x) >> a.c.page_shift];
     };
-    u32x4 kr[2][KC];
-    VT vr[8][VL];
+    u32x4 kr[U][KC];
+    VT vr[J][VL];
     // what the loads of a tile need: page numbers clamped into the pool, and whether they were in it
     struct Pages { int id[NP]; bool ok; };
     auto settle = [&]() {
@@ -295,14 +304,14 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttnArgs a) {
     };
     auto load_k = [&](int t, const Pages& p) {
         if constexpr (PAGES == 0) {
-            const char* base = kbase + ((long long)p.id[0] * a.c.kp + (long long)((t * 32) & in_page) * a.c.ks) * EB;
+            const char* base = kbase + ((long long)p.id[0] * a.c.kp + (long long)((t * TK) & in_page) * a.c.ks) * EB;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int c = 0; c < KC; ++c) kr[u][c] = *reinterpret_cast<const u32x4*>(base + (unsigned)((16 * u + n) * ksb + 64 * c + 16 * g));
         } else {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < U; ++u) {
                 const int slot = key_of(t, u) & in_page;
                 const char* base = kbase + ((long long)p.id[u] * a.c.kp + (long long)slot * a.c.ks) * EB + 16 * g;
 #pragma unroll
@@ -312,15 +321,15 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttnArgs a) {
     };
     auto load_v = [&](int t, const Pages& p) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < J; ++j) {
             if constexpr (PAGES == 0) {
-                const char* base = vbase + ((long long)p.id[0] * a.c.vp + (long long)((t * 32) & in_page) * a.c.vs) * EB;
+                const char* base = vbase + ((long long)p.id[0] * a.c.vp + (long long)((t * TK) & in_page) * a.c.vs) * EB;
 #pragma unroll
                 for (int h = 0; h < VL; ++h)
                     vr[j][h] = *reinterpret_cast<const VT*>(base + (unsigned)((16 * (j >> 2) + 4 * g + (j & 3)) * vsb + 256 * h + (unsigned)sizeof(VT) * n));
             } else {
-                const int x = PAGES == 1 ? 2 + (j >> 2) : 2 + j;
-                const int key = min(t * 32 + 16 * (j >> 2) + 4 * g + (j & 3), rp.len - 1);
+                const int x = PAGES == 1 ? U + (j >> 2) : U + j;
+                const int key = min(t * TK + 16 * (j >> 2) + 4 * g + (j & 3), rp.len - 1);
                 // (PAGES 1: keys 4 g .. 4 g + 3 share a page; a clamped key may not, and then only its slot has to be inside)
                 const int slot = key & in_page;
                 const char* base = vbase + ((long long)p.id[x] * a.c.vp + (long long)slot * a.c.vs) * EB + sizeof(VT) * n;
@@ -335,48 +344,49 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttnArgs a) {
     for (int e = 0; e < NT; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     const float scale2 = a.scale * 1.4426950408889634f;
-    int t = t_begin + wave;
+    int t = t_begin + wk;
     if (t < t_end) {
         // page numbers are asked for one tile before the loads that need them, so that nothing waits for them
         ask(t);
         Pages pg = settle();
-        ask(min(t + nw, t_end - 1));
+        ask(min(t + kw, t_end - 1));
         load_k(t, pg);
         load_v(t, pg);
         while (true) {
-            const int t_next = min(t + nw, t_end - 1);   // (past the end: a tile that is asked for again, from L2, and not used)
-            f32x4 s[2];
-            s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+            const int t_next = min(t + kw, t_end - 1);   // (past the end: a tile that is asked for again, from L2, and not used)
+            f32x4 s[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
             if constexpr (KB) {
 #pragma unroll
                 for (int part = QS - 1; part >= 0; --part)   // small parts first
 #pragma unroll
                     for (int c = 0; c < KC; ++c)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[u][c]), qb[part][c], s[u], 0, 0, 0);
+                        for (int u = 0; u < U; ++u) s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[u][c]), qb[part][c], s[u], 0, 0, 0);
             } else {
 #pragma unroll
                 for (int c = 0; c < KC; ++c)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, kr[u][c])[i], qf[c][i], s[u], 0, 0, 0);
+                        for (int u = 0; u < U; ++u) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, kr[u][c])[i], qf[c][i], s[u], 0, 0, 0);
             }
             const Pages next = settle();
-            ask(min(t + 2 * nw, t_end - 1));
+            ask(min(t + 2 * kw, t_end - 1));
             load_k(t_next, next);
-            // softmax: x = scores in units of log2, keys 32 t + 16 u + 4 g + i of head n
-            float p[8];
+            // softmax: x = scores in units of log2, keys TK t + 16 u + 4 g + i of head n
+            float p[J];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = s[j >> 2][j & 3] * scale2;
-            const bool whole = t * 32 >= rp.first && t * 32 + 32 <= rp.len;
+            for (int j = 0; j < J; ++j) p[j] = s[j >> 2][j & 3] * scale2;
+            const bool whole = t * TK >= rp.first && t * TK + TK <= rp.len;
             bool all_in = true;
             if constexpr (PAGES == 0) all_in = pg.ok;
             else all_in = __builtin_amdgcn_ballot_w64(!pg.ok) == 0;
             if (!(whole && all_in)) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int key = t * 32 + 16 * (j >> 2) + 4 * g + (j & 3);
+                for (int j = 0; j < J; ++j) {
+                    const int key = t * TK + 16 * (j >> 2) + 4 * g + (j & 3);
                     bool live = key >= rp.first && key < rp.len;
                     if (!all_in) {
                         const int id = key < rp.len ? trow[key >> a.c.page_shift] : -1;
@@ -389,7 +399,8 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttnArgs a) {
                         for (int w = 0; w < (int)(sizeof(VT) / 4); ++w) vr[j][h][w] = live ? vr[j][h][w] : 0u;   // what is there may be NaN
                 }
             }
-            float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+            float mx = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+            if constexpr (U == 2) mx = fmaxf(mx, fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
             mx = fmaxf(m, group_max(mx));
             const float ref = mx > -INFINITY ? mx : 0.f;
             if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
@@ -400,8 +411,9 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttnArgs a) {
                 m = mx;
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(p[j] - ref);
-            l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            for (int j = 0; j < J; ++j) p[j] = __builtin_amdgcn_exp2f(p[j] - ref);
+            if constexpr (U == 2) l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            else l += (p[0] + p[1]) + (p[2] + p[3]);
             if constexpr (KB) {
                 bf16x8 pb[PARTS];
                 to_parts<PARTS>(p, pb);
@@ -417,13 +429,13 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttnArgs a) {
                 }
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                for (int j = 0; j < J; ++j)
 #pragma unroll
                     for (int e = 0; e < NT; ++e)
                         acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[j][e >> 2][e & 3]), p[j], acc[e], 0, 0, 0);
             }
             load_v(t_next, next);
-            t += nw;
+            t += kw;
             if (t >= t_end) break;
             pg = next;
         }
@@ -441,7 +453,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttnArgs a) {
     }
     __syncthreads();
     float top = -INFINITY;
-    for (int w = 0; w < nw; ++w) top = fmaxf(top, sm_m[w * 16 + n]);
+    for (int w = wh; w < nw; w += hw) top = fmaxf(top, sm_m[w * 16 + n]);
     if (n < gn) {
         const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.f;
         float* o = sm_o + (wave * gn + n) * D;
@@ -455,59 +467,115 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttnArgs a) {
             }
     }
     __syncthreads();
-    for (int x = threadIdx.x; x < gn * (D / 4); x += blockDim.x) {
-        const int hn = x / (D / 4), d4 = (x % (D / 4)) * 4;
+    for (int x = threadIdx.x; x < hw * gn * (D / 4); x += blockDim.x) {
+        const int d4 = (x % (D / 4)) * 4, hn = (x / (D / 4)) % gn, ho = x / (D / 4) / gn;
+        if (hk0 + ho >= a.c.kv_heads) continue;
+        const int h = (hk0 + ho) * group + q16 * 16 + hn;
         float big = -INFINITY, sum = 0.f;
-        for (int w = 0; w < nw; ++w) big = fmaxf(big, sm_m[w * 16 + hn]);
+        for (int w = ho; w < nw; w += hw) big = fmaxf(big, sm_m[w * 16 + hn]);
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        for (int w = 0; w < nw; ++w) {
+        for (int w = ho; w < nw; w += hw) {
             const float mw = sm_m[w * 16 + hn];
             sum += mw > -INFINITY ? sm_l[w * 16 + hn] * __builtin_amdgcn_exp2f(mw - big) : 0.f;
             o += *reinterpret_cast<const f32x4*>(sm_o + (w * gn + hn) * D + d4);
         }
         if (rp.active > 1) {
-            const long long part = ((long long)row * a.q_heads + h0 + hn) * a.n_split + split;
+            const long long part = ((long long)row * a.q_heads + h) * a.n_split + split;
             *reinterpret_cast<f32x4*>(a.ws + part * D + d4) = o;
             if (d4 == 0) *reinterpret_cast<float2*>(a.ws + (long long)a.rows * a.q_heads * a.n_split * D + part * 2) = float2{big, sum};
         } else {
-            store_out(a, row, h0 + hn, d4, o, sum);
+            store_out(a, row, h, d4, o, sum);
         }
     }
 }
 
-// one block per (row, query head): the row's partial results joined in a fixed order
+// a row's few (at most 8) partial results joined in a fixed order, one wave per (row, query head), four to a block
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_few_kernel(PagedAttnArgs a) {
+    constexpr int LP = D / 4, NS = 64 / LP;         // lanes of a partial, partials at a time
+    const int pair = blockIdx.x * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (pair >= a.rows * a.q_heads) return;
+    const int row = pair / a.q_heads, h = pair - row * a.q_heads;
+    if (a.lengths[row] < 0) return;
+    const RowPlan rp = plan_row(a, row, a.seq ? a.seq[row] : row);
+    if (rp.active <= 1) return;
+    const long long part = (long long)pair * a.n_split;
+    const float2* ml = reinterpret_cast<const float2*>(a.ws + (long long)a.rows * a.q_heads * a.n_split * D) + part;
+    const int sub = lane / LP, d4 = (lane % LP) * 4;
+    float2 x[8];
+    f32x4 v[8 / NS];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) x[s] = s < rp.active ? ml[s] : float2{-INFINITY, 0.f};
+#pragma unroll
+    for (int k = 0; k < 8 / NS; ++k) {
+        const int s = k * NS + sub;
+        v[k] = s < rp.active ? *reinterpret_cast<const f32x4*>(a.ws + (part + s) * D + d4) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    float big = x[0].x, sum = 0.f, f[8];
+#pragma unroll
+    for (int s = 1; s < 8; ++s) big = fmaxf(big, x[s].x);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        f[s] = x[s].x > -INFINITY ? __builtin_amdgcn_exp2f(x[s].x - big) : 0.f;
+        sum += x[s].y * f[s];
+    }
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 8 / NS; ++k) {
+        float w = f[k * NS];
+#pragma unroll
+        for (int q = 1; q < NS; ++q) w = sub == q ? f[k * NS + q] : w;
+        o += v[k] * w;
+    }
+#pragma unroll
+    for (int d = LP; d < 64; d <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], d, 64);
+    if (sub == 0) store_out(a, row, h, d4, o, sum);
+}
+
+// many partial results: one block per (row, query head).  Three memory latencies: the row's plan, the maxima and sums, the partial results
 template <int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     constexpr int LP = D / 4, NS = 256 / LP;        // threads of a partial, partials at a time
     __shared__ __attribute__((aligned(16))) float sm_o[NS][D];
-    __shared__ float sm_l[NS];
+    __shared__ float sm_f[kMaxSplit], sm_l;
     const int row = blockIdx.x / a.q_heads, h = blockIdx.x % a.q_heads, tid = threadIdx.x;
     if (a.lengths[row] < 0) return;
     const RowPlan rp = plan_row(a, row, a.seq ? a.seq[row] : row);
     if (rp.active <= 1) return;
     const long long part = (long long)blockIdx.x * a.n_split;
-    const float* ml = a.ws + (long long)a.rows * a.q_heads * a.n_split * D + part * 2;
-    float big = -INFINITY;
-    for (int s = 0; s < rp.active; ++s) big = fmaxf(big, ml[2 * s]);
     const int sub = tid / LP, d4 = (tid % LP) * 4;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-#pragma unroll 4
-    for (int s = sub; s < rp.active; s += NS) {
-        const float2 x = *reinterpret_cast<const float2*>(ml + 2 * s);
+    if (tid < 64) {                                 // kMaxSplit = 64: a lane each
+        const float2* ml = reinterpret_cast<const float2*>(a.ws + (long long)a.rows * a.q_heads * a.n_split * D) + part;
+        const float2 x = tid < rp.active ? ml[tid] : float2{-INFINITY, 0.f};
+        float big = x.x;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
         const float f = x.x > -INFINITY ? __builtin_amdgcn_exp2f(x.x - big) : 0.f;
-        o += *reinterpret_cast<const f32x4*>(a.ws + (part + s) * D + d4) * f;
-        sum += x.y * f;
+        sm_f[tid] = f;
+        float sum = x.y * f;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        if (tid == 0) sm_l = sum;
     }
+    f32x4 x[kMaxSplit / NS];
+#pragma unroll
+    for (int k = 0; k < kMaxSplit / NS; ++k) {
+        const int s = k * NS + sub;
+        x[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (k * NS < rp.active && s < rp.active) x[k] = *reinterpret_cast<const f32x4*>(a.ws + (part + s) * D + d4);
+    }
+    __syncthreads();
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kMaxSplit / NS; ++k) o += x[k] * sm_f[k * NS + sub];
     *reinterpret_cast<f32x4*>(&sm_o[sub][d4]) = o;
-    if (d4 == 0) sm_l[sub] = sum;
     __syncthreads();
     if (sub == 0) {
-        for (int x = 1; x < NS; ++x) {
-            o += *reinterpret_cast<const f32x4*>(&sm_o[x][d4]);
-            sum += sm_l[x];
-        }
-        store_out(a, row, h, d4, o, sum);
+#pragma unroll
+        for (int k = 1; k < NS; ++k) o += *reinterpret_cast<const f32x4*>(&sm_o[k][d4]);
+        store_out(a, row, h, d4, o, sm_l);
     }
 }
 
@@ -535,36 +603,66 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
 
 namespace {
 
-template <bool QB, bool KB, int D, int PARTS>
+template <bool QB, bool KB, int D, int TK, int PARTS>
 void launch_attention_p(const PagedAttnArgs& a, unsigned blocks, unsigned threads, size_t lds, hipStream_t s) {
     const dim3 grid(blocks), block(threads);
-    if (a.c.page_shift >= 5) hipLaunchKernelGGL((paged_attention_kernel<QB, KB, D, 0, PARTS>), grid, block, lds, s, a);
-    else if (a.c.page_shift >= 2) hipLaunchKernelGGL((paged_attention_kernel<QB, KB, D, 1, PARTS>), grid, block, lds, s, a);
-    else hipLaunchKernelGGL((paged_attention_kernel<QB, KB, D, 2, PARTS>), grid, block, lds, s, a);
+    if (a.c.page_shift >= a.tile_shift) hipLaunchKernelGGL((paged_attention_kernel<QB, KB, D, TK, 0, PARTS>), grid, block, lds, s, a);
+    else if (a.c.page_shift >= 2) hipLaunchKernelGGL((paged_attention_kernel<QB, KB, D, TK, 1, PARTS>), grid, block, lds, s, a);
+    else hipLaunchKernelGGL((paged_attention_kernel<QB, KB, D, TK, 2, PARTS>), grid, block, lds, s, a);
 }
 template <int D>
 void launch_attention_d(const PagedAttnArgs& a, unsigned blocks, unsigned threads, size_t lds, hipStream_t s) {
-    if (!a.c.bf16) launch_attention_p<false, false, D, 1>(a, blocks, threads, lds, s);
-    else if (a.q_bf16 && a.out_bf16) launch_attention_p<true, true, D, 1>(a, blocks, threads, lds, s);
-    else if (a.q_bf16) launch_attention_p<true, true, D, 3>(a, blocks, threads, lds, s);
-    else if (a.out_bf16) launch_attention_p<false, true, D, 1>(a, blocks, threads, lds, s);
-    else launch_attention_p<false, true, D, 3>(a, blocks, threads, lds, s);
-    if (a.n_split > 1) hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)(a.rows * a.q_heads)), dim3(256), 0, s, a);
+    if (!a.c.bf16) launch_attention_p<false, false, D, 16, 1>(a, blocks, threads, lds, s);
+    else if (a.q_bf16 && a.out_bf16) launch_attention_p<true, true, D, 32, 1>(a, blocks, threads, lds, s);
+    else if (a.q_bf16) launch_attention_p<true, true, D, 32, 3>(a, blocks, threads, lds, s);
+    else if (a.out_bf16) launch_attention_p<false, true, D, 32, 1>(a, blocks, threads, lds, s);
+    else launch_attention_p<false, true, D, 32, 3>(a, blocks, threads, lds, s);
+    // (3072 pairs of 3 partial results: 8.3 us with a block to each, 5.1 with a wave)
+    if (a.n_split > 8) hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)(a.rows * a.q_heads)), dim3(256), 0, s, a);
+    else if (a.n_split > 1) hipLaunchKernelGGL((paged_join_few_kernel<D>), dim3((unsigned)(a.rows * a.q_heads + 3) / 4), dim3(256), 0, s, a);
 }
 
 }  // namespace
 
 void plan_paged_attention(PagedAttnArgs& a) {
-    const int group = a.q_heads / a.c.kv_heads;
+    const int group = a.q_heads / a.c.kv_heads, eb = a.c.bf16 ? 2 : 4;
+    a.tile_shift = a.c.bf16 ? 5 : 4;
+    const long long tiles = ((long long)a.max_length + (1 << a.tile_shift) - 1) >> a.tile_shift;
     const long long pairs = (long long)a.rows * a.c.kv_heads * ((group + 15) / 16);
-    const int tiles = (a.max_length + 31) / 32;
-    a.waves = 4;
+    // 128-byte rows that lie beside those of the other heads: blocks of four heads, two waves each, so that a block reads 512 bytes in a
+    // row (128 rows of 16 key heads of 64 bf16, up to 1100 keys: 67 us, a head a block 76; with the heads apart in memory 62)
+    if (group <= 16 && a.c.head_dim * eb == 128 && a.c.kh < a.c.ks && a.c.kv_heads >= 4 && pairs >= 1024) {
+        a.head_waves = 4;
+        a.waves = 8;
+        a.min_tiles = 8;
+        const long long blocks = (long long)a.rows * ((a.c.kv_heads + 3) / 4);
+        const long long n = std::min((4096 + blocks - 1) / blocks, (tiles + a.min_tiles - 1) / a.min_tiles);   // (at most 16)
+        a.n_split = (int)std::max(n, 1LL);
+        return;
+    }
+    a.head_waves = 1;
+    // Short contexts: about 1024 waves (one to a SIMD) without a second launch, where a wave's share stays within 160 KB.  (8 rows of 16 fp32 key
+    // heads, 350 keys: one block of 8 waves 11.1 us, split 13.7; 200 rows of one bf16 head, 900 keys: 4 waves 12.0, split 19.3.)
+    const long long one = (1024 + pairs - 1) / pairs;
+    const int w1 = one <= 1 ? 1 : (one <= 2 ? 2 : (one <= 6 ? 4 : (one <= 12 ? 8 : 0)));
+    a.n_split = 1;
+    if (w1 > 0 && tiles <= (a.c.head_dim == 64 ? 20 : 10) * w1) {
+        a.waves = w1;
+    } else {
+        // Else a wave to 8 tiles of the call, 1024 to 8192 of them, in blocks that grow with the work: the fewer partial results, the shorter the
+        // join.  (One row, 30000 bf16 keys, 8 key heads of 128: 2 waves x 32 splits 30.9 us, 4 x 32 33.0, 2 x 64 35.1; three rows of 131071: 8 x 43
+        // 258 us, 4 x 43 264; 96 rows of up to 8190: 4 x 3 333 us, 8 x 3 337, 4 x 1 394.)
+        const long long all = pairs * tiles;                                       // if every row is as long as the longest
+        const long long waves = std::min(std::max(all / 8, 1024LL), 8192LL);
+        const long long share = std::max(std::min((waves + pairs - 1) / pairs, (tiles + 1) / 2), 1LL);   // of a pair, two tiles to a wave at least
+        if (share <= 4) {
+            a.waves = share <= 1 ? 1 : (share <= 2 ? 2 : 4);
+        } else {
+            a.waves = share > 128 ? 8 : (all > 65536 ? 4 : 2);
+            a.n_split = (int)std::min((share + a.waves - 1) / a.waves, (long long)(a.waves == 2 ? kMaxSplit / 2 : kMaxSplit));
+        }
+    }
     a.min_tiles = 2 * a.waves;
-    long long n = (2048 + pairs - 1) / pairs;
-    n = n > 128 ? 128 : n;
-    const long long most = (tiles + a.min_tiles - 1) / a.min_tiles;
-    a.n_split = (int)(n < most ? n : most);
-    if (a.n_split < 1) a.n_split = 1;
 }
 
 size_t paged_attention_workspace(const PagedAttnArgs& a) {
@@ -573,8 +671,9 @@ size_t paged_attention_workspace(const PagedAttnArgs& a) {
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s) {
     const int group = a.q_heads / a.c.kv_heads;
-    const long long blocks = (long long)a.rows * a.c.kv_heads * ((group + 15) / 16) * a.n_split;
-    if (a.rows <= 0 || a.n_split < 1 || a.min_tiles < 1 || a.waves < 1 || a.waves > 4 || blocks > 0x7FFFFFFFLL) return hipErrorInvalidValue;
+    if (a.head_waves < 1 || a.waves % a.head_waves) return hipErrorInvalidValue;
+    const long long blocks = (long long)a.rows * ((a.c.kv_heads + a.head_waves - 1) / a.head_waves) * ((group + 15) / 16) * a.n_split;
+    if (a.rows <= 0 || a.n_split < 1 || a.n_split > kMaxSplit || a.min_tiles < 1 || a.waves < 1 || a.waves > 8 || blocks > 0x7FFFFFFFLL) return hipErrorInvalidValue;
     if (a.n_split > 1 && a.ws == nullptr) return hipErrorInvalidValue;
     const size_t lds = (size_t)a.waves * (32 + (size_t)(group < 16 ? group : 16) * a.c.head_dim) * 4;
     if (a.c.head_dim == 64) launch_attention_d<64>(a, (unsigned)blocks, 64u * a.waves, lds, s);
