@@ -68,6 +68,12 @@ class HiftInfo(C.Structure):
                                          "device", "reserved_")] + [("weight_bytes", C.c_int64)]
 
 
+class LogitRules(C.Structure):
+    """t3mi_logit_rules"""
+    _fields_ = [("bias_ids", C.POINTER(C.c_int32)), ("bias_values", C.POINTER(C.c_float)), ("allowed", C.POINTER(C.c_uint32)), ("n_bias", C.c_int32),
+                ("frequency_penalty", C.c_float), ("presence_penalty", C.c_float), ("reserved_", C.c_int32)]
+
+
 class PagedCache(C.Structure):
     """t3mi_paged_cache (a struct's fields in its order: the operators fill them by position)."""
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("block_table", C.c_void_p),
@@ -164,6 +170,10 @@ SYMBOLS = {
     "t3mi_hift_close": (C.c_int, [_H]),
     "t3mi_hift_get_info": (C.c_int, [_H, C.POINTER(HiftInfo)]),
     "t3mi_hift_inference": (C.c_int, [_H, C.c_int, _FP, _FP, _FP, _FP, C.c_int, _FP, _FP, _FP, _FP]),
+    "t3mi_set_paged_kv": (C.c_int, [_H, C.c_int, C.c_int]),
+    "t3mi_session_pages": (C.c_int, [_H, _IP, _IP]),
+    "t3mi_set_logit_rules": (C.c_int, [_H, C.POINTER(LogitRules)]),
+    "t3mi_session_logit_rules": (C.c_int, [_H, C.c_int, C.POINTER(LogitRules)]),
     "t3mi_paged_append": (C.c_int, [C.POINTER(PagedCache), C.POINTER(AppendArgs), C.c_void_p]),
     "t3mi_paged_attention_workspace": (C.c_int, [C.POINTER(PagedCache), C.POINTER(AttentionArgs), C.POINTER(C.c_size_t)]),
     "t3mi_paged_attention": (C.c_int, [C.POINTER(PagedCache), C.POINTER(AttentionArgs), C.c_void_p]),

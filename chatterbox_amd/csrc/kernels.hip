@@ -798,9 +798,9 @@ __global__ __launch_bounds__(kSampThreads) void sampler_kernel(SamplerArgs a, in
     int* misc = reinterpret_cast<int*>(scratch + 32);
 
     const int step = a.n_tokens[u];
-    const float* lc = a.logits + (size_t)u * a.rpu * V;
+    const float* lc = a.logits + (size_t)u * a.logit_rows * V;
     const uint8_t* seen = a.seen + (size_t)u * V;
-    const bool use_cfg = a.cfg_w > 0.f && a.rpu > 1;
+    const bool use_cfg = a.cfg_w > 0.f && a.logit_rows > 1;
     const bool turbo = a.variant == 2;   // .turbo_sample_token (R/t3.R:1688-1742)
 
     // 1. CFG, penalty, temperature  (R/t3.R:518-537)

@@ -159,6 +159,7 @@ struct EmbedArgs {                // token-by-token prefill input (R/t3.R:494, :
 struct SamplerArgs {
     const float* logits = nullptr;  // [n_utt*rpu, V]
     int V = 0, rpu = 1, n_utt = 0;
+    int logit_rows = 1;           // rows of `logits` per utterance: rpu, or 1 when guidance has been applied (rpu counts the rows of x and rowpos)
     float cfg_w = 0.f, temperature = 1.f, top_p = 1.f, min_p = 0.f, penalty = 1.f;
     int variant = 0, top_k = 0, stop_token = -1, start_token = -1, mask_stop = 0, max_new_tokens = 0;
     unsigned long long seed = 0;

@@ -24,6 +24,7 @@
 #include <vector>
 
 #include "kernels.hpp"
+#include "ops_kernels.hpp"
 #include "prompt.hpp"
 #include "safetensors.hpp"
 
@@ -113,6 +114,15 @@ struct LayerW {
     const float* b_down = nullptr;
 };
 
+// host copy of a t3mi_logit_rules
+struct LogitRules {
+    std::vector<int32_t> ids;
+    std::vector<float> vals;
+    std::vector<uint32_t> allowed;   // empty: every token
+    float fre = 0.f, pre = 0.f;
+    bool any() const { return !ids.empty() || !allowed.empty() || fre != 0.f || pre != 0.f; }
+};
+
 struct Session {
     int n_utt = 0, rpu = 1, rows = 0, max_len = 0, cap = 0, max_s0 = 0;
     int kps = 64, n_split = 1;  // attention split: keys per block, blocks per (row, head)
@@ -128,7 +138,19 @@ struct Session {
     std::vector<int32_t> s0;
     DevBuf kc, vc, x, qbuf, pm, pl, pacc, hbuf, logits, rope_cur, rowpos, start, emb_rows, emb_data, seen, tokens, n_tokens,
         done, s0_dev, forced, dist_ids, dist_probs, dist_n, drawn;
-    DevBuf pfs[9];              // prefill scratch (prefill_rows): grown on demand, freed after t3mi_session_begin's prefill when it is large
+    DevBuf pfs[11];             // prefill scratch (prefill_rows): grown on demand, freed after t3mi_session_begin's prefill when it is large
+    // paged cache (t3mi_set_paged_kv): kc / vc hold [layer][page][head][slot][64]; row r's positions are in the pages of its table row
+    bool paged = false;
+    int page_size = 0, n_pages = 0, table_w = 0;
+    DevBuf table, qkv, pws;     // [rows][table_w] page numbers, [rows][3 d] projections of a decode step, its attention's workspace
+    std::vector<int32_t> table_h;
+    std::vector<int> free_pages;               // pool pages no utterance holds
+    std::vector<std::vector<int>> held;        // [n_utt] pages of the slot's rows
+    // rules on the logits (t3mi_set_logit_rules, t3mi_session_logit_rules): with any, a launch before the sampler applies them
+    bool rules = false;
+    int rule_cap = 0;           // biases of a slot the buffers have room for
+    std::vector<LogitRules> slot_rules;        // [n_utt]
+    DevBuf lr_ids, lr_vals, lr_allowed, lr_fre, lr_pre, lr_out;
     DevBuf utt_ids, max_new_u;  // [n_utt] global utterance index (RNG stream) and token limit of each slot (t3mi_session_refill changes them)
     DevBuf filt;                // [n_utt][V] logits after CFG / penalty / temperature (t3mi_session_keep_filtered), else empty
     int n_forced = 0;
@@ -209,6 +231,9 @@ struct t3mi_model {
     std::unique_ptr<Session> sess;
     int cache_state = 0;                   // T3MI_CACHE_*: what t3mi_open_cached did with the packed bf16 file
     void* static_scratch = nullptr;        // this GPU's copy of the file-scope `scratch` array (hipGetSymbolAddress at open)
+    int paged_size = 0, paged_pages = 0;   // t3mi_set_paged_kv: page size (0: contiguous slabs) and pool pages (0: enough for any session)
+    LogitRules rules;                      // t3mi_set_logit_rules: what the utterances of a session start with
+    std::vector<int32_t> begin_limits;     // token limits of the slots of the session about to begin (run_continuous), or empty
     t3mi::PromptModel* prompt = nullptr;   // text_emb / cond_enc.* tensors (nullptr: decode-only checkpoint)
     DevBuf prompt_buf;                     // prompts built on device, alive until the next build
     bool use_graph = true;
@@ -949,10 +974,42 @@ struct GemmCtx {
     // K-split residual GEMM whose partial slabs are still to be folded into x (by the next norm launch)
     int pend_ks = 0;
     const float* pend_bias = nullptr;
+    float* qkv = nullptr;      // paged cache: [M][3 d] projections before the append
+    void* ws = nullptr;        // and the attention's workspace
     // bf16 weight storage with fp32 activation rows (exact fp32 products, the arithmetic of the GEMV path): the prefill
     // of sessions that decode with <= 4 rows
     bool act_f32 = false;
 };
+
+// ---- paged cache: the session's pool as the operators take it ----------------------------------------------------------------
+t3k::PagedCache paged_layer(const t3mi_model* m, const Session* s, int layer) {
+    t3k::PagedCache c;
+    const long long page = (long long)m->H * s->page_size * 64;
+    const size_t off = (size_t)layer * (size_t)s->n_pages * (size_t)page * (s->kv_bf16 ? 2 : 4);
+    c.k = s->kc.as<char>() + off;
+    c.v = s->vc.as<char>() + off;
+    c.kp = c.vp = page;
+    c.ks = c.vs = 64;
+    c.kh = c.vh = (long long)s->page_size * 64;   // a head's slots side by side: one run of memory for the attention
+    c.table = s->table.as<int>();
+    c.table_stride = s->table_w;
+    c.n_seqs = s->rows; c.max_pages = s->table_w; c.n_pages = s->n_pages;
+    c.page_shift = __builtin_ctz((unsigned)s->page_size);
+    c.kv_heads = m->H; c.head_dim = 64; c.bf16 = s->kv_bf16 ? 1 : 0;
+    return c;
+}
+// attention of M items (query rows c.q, positions c.posmap) over a layer's pool, as launched and as planned for the workspace
+t3k::PagedAttnArgs paged_attn(const t3mi_model* m, const Session* s, int layer, int M, int out_bf16) {
+    t3k::PagedAttnArgs a;
+    a.c = paged_layer(m, s, layer);
+    a.qr = a.outr = m->d;
+    a.qh = a.outh = 64;
+    a.scale = 0.125f;
+    a.rows = M; a.q_heads = m->H; a.q_bf16 = 0; a.out_bf16 = out_bf16;
+    a.max_length = s->max_len; a.length_add = 1;
+    t3k::plan_paged_attention(a);
+    return a;
+}
 
 int run_layers_gemm(t3mi_model* m, Session* s, GemmCtx& c, StepTimer* tm) {
     const int d = m->d, F = m->F, H = m->H;
@@ -1007,7 +1064,7 @@ int run_layers_gemm(t3mi_model* m, Session* s, GemmCtx& c, StepTimer* tm) {
         bool split_ln2 = false;
         // (measured, Llama bf16, ms per step without -> with: 4 utterances 0.929 -> 0.875, 16: 1.056 -> 1.009, 32: 1.303 -> 1.293, 64: 1.804 ->
         // 1.773, 96: 2.349 -> 2.340, 128: 2.764 -> 2.762, 192: 3.741 -> 3.753: up to 128 rows)
-        if ((m->norm_split & 1) && c.row_ss != nullptr && gu_f != nullptr && d % 32 == 0 && d / 32 <= 32 && c.M <= 128 && t3k::gemm_as_takes(c.M, d) &&
+        if ((m->norm_split & 1) && !(s->paged && turbo) && c.row_ss != nullptr && gu_f != nullptr && d % 32 == 0 && d / 32 <= 32 && c.M <= 128 && t3k::gemm_as_takes(c.M, d) &&
             (!turbo || (c.row_mu != nullptr && lw.o_colmean != nullptr && H <= 32 && (abf || c.M <= 32)))) {
             // (Turbo, S0 407, ms per step without -> with; bf16: 8 sentences 0.826 -> 0.787, 16: 0.870 -> 0.830, 32: 0.995 -> 0.953, 64: 1.321 ->
             // 1.300, 128: 1.991 -> 1.957; fp32: 8: 1.216 -> 1.216, 16: 1.272 -> 1.254, 32: 1.573 -> 1.557, 64: 2.345 -> 2.414: fp32 up to 32 rows)
@@ -1020,34 +1077,55 @@ int run_layers_gemm(t3mi_model* m, Session* s, GemmCtx& c, StepTimer* tm) {
                                               split_ln2 ? c.row_mu : nullptr));
         else if (!ln1_done) HIPCHK(t3k::launch_rmsnorm_rows(c.x, lw.ln1, m->eps, c.xn, c.M, d, abf, st, gp, c.pend_ks, c.pend_bias));
         c.pend_ks = 0;
-        {
+        if (s->paged) {
+            // projections, append (rotation on the way) and attention as launches of their own: the slab path's fused epilogue writes
+            // to rows of contiguous positions
             t3k::GemmArgs a;
-            a.W = lw.wqkv; a.Wf = as_ok ? m->frag(lw.wqkv, 1, c.M) : nullptr; a.A = c.xn; a.M = c.M; a.N = 3 * d; a.K = d;
-            a.posmap = c.posmap; a.rowmap = c.rowmap;
-            a.rope_cos = m->rope_cos.as<float>(); a.rope_sin = m->rope_sin.as<float>();
-            a.q = c.q; a.kcache = kc; a.vcache = vc; a.kv_bf16 = s->kv_bf16 ? 1 : 0; a.n_heads = H; a.max_len = s->max_len;
-            if (turbo) { a.bias = lw.b_qkv; a.rope = 0; }
-            if (ln1_done) { a.row_ss = c.row_ss; a.row_ss_tiles = d / 32; a.norm_eps = m->eps; }
-            if (pf_q && a.Wf) {
-                pf_region(a.pf, 0, 1, wo_f, d, d, t3k::EPI_RESID, true, split_ln2);
-                pf_region(a.pf, 1, 2, gu_f, turbo ? F : 2 * F, d, turbo ? t3k::EPI_GELU : t3k::EPI_SWIGLU, false, false);
-                pf_arm(a.pf, m->pf_gblocks);
+            a.W = lw.wqkv; a.A = c.xn; a.M = c.M; a.N = 3 * d; a.K = d; a.y = c.qkv; a.ldy = 3 * d;
+            if (turbo) a.bias = lw.b_qkv;
+            HIPCHK(t3k::launch_gemm(a, t3k::EPI_STORE, wdt, st));
+            t3k::PagedAppendArgs p;
+            p.c = paged_layer(m, s, l);
+            p.q = c.qkv; p.k = c.qkv + d; p.v = c.qkv + 2 * d; p.q_out = c.q;
+            p.qr = p.kr = p.vr = 3 * (long long)d; p.qor = d;
+            p.qh = p.kh = p.vh = p.qoh = 64;
+            if (!turbo) { p.cos = m->rope_cos.as<float>(); p.sin = m->rope_sin.as<float>(); p.rope_stride = 64; p.rope_len = m->rope_len; }
+            p.positions = c.posmap; p.seq = c.rowmap; p.rows = c.M; p.q_heads = H; p.in_bf16 = 0;
+            HIPCHK(t3k::launch_paged_append(p, st));
+            if (tm) tm->mark(K_QKV);
+            t3k::PagedAttnArgs t = paged_attn(m, s, l, c.M, abf);
+            t.q = c.q; t.out = c.attn_out; t.lengths = c.posmap; t.seq = c.rowmap; t.ws = static_cast<float*>(c.ws);
+            HIPCHK(t3k::launch_paged_attention(t, st));
+        } else {
+            {
+                t3k::GemmArgs a;
+                a.W = lw.wqkv; a.Wf = as_ok ? m->frag(lw.wqkv, 1, c.M) : nullptr; a.A = c.xn; a.M = c.M; a.N = 3 * d; a.K = d;
+                a.posmap = c.posmap; a.rowmap = c.rowmap;
+                a.rope_cos = m->rope_cos.as<float>(); a.rope_sin = m->rope_sin.as<float>();
+                a.q = c.q; a.kcache = kc; a.vcache = vc; a.kv_bf16 = s->kv_bf16 ? 1 : 0; a.n_heads = H; a.max_len = s->max_len;
+                if (turbo) { a.bias = lw.b_qkv; a.rope = 0; }
+                if (ln1_done) { a.row_ss = c.row_ss; a.row_ss_tiles = d / 32; a.norm_eps = m->eps; }
+                if (pf_q && a.Wf) {
+                    pf_region(a.pf, 0, 1, wo_f, d, d, t3k::EPI_RESID, true, split_ln2);
+                    pf_region(a.pf, 1, 2, gu_f, turbo ? F : 2 * F, d, turbo ? t3k::EPI_GELU : t3k::EPI_SWIGLU, false, false);
+                    pf_arm(a.pf, m->pf_gblocks);
+                }
+                HIPCHK(t3k::launch_gemm(a, t3k::EPI_ROPE_KV, wdt, st));
             }
-            HIPCHK(t3k::launch_gemm(a, t3k::EPI_ROPE_KV, wdt, st));
-        }
-        if (tm) tm->mark(K_QKV);
-        {
-            t3k::AttnRowsArgs a;
-            a.q = c.q; a.kcache = kc; a.vcache = vc; a.posmap = c.posmap; a.rowmap = c.rowmap;
-            a.out = c.attn_out; a.M = c.M; a.n_heads = H; a.max_len = s->max_len;
-            a.kv_bf16 = s->kv_bf16 ? 1 : 0; a.out_bf16 = abf;
-            if (split_ln2 && turbo) { a.dot_vec = lw.o_colmean; a.dot_out = c.row_mu + t3k::kAsMaxRows; }
-            if (pf_attn) {   // the idle CUs fetch o_proj's and gate_up's weights
-                pf_region(a.pf, 0, 1, wo_f, d, d, t3k::EPI_RESID, true, split_ln2);
-                pf_region(a.pf, 1, 2, gu_f, turbo ? F : 2 * F, d, turbo ? t3k::EPI_GELU : t3k::EPI_SWIGLU, false, false);
-                pf_arm(a.pf, m->pf_blocks);
+            if (tm) tm->mark(K_QKV);
+            {
+                t3k::AttnRowsArgs a;
+                a.q = c.q; a.kcache = kc; a.vcache = vc; a.posmap = c.posmap; a.rowmap = c.rowmap;
+                a.out = c.attn_out; a.M = c.M; a.n_heads = H; a.max_len = s->max_len;
+                a.kv_bf16 = s->kv_bf16 ? 1 : 0; a.out_bf16 = abf;
+                if (split_ln2 && turbo) { a.dot_vec = lw.o_colmean; a.dot_out = c.row_mu + t3k::kAsMaxRows; }
+                if (pf_attn) {   // the idle CUs fetch o_proj's and gate_up's weights
+                    pf_region(a.pf, 0, 1, wo_f, d, d, t3k::EPI_RESID, true, split_ln2);
+                    pf_region(a.pf, 1, 2, gu_f, turbo ? F : 2 * F, d, turbo ? t3k::EPI_GELU : t3k::EPI_SWIGLU, false, false);
+                    pf_arm(a.pf, m->pf_blocks);
+                }
+                HIPCHK(t3k::launch_attn_rows(a, st));
             }
-            HIPCHK(t3k::launch_attn_rows(a, st));
         }
         if (tm) tm->mark(K_ATTN);
         {
@@ -1094,7 +1172,7 @@ int run_layers_gemm(t3mi_model* m, Session* s, GemmCtx& c, StepTimer* tm) {
             // of K in LDS) writes x, w_ln1 * x in the activation type and per-tile sums of squares; the next qkv scales its rows before
             // RoPE.  Removes the norm launch and down_proj's partial slabs -- and measured SLOWER (64 utterances 1.758 -> 1.770 ms per step,
             // 16 utterances 1.007 -> 1.074: down_proj 6.7 -> 10.1 us, qkv 6.5 -> 7.5, against 4.9 for the norm launch), so it is off by default.
-            ln1_done = (m->norm_split & 2) && !turbo && abf && c.row_ss != nullptr && l + 1 < m->n_layers && F == 4096 && d % 32 == 0 &&
+            ln1_done = (m->norm_split & 2) && !s->paged && !turbo && abf && c.row_ss != nullptr && l + 1 < m->n_layers && F == 4096 && d % 32 == 0 &&
                        d / 32 <= 32 && c.M >= m->ln1_lo && c.M <= m->ln1_hi && c.M <= 128 && a.Wf != nullptr &&
                        m->frag(m->layers[l + 1].wqkv, 1, c.M) != nullptr;
             if (ln1_done) { a.part = nullptr; a.part_floats = 0; a.next_act = c.xn; a.next_norm_w = m->layers[l + 1].ln1; a.next_ss = c.row_ss; }
@@ -1124,6 +1202,8 @@ GemmCtx decode_ctx(Session* s) {
     c.kps = s->kps; c.n_split = s->n_split;
     c.row_ss = s->rowss.as<float>();
     c.row_mu = s->rowmu;
+    c.qkv = s->qkv.as<float>();
+    c.ws = s->pws.p;
     return c;
 }
 
@@ -1165,7 +1245,21 @@ int run_head(t3mi_model* m, Session* s, StepTimer* tm) {
 int run_sampler(t3mi_model* m, Session* s, StepTimer* tm) {
     t3k::SamplerArgs a;
     const t3mi_params& p = s->prm;
-    a.logits = s->logits.as<float>(); a.V = m->V; a.rpu = s->rpu; a.n_utt = s->n_utt;
+    if (s->rules) {
+        // guidance and the slots' rules in one pass over the logits rows; the sampler then reads one row per utterance
+        t3k::LogitsArgs r;
+        const bool cfg = p.cfg_weight > 0.f && s->rpu > 1;
+        r.logits = s->logits.p; r.lr = (long long)s->rpu * m->V;
+        if (cfg) { r.uncond = s->logits.as<float>() + m->V; r.ur = r.lr; r.cfg_weight = p.cfg_weight; }
+        r.out = s->lr_out.p; r.outr = m->V; r.rows = s->n_utt; r.vocab = m->V;
+        r.tokens = s->tokens.as<int>(); r.n_tokens = s->n_tokens.as<int>(); r.tr = s->cap; r.cap = s->cap;
+        r.frequency = s->lr_fre.as<float>(); r.presence = s->lr_pre.as<float>();
+        r.bias_ids = s->lr_ids.as<int>(); r.bias_values = s->lr_vals.as<float>(); r.br = r.bvr = s->rule_cap; r.n_bias = s->rule_cap;
+        r.allowed = s->lr_allowed.as<uint32_t>(); r.ar = (m->V + 31) / 32;
+        HIPCHK(t3k::launch_process_logits(r, m->stream));
+    }
+    a.logits = s->rules ? s->lr_out.as<float>() : s->logits.as<float>(); a.V = m->V; a.rpu = s->rpu; a.n_utt = s->n_utt;
+    a.logit_rows = s->rules ? 1 : s->rpu;
     a.cfg_w = p.cfg_weight; a.temperature = p.temperature; a.top_p = p.top_p; a.min_p = p.min_p;
     a.penalty = p.repetition_penalty; a.variant = p.sampler; a.top_k = p.top_k; a.stop_token = p.stop_token;
     a.mask_stop = p.mask_stop; a.max_new_tokens = p.max_new_tokens; a.seed = p.seed;
@@ -1257,6 +1351,7 @@ int prefill_rows(t3mi_model* m, Session* s, const std::vector<int>& rows_list, c
     HIPCHK(grow(dpos, max_items * 4));
     HIPCHK(grow(drow, max_items * 4));
     HIPCHK(grow(dlast, (size_t)nr * sizeof(void*)));
+    if (s->paged) HIPCHK(grow(s->pfs[9], max_items * 3 * d * 4));
     std::vector<const float*> isrc, last;
     std::vector<int32_t> ipos, irow;
     int rc;
@@ -1283,6 +1378,11 @@ int prefill_rows(t3mi_model* m, Session* s, const std::vector<int>& rows_list, c
         c.xn = xnpf.p; c.attn_out = aopf.p; c.hact = hpf.p;
         c.posmap = dpos.as<int>(); c.rowmap = drow.as<int>();
         c.act_f32 = pf_act_f32;
+        if (s->paged) {
+            HIPCHK(grow(s->pfs[10], t3k::paged_attention_workspace(paged_attn(m, s, 0, c.M, as == 2 ? 1 : 0))));
+            c.qkv = s->pfs[9].as<float>();
+            c.ws = s->pfs[10].p;
+        }
         if ((rc = run_layers_gemm(m, s, c, nullptr))) return rc;
         if ((rc = fold_pending(m, s, c))) return rc;
         // the last prompt position of every row feeds the first speech-head evaluation: runs of consecutive session rows at a time
@@ -1295,6 +1395,117 @@ int prefill_rows(t3mi_model* m, Session* s, const std::vector<int>& rows_list, c
         HIPCHK(hipStreamSynchronize(st));  // the host vectors are refilled by the next group; the scratch dies after the last
     }
     return T3MI_OK;
+}
+
+// ---- pages of the slots ---------------------------------------------------------------------------------------------------------
+// pages one row of an utterance needs: its prompt and every token up to its limit, never more than the cache rows have room for
+int pages_of(const Session* s, int s0, int limit) {
+    const long long n = std::min<long long>((long long)s0 + limit, s->max_len);
+    return (int)((n + s->page_size - 1) / s->page_size);
+}
+void release_pages(Session* s, int u) {
+    s->free_pages.insert(s->free_pages.end(), s->held[u].begin(), s->held[u].end());
+    s->held[u].clear();
+}
+// the caller has made sure that there are enough; fills the slot's rows of the host table
+void take_pages(Session* s, int u, int per_row) {
+    for (int r = 0; r < s->rpu; ++r) {
+        int32_t* row = s->table_h.data() + (size_t)(u * s->rpu + r) * s->table_w;
+        for (int e = 0; e < s->table_w; ++e) {
+            row[e] = -1;
+            if (e >= per_row) continue;
+            row[e] = s->free_pages.back();
+            s->held[u].push_back(row[e]);
+            s->free_pages.pop_back();
+        }
+    }
+}
+
+// ---- rules on the logits --------------------------------------------------------------------------------------------------------
+int take_rules(const t3mi_model* m, const t3mi_logit_rules* r, LogitRules& o) {
+    o = LogitRules();
+    if (!r) return T3MI_OK;
+    if (r->n_bias < 0 || r->n_bias > 4094 || (r->n_bias > 0 && (!r->bias_ids || !r->bias_values)))
+        return fail(T3MI_ERR_ARG, "logit rules: n_bias must be 0..4094, with ids and values");
+    for (int i = 0; i < r->n_bias; ++i) {
+        if (r->bias_ids[i] < 0 || r->bias_ids[i] >= m->V)
+            return fail(T3MI_ERR_ARG, "logit rules: bias on token " + std::to_string(r->bias_ids[i]) + " outside the vocabulary");
+        if (!std::isfinite(r->bias_values[i])) return fail(T3MI_ERR_ARG, "logit rules: biases must be finite (allowed says what may not be drawn)");
+    }
+    if (!std::isfinite(r->frequency_penalty) || !std::isfinite(r->presence_penalty)) return fail(T3MI_ERR_ARG, "logit rules: penalties must be finite");
+    if (r->allowed) {
+        bool some = false;
+        for (int t = 0; t < m->V && !some; ++t) some = (r->allowed[t >> 5] >> (t & 31)) & 1u;
+        if (!some) return fail(T3MI_ERR_ARG, "logit rules: no token is allowed");
+        o.allowed.assign(r->allowed, r->allowed + (m->V + 31) / 32);
+    }
+    if (r->n_bias > 0) {
+        o.ids.assign(r->bias_ids, r->bias_ids + r->n_bias);
+        o.vals.assign(r->bias_values, r->bias_values + r->n_bias);
+    }
+    o.fre = r->frequency_penalty;
+    o.pre = r->presence_penalty;
+    return T3MI_OK;
+}
+
+// slot u's rules to the device (the stream is idle)
+int upload_rules(t3mi_model* m, Session* s, int u) {
+    const LogitRules& r = s->slot_rules[u];
+    const size_t cap = s->rule_cap, words = (m->V + 31) / 32;
+    std::vector<int32_t> ids(cap, -1);
+    std::vector<float> vals(cap, 0.f);
+    std::vector<uint32_t> all(words, 0xFFFFFFFFu);
+    std::copy(r.ids.begin(), r.ids.end(), ids.begin());
+    std::copy(r.vals.begin(), r.vals.end(), vals.begin());
+    HIPCHK(hipMemcpy(s->lr_ids.as<int>() + u * cap, ids.data(), cap * 4, hipMemcpyHostToDevice));
+    HIPCHK(hipMemcpy(s->lr_vals.as<float>() + u * cap, vals.data(), cap * 4, hipMemcpyHostToDevice));
+    HIPCHK(hipMemcpy(s->lr_allowed.as<uint32_t>() + u * words, r.allowed.empty() ? all.data() : r.allowed.data(), words * 4, hipMemcpyHostToDevice));
+    HIPCHK(hipMemcpy(s->lr_fre.as<float>() + u, &r.fre, 4, hipMemcpyHostToDevice));
+    HIPCHK(hipMemcpy(s->lr_pre.as<float>() + u, &r.pre, 4, hipMemcpyHostToDevice));
+    return T3MI_OK;
+}
+
+// the rules of slots `utts` change (the stream is idle).  The first rules of a session, and more biases than its buffers hold, change what a
+// step launches: the captured graph is dropped and the next step captures another.
+int set_slot_rules(t3mi_model* m, Session* s, const std::vector<int>& utts, const LogitRules& r) {
+    if (!s->rules && !r.any()) return T3MI_OK;
+    s->slot_rules.resize(s->n_utt);
+    for (int u : utts) s->slot_rules[u] = r;
+    int rc;
+    if (s->rules && (int)r.ids.size() <= s->rule_cap) {
+        for (int u : utts)
+            if ((rc = upload_rules(m, s, u))) return rc;
+        return T3MI_OK;
+    }
+    if (s->gexec) (void)hipGraphExecDestroy(s->gexec);
+    if (s->graph) (void)hipGraphDestroy(s->graph);
+    s->gexec = nullptr;
+    s->graph = nullptr;
+    s->graph_tried = false;
+    s->rules = false;
+    s->rule_cap = (int)((std::max<size_t>(r.ids.size(), 1) + 63) / 64 * 64);
+    const size_t U = s->n_utt, cap = s->rule_cap;
+    HIPCHK(s->lr_ids.alloc(U * cap * 4));
+    HIPCHK(s->lr_vals.alloc(U * cap * 4));
+    HIPCHK(s->lr_allowed.alloc(U * ((m->V + 31) / 32) * 4));
+    HIPCHK(s->lr_fre.alloc(U * 4));
+    HIPCHK(s->lr_pre.alloc(U * 4));
+    HIPCHK(s->lr_out.alloc(U * (size_t)m->V * 4));
+    for (int u = 0; u < s->n_utt; ++u)
+        if ((rc = upload_rules(m, s, u))) return rc;
+    s->rules = true;
+    return T3MI_OK;
+}
+
+// nothing throws across the C boundary
+template <typename F> int guarded(F f) {
+    try {
+        return f();
+    } catch (const std::exception& e) {
+        g_err = "out of memory";
+        (void)e;
+        return T3MI_ERR_HIP;
+    }
 }
 
 int need_session(t3mi_model* m) {
@@ -1517,11 +1728,36 @@ int t3mi_session_begin(t3mi_model* m, int n_utt, int rpu, const float* const* em
     {
         const char* gm = std::getenv("T3MI_GEMM_ROWS");  // rows above which the MFMA path is used (default 4)
         const int thr = gm ? std::atoi(gm) : 4;
-        s->gemm_mode = (int)rows > thr;
+        s->paged = m->paged_size > 0;
+        s->gemm_mode = (int)rows > thr || s->paged;      // (the few-row kernels know contiguous slabs alone)
         const char* kve = std::getenv("T3MI_KV");        // "f32" keeps fp32 KV slabs in the many-row bf16 regime
         s->kv_bf16 = s->gemm_mode && m->wdtype == T3MI_W_BF16 && d % 256 == 0 && !(kve && kve[0] == 'f');
     }
-    const size_t kv = (size_t)m->n_layers * rows * m->H * s->max_len * 64 * (s->kv_bf16 ? 2 : 4);
+    size_t kv = (size_t)m->n_layers * rows * m->H * s->max_len * 64 * (s->kv_bf16 ? 2 : 4);
+    if (s->paged) {
+        s->page_size = m->paged_size;
+        s->table_w = (s->max_len + s->page_size - 1) / s->page_size;
+        const size_t most = rows * (size_t)s->table_w;
+        if (most > 0x7FFFFFFFu) return fail(T3MI_ERR_ARG, "t3mi_session_begin: too many pages");
+        s->n_pages = m->paged_pages > 0 ? (int)std::min<size_t>((size_t)m->paged_pages, most) : (int)most;
+        s->table_h.assign(most, -1);
+        s->held.resize(n_utt);
+        s->free_pages.resize(s->n_pages);
+        for (int i = 0; i < s->n_pages; ++i) s->free_pages[i] = s->n_pages - 1 - i;
+        for (int u = 0; u < n_utt; ++u) {
+            const int limit = m->begin_limits.size() == (size_t)n_utt ? m->begin_limits[u] : max_new;
+            const int per_row = pages_of(s.get(), s0[u], std::min(limit, max_new));
+            if ((size_t)per_row * rpu > s->free_pages.size())
+                return fail(T3MI_ERR_ARG, "t3mi_session_begin: the pool of " + std::to_string(s->n_pages) + " pages is too small: utterance " + std::to_string(u) +
+                                              " needs " + std::to_string(per_row * rpu) + ", " + std::to_string(s->free_pages.size()) + " are left");
+            take_pages(s.get(), u, per_row);
+        }
+        kv = (size_t)m->n_layers * s->n_pages * m->H * s->page_size * 64 * (s->kv_bf16 ? 2 : 4);
+        HIPCHK(s->table.alloc(most * 4));
+        HIPCHK(hipMemcpy(s->table.p, s->table_h.data(), most * 4, hipMemcpyHostToDevice));
+        HIPCHK(s->qkv.alloc(rows * 3 * d * 4));
+        HIPCHK(s->pws.alloc(t3k::paged_attention_workspace(paged_attn(m, s.get(), 0, (int)rows, m->wdtype == T3MI_W_BF16 ? 1 : 0))));
+    }
     HIPCHK(s->kc.alloc(kv));
     HIPCHK(s->vc.alloc(kv));
     HIPCHK(s->x.alloc(rows * d * 4));
@@ -1537,6 +1773,7 @@ int t3mi_session_begin(t3mi_model* m, int n_utt, int rpu, const float* const* em
         const size_t as = m->wdtype == T3MI_W_BF16 ? 2 : 4;
         HIPCHK(s->xn.alloc(rows * d * as));
         HIPCHK(s->attn_out.alloc(rows * d * as));
+        if (s->paged) HIPCHK(hipMemsetAsync(s->attn_out.p, 0, rows * d * as, m->stream));   // (a row without an utterance is never written)
         HIPCHK(s->hact.alloc(rows * F * as));
         // K-split partial slabs: the decode rows of a many-row session, and the prompt items of a short prefill
         // (few row chunks: the residual GEMMs need the K split to fill the chip)
@@ -1635,7 +1872,7 @@ int t3mi_session_begin(t3mi_model* m, int n_utt, int rpu, const float* const* em
     const bool pf_act_f32 = m->wdtype == T3MI_W_BF16 && !s->gemm_mode;
     if (pfenv && std::strcmp(pfenv, "token") == 0) gemm_prefill = false;
     if (pfenv && std::strcmp(pfenv, "gemm") == 0) gemm_prefill = true;
-    if (s->kv_bf16) gemm_prefill = true;   // the one-position decode kernels write fp32 cache slots
+    if (s->kv_bf16 || s->paged) gemm_prefill = true;   // the one-position decode kernels write fp32 slots of contiguous slabs
     s->gemm_prefill = gemm_prefill; s->pf_act_f32 = pf_act_f32;
     if (gemm_prefill) {
         std::vector<int> all_rows(rows);
@@ -1662,8 +1899,57 @@ int t3mi_session_begin(t3mi_model* m, int n_utt, int rpu, const float* const* em
     }
     if ((rc = run_head(m, s.get(), nullptr))) return rc;
     HIPCHK(hipStreamSynchronize(st));
+    {
+        std::vector<int> every(n_utt);
+        for (int u = 0; u < n_utt; ++u) every[u] = u;
+        if ((rc = set_slot_rules(m, s.get(), every, m->rules))) return rc;
+    }
     m->sess = std::move(s);
     return T3MI_OK;
+}
+
+int t3mi_set_paged_kv(t3mi_model* m, int page_size, int n_pages) {
+    if (!m) return fail(T3MI_ERR_ARG, "null model handle");
+    if (page_size != 0 && (page_size < 4 || page_size > 1024 || (page_size & (page_size - 1))))
+        return fail(T3MI_ERR_ARG, "t3mi_set_paged_kv: page_size must be 0 or a power of two, 4..1024");
+    if (n_pages < 0 || (page_size == 0 && n_pages != 0)) return fail(T3MI_ERR_ARG, "t3mi_set_paged_kv: n_pages must be >= 0, and 0 without pages");
+    m->paged_size = page_size;
+    m->paged_pages = n_pages;
+    return T3MI_OK;
+}
+
+int t3mi_session_pages(t3mi_model* m, int32_t* total, int32_t* free_pages) {
+    int rc = need_session(m);
+    if (rc) return rc;
+    if (!total || !free_pages) return fail(T3MI_ERR_ARG, "t3mi_session_pages: null result");
+    *total = m->sess->paged ? m->sess->n_pages : 0;
+    *free_pages = (int32_t)m->sess->free_pages.size();
+    return T3MI_OK;
+}
+
+int t3mi_set_logit_rules(t3mi_model* m, const t3mi_logit_rules* r) {
+    if (!m) return fail(T3MI_ERR_ARG, "null model handle");
+    return guarded([&] {
+        LogitRules o;
+        const int rc = take_rules(m, r, o);
+        if (!rc) m->rules = std::move(o);
+        return rc;
+    });
+}
+
+int t3mi_session_logit_rules(t3mi_model* m, int utt, const t3mi_logit_rules* r) {
+    int rc = need_session(m);
+    if (rc) return rc;
+    Session* s = m->sess.get();
+    if (utt < 0 || utt >= s->n_utt) return fail(T3MI_ERR_ARG, "t3mi_session_logit_rules: no such slot");
+    return guarded([&]() -> int {
+        LogitRules o;
+        int rc2 = take_rules(m, r, o);
+        if (rc2) return rc2;
+        HIPCHK(hipSetDevice(m->device));
+        HIPCHK(hipStreamSynchronize(m->stream));   // the steps enqueued so far keep the rules they were enqueued under
+        return set_slot_rules(m, s, {utt}, o);
+    });
 }
 
 int t3mi_session_force(t3mi_model* m, const int32_t* forced, int n_forced) {
@@ -2154,6 +2440,25 @@ int t3mi_session_refill(t3mi_model* m, int n, const int32_t* utts, const float* 
     HIPCHK(hipSetDevice(m->device));
     hipStream_t st = m->stream;
     HIPCHK(hipStreamSynchronize(st));   // the steps enqueued so far are over: the slots' tokens were the caller's to read before this call
+    if (s->paged) {
+        // the pages of the slots that are refilled, and of every other slot whose utterance has ended, go back to the pool first
+        std::vector<int32_t> over(s->n_utt);
+        HIPCHK(hipMemcpy(over.data(), s->done.p, (size_t)s->n_utt * 4, hipMemcpyDeviceToHost));
+        size_t want = 0, have = s->free_pages.size();
+        for (int u = 0; u < s->n_utt; ++u)
+            if (taken[u] || over[u]) have += s->held[u].size();
+        for (int i = 0; i < n; ++i) want += (size_t)rpu * pages_of(s, s0[i], mn[i]);
+        if (want > have)
+            return fail(T3MI_ERR_STATE, "t3mi_session_refill: " + std::to_string(want) + " pages are needed, " + std::to_string(have) + " of " +
+                                            std::to_string(s->n_pages) + " are free");
+        for (int u = 0; u < s->n_utt; ++u)
+            if (taken[u] || over[u]) release_pages(s, u);
+        for (int i = 0; i < n; ++i) take_pages(s, utts[i], pages_of(s, s0[i], mn[i]));
+        HIPCHK(hipMemcpy(s->table.p, s->table_h.data(), s->table_h.size() * 4, hipMemcpyHostToDevice));
+    }
+    if (s->rules || m->rules.any()) {   // a slot's rules are its utterance's: the new one starts with the model's
+        if ((rc = set_slot_rules(m, s, std::vector<int>(utts, utts + n), m->rules))) return rc;
+    }
     // prompts to the device
     DevBuf stage;
     std::vector<int> order(n);
@@ -2228,17 +2533,34 @@ int t3mi_session_refill_tokens(t3mi_model* m, int n, const int32_t* utts, const 
 // ---- continuous batching driver: n_utt utterances through `slots` session slots (t3mi_session_refill between polls) ---------------
 namespace {
 struct ContinuousJob {
-    int n_utt = 0, slots = 0, poll = 16;
+    int n_utt = 0, slots = 0, poll = 16, rows = 1;   // rows: of an utterance
     std::vector<int32_t> mx;                 // token limit of each utterance (without Turbo's extra first token)
     std::vector<int32_t> order;              // the queue: utterance indices in the order they are started
+    std::vector<int32_t> s0;                 // prompt lengths
     std::function<int(const std::vector<int32_t>& items)> begin;                                          // session whose slot u holds utterance items[u]
     std::function<int(const std::vector<int32_t>& slots, const std::vector<int32_t>& items)> refill;      // slots[i] takes utterance items[i]
 };
 
-int run_continuous(t3mi_model* m, const ContinuousJob& job, int32_t* out, int32_t cap, int32_t* n_out, int32_t* stats) {
+int run_continuous(t3mi_model* m, ContinuousJob& job, int32_t* out, int32_t cap, int32_t* n_out, int32_t* stats) {
     const int extra = m->variant == T3MI_VARIANT_TURBO ? 1 : 0;
+    if (m->paged_size > 0 && m->paged_pages > 0) {
+        // Every utterance has to fit an empty pool; and no more slots than it serves from the start (an utterance holds the pages of its
+        // prompt and its own limit)
+        const auto pages = [&](int i) { return (long long)job.rows * ((job.s0[i] + job.mx[i] + extra + m->paged_size - 1) / m->paged_size); };
+        for (int i = 0; i < job.n_utt; ++i)
+            if (pages(i) > m->paged_pages)
+                return fail(T3MI_ERR_ARG, "t3mi_generate_continuous: utterance " + std::to_string(i) + " needs " + std::to_string(pages(i)) + " pages, the pool has " +
+                                              std::to_string(m->paged_pages));
+        long long left = m->paged_pages;
+        int fit = 0;
+        while (fit < job.slots && pages(job.order[fit]) <= left) left -= pages(job.order[fit++]);
+        job.slots = fit;
+    }
     std::vector<int32_t> owner(job.order.begin(), job.order.begin() + job.slots);
+    m->begin_limits.resize(job.slots);
+    for (int u = 0; u < job.slots; ++u) m->begin_limits[u] = job.mx[owner[u]] + extra;
     int rc = job.begin(owner);
+    m->begin_limits.clear();
     if (rc) return rc;
     Session* s = m->sess.get();
     {   // t3mi_session_begin numbered the slots first_utterance_id + slot and gave all of them the session's limit: each slot gets
@@ -2281,9 +2603,26 @@ int run_continuous(t3mi_model* m, const ContinuousJob& job, int32_t* out, int32_
             owner[u] = -1;
             --live;
             freed.push_back(u);
+            if (s->paged) release_pages(s, u);
         }
         if (rc) break;
-        const int take = std::min<int>((int)freed.size(), job.n_utt - next);
+        if (s->paged) {   // slots freed earlier, when no page was left for the next utterance, wait with the others
+            freed.clear();
+            for (int u = 0; u < job.slots; ++u)
+                if (owner[u] < 0) freed.push_back(u);
+        }
+        int take = std::min<int>((int)freed.size(), job.n_utt - next);
+        if (s->paged) {
+            long long left = (long long)s->free_pages.size();   // (all of them once no slot is live: one utterance at least is taken then)
+            int fit = 0;
+            while (fit < take) {
+                const int i = job.order[next + fit];
+                left -= (long long)s->rpu * pages_of(s, job.s0[i], std::min(job.mx[i] + extra, s->cap));
+                if (left < 0) break;
+                ++fit;
+            }
+            take = fit;
+        }
         if (take > 0) {
             std::vector<int32_t> sl(freed.begin(), freed.begin() + take), it(take);
             for (int k = 0; k < take; ++k) { it[k] = job.order[next + k]; owner[sl[k]] = it[k]; }
@@ -2318,6 +2657,7 @@ int continuous_setup(t3mi_model* m, int n_utt, const int32_t* s0, const int32_t*
     if (flags & ~T3MI_CONTINUOUS_LONGEST_FIRST) return fail(T3MI_ERR_ARG, "t3mi_generate_continuous: unknown flag");
     const int extra = m->variant == T3MI_VARIANT_TURBO ? 1 : 0;
     job.n_utt = n_utt;
+    job.s0.assign(s0, s0 + n_utt);
     job.slots = std::min(slots, n_utt);
     job.poll = poll_steps;
     job.mx.resize(n_utt);
@@ -2353,6 +2693,7 @@ int t3mi_generate_continuous(t3mi_model* m, int n_utt, int rows_per_utt, const f
     t3mi_params sp;
     int rc = continuous_setup(m, n_utt, s0, max_new_each, s0, slots, poll_steps, flags, p, cap, job, sp);
     if (rc) return rc;
+    job.rows = rows_per_utt;
     job.begin = [&](const std::vector<int32_t>& it) {
         std::vector<const float*> e(it.size());
         std::vector<int32_t> l(it.size());
@@ -2392,6 +2733,7 @@ int t3mi_generate_continuous_tokens(t3mi_model* m, int n_utt, const t3mi_cond* c
     t3mi_params sp;
     int rc = continuous_setup(m, n_utt, s0.data(), max_new_each, n_text, slots, poll_steps, flags, p, cap, job, sp);
     if (rc) return rc;
+    job.rows = p->cfg_weight > 0.f && m->variant != T3MI_VARIANT_TURBO ? 2 : 1;
     auto pick = [&](const std::vector<int32_t>& it, std::vector<t3mi_cond>& c, std::vector<const int32_t*>& t, std::vector<int32_t>& nt) {
         c.resize(it.size()); t.resize(it.size()); nt.resize(it.size());
         for (size_t k = 0; k < it.size(); ++k) { c[k] = conds[it[k]]; t[k] = text_tokens[it[k]]; nt[k] = n_text[it[k]]; }

@@ -61,6 +61,19 @@ class T3Model:
             self._lib.t3mi_close(self._h)
             self._h = None
 
+    def set_paged_kv(self, page_size: int = 64, pages: int = 0) -> None:
+        """Sessions begun from now on keep keys and values in pages of `page_size` positions out of one pool of `pages` pages (0: the worst
+        case); page_size 0: contiguous slabs again.  An utterance holds the pages of its prompt and its own token limit, so ragged
+        batches run in the memory they need (t3mi_set_paged_kv)."""
+        _lib.check(self._lib.t3mi_set_paged_kv(self._h, int(page_size), int(pages)))
+
+    def set_logit_rules(self, bias=None, allowed=None, frequency_penalty: float = 0.0, presence_penalty: float = 0.0) -> None:
+        """What every utterance to come is sampled under, until changed (t3mi_set_logit_rules; no argument: no rules).  bias: {token: value added
+        to its logit}; allowed: the tokens that may be drawn (ids, or a bool array [vocab]); frequency_penalty is subtracted
+        once for every time a token has been drawn, presence_penalty if it has been.  Applied after guidance, before the sampler's own
+        repetition penalty, temperature, min-p and top-p."""
+        _lib.check(self._lib.t3mi_set_logit_rules(self._h, _logit_rules(self, bias, allowed, frequency_penalty, presence_penalty)))
+
     def __del__(self):
         try:
             self.close()
@@ -72,6 +85,31 @@ class T3Model:
 
     def __exit__(self, *exc):
         self.close()
+
+
+def _logit_rules(model: T3Model, bias, allowed, frequency_penalty, presence_penalty) -> _lib.LogitRules:
+    r = _lib.LogitRules(frequency_penalty=float(frequency_penalty), presence_penalty=float(presence_penalty))
+    if bias:
+        r.n_bias = len(bias)
+        r.bias_ids = (C.c_int32 * len(bias))(*[int(t) for t in bias])
+        r.bias_values = (C.c_float * len(bias))(*[float(v) for v in bias.values()])
+    if allowed is not None:
+        a = np.asarray(allowed)
+        if a.dtype == bool:
+            if a.shape != (model.vocab,):
+                raise ValueError(f"allowed: a bool array must be [{model.vocab}], got {a.shape}")
+            bits = a
+        else:
+            ids = a.astype(np.int64).reshape(-1)
+            if ids.size and (ids.min() < 0 or ids.max() >= model.vocab):
+                raise ValueError(f"allowed: token ids must be in 0..{model.vocab - 1}")
+            bits = np.zeros(model.vocab, bool)
+            bits[ids] = True
+        words = np.zeros((model.vocab + 31) // 32 * 32, np.uint8)
+        words[:model.vocab] = bits
+        words = np.packbits(words, bitorder="little").view(np.uint32)
+        r.allowed = (C.c_uint32 * len(words))(*[int(w) for w in words])
+    return r
 
 
 def load_t3(path: str, device: int = 0, dtype: str = "f32", **kw) -> T3Model:
@@ -494,6 +532,17 @@ class Session:
         ptrs = (C.c_void_p * n)(*[e.ctypes.data for e in es])
         s0 = (C.c_int32 * n)(*[e.shape[1] for e in es])
         _lib.check(L.t3mi_session_refill(self.model._h, n, ua, ptrs, s0, mn, ids, 0))
+
+    def logit_rules(self, utt: int = 0, bias=None, allowed=None, frequency_penalty: float = 0.0, presence_penalty: float = 0.0) -> None:
+        """The rules of slot `utt` from the next step on (t3mi_session_logit_rules; arguments as T3Model.set_logit_rules, none: no rules).  A
+        grammar sets `allowed` between steps of one."""
+        _lib.check(self.model._lib.t3mi_session_logit_rules(self.model._h, int(utt), _logit_rules(self.model, bias, allowed, frequency_penalty, presence_penalty)))
+
+    def pages(self) -> Tuple[int, int]:
+        """(pages of the session's pool, pages no utterance holds); (0, 0) without T3Model.set_paged_kv."""
+        total, free = C.c_int32(0), C.c_int32(0)
+        _lib.check(self.model._lib.t3mi_session_pages(self.model._h, C.byref(total), C.byref(free)))
+        return int(total.value), int(free.value)
 
     def decode(self, n_steps: int = 1):
         _lib.check(self.model._lib.t3mi_session_decode(self.model._h, int(n_steps)))

@@ -191,6 +191,36 @@ int t3mi_generate_batch_tokens(t3mi_model* m, int n_utt, const t3mi_cond* conds,
 int t3mi_session_begin_tokens(t3mi_model* m, int n_utt, const t3mi_cond* conds, const int32_t* const* text_tokens,
                               const int32_t* n_text, const t3mi_params* p);
 
+/* ---- paged key-value cache and logit rules of the sessions ------------------------------------------------------------------
+ * Sessions begun after t3mi_set_paged_kv keep their keys and values in pages of `page_size` positions (a power of two, 4..1024; 0: the
+ * contiguous slabs of create_kv_cache again) out of one pool of `n_pages` pages per session (0: enough for the session's worst
+ * case).  An utterance holds the pages of its prompt and of its own token limit, from its begin or refill until it has ended and its slot
+ * or another is refilled, instead of a slab as long as the longest utterance may get: with n_pages below the worst case, a batch of
+ * ragged utterances runs in the memory it needs.  t3mi_session_begin refuses (T3MI_ERR_ARG) what does not fit the pool, t3mi_session_refill
+ * likewise (T3MI_ERR_STATE, the session is as it was); t3mi_generate_continuous opens as many slots as the pool serves and starts a
+ * waiting utterance when enough pages are free.  Arithmetic is the batched path's (whatever the number of rows); keys and values go through
+ * t3mi_paged_append and are read by t3mi_paged_attention. */
+int t3mi_set_paged_kv(t3mi_model* m, int page_size, int n_pages);
+/* pages of the running session's pool, and how many no utterance holds (0, 0 without pages) */
+int t3mi_session_pages(t3mi_model* m, int32_t* total, int32_t* free_pages);
+/* Rules on an utterance's logits (t3mi_process_logits, after guidance and before the sampler's own penalty): biases, frequency and presence
+ * penalties over the utterance's tokens so far, and the set of tokens that may be drawn.  The reference has none; allowing the ids below
+ * SPEECH_VOCAB_SIZE and the stop token, for one, leaves nothing for drop_invalid_tokens to drop (R/s3tokenizer.R:678-687).  Host arrays, copied. */
+typedef struct t3mi_logit_rules {
+    const int32_t* bias_ids;     /* [n_bias] token ids and the finite values added to their logits (an id named twice: the last)  */
+    const float* bias_values;
+    const uint32_t* allowed;     /* [ceil(vocab / 32)] bits, token t's is bit t & 31 of word t >> 5; NULL: every token.  Some token must be allowed */
+    int32_t n_bias;              /* at most 4094                                             */
+    float frequency_penalty;     /* subtracted once for every time the token has been drawn  */
+    float presence_penalty;      /* subtracted if it has been drawn                          */
+    int32_t reserved_;
+} t3mi_logit_rules;
+/* what every utterance of the sessions and refills to come starts with (NULL: none); the generate entry points use it too */
+int t3mi_set_logit_rules(t3mi_model* m, const t3mi_logit_rules* rules);
+/* the rules of slot `utt` of the running session, from the next enqueued step on (NULL: none); waits for the enqueued steps.  A grammar calls
+ * this between steps of one.  The first rules of a session change what a step launches (its graph is captured again). */
+int t3mi_session_logit_rules(t3mi_model* m, int utt, const t3mi_logit_rules* rules);
+
 /* ---- session API: the same loop in pieces (bench timing, parity hooks) ---------------- */
 
 /* Allocate KV slabs (create_kv_cache, R/llama_traced.R:274-297), upload prompts, run the

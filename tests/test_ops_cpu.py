@@ -91,6 +91,10 @@ def test_bad_logits_calls_are_refused(kw, word):
 
 def test_null_structs_are_refused():
     L = _lib.load()
+    refused(L.t3mi_set_paged_kv(None, 16, 0), "null")
+    refused(L.t3mi_set_logit_rules(None, None), "null")
+    refused(L.t3mi_session_logit_rules(None, 0, None), "null")
+    refused(L.t3mi_session_pages(None, None, None), "null")
     refused(L.t3mi_paged_append(None, append(), None), "null")
     refused(L.t3mi_paged_append(cache(), None, None), "null")
     refused(L.t3mi_paged_attention(cache(), None, None), "null")
