@@ -188,12 +188,13 @@ constexpr int kMaxSplit = 64;      // blocks that share a row's keys at most
 struct RowPlan {
     int first, len, t0, t1, per, active;
 };
-__device__ __forceinline__ RowPlan plan_row(const PagedAttnArgs& a, int row, int s) {
+// len, first, s: the row's entries of lengths (>= 0), starts (or 0) and seq (or the row)
+__device__ __forceinline__ RowPlan plan_row(const PagedAttnArgs& a, int len, int first, int s) {
     RowPlan p;
-    long long n = (long long)a.lengths[row] + a.length_add;
+    long long n = (long long)len + a.length_add;
     const long long most = (long long)a.c.max_pages << a.c.page_shift;
     n = n > most ? most : n;
-    p.first = a.starts ? max(a.starts[row], 0) : 0;
+    p.first = max(first, 0);
     p.len = (s < 0 || s >= a.c.n_seqs) ? 0 : (int)n;
     p.t0 = p.first >> a.tile_shift;
     p.t1 = (p.len + (1 << a.tile_shift) - 1) >> a.tile_shift;
@@ -228,42 +229,48 @@ __global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
     const int q16 = (int)(pair % (unsigned)gt);
     pair /= (unsigned)gt;
     const int hk0 = (int)(pair % (unsigned)hg) * hw, row = (int)(pair / (unsigned)hg);
-    if (a.lengths[row] < 0) return;
-    const int seq = a.seq ? a.seq[row] : row;
-    const RowPlan rp = plan_row(a, row, seq);
-    if ((int)split >= rp.active) return;
+    // what the row is, and its queries, are asked for together, before anything waits
+    const int row_len = a.lengths[row], seq = a.seq ? a.seq[row] : row, row_first = a.starts ? a.starts[row] : 0;
     const int gn = min(16, group - q16 * 16);       // live query heads of a key head in this block
     const bool idle = hk0 + wh >= a.c.kv_heads;     // (a wave past the last key head: no tile, nothing stored)
     const int hk = idle ? a.c.kv_heads - 1 : hk0 + wh;
     const int h0 = hk * group + q16 * 16;
-    const int t_begin = rp.t0 + (int)split * rp.per, t_end = idle ? t_begin : min(rp.t1, t_begin + rp.per);
 
     // queries: lane (n, g) holds, for piece c, elements 32 c + 8 g + j (bf16 cache) or 16 c + 4 g + i (fp32 cache) of head n
+    constexpr int QW = KB && !QB ? 2 : 1;           // 16-byte words of a piece
+    u32x4 qw[KC][QW];
+    {
+        const long long qo = row * a.qr + (long long)(h0 + (n < gn ? n : 0)) * a.qh;
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int w = 0; w < QW; ++w) {
+                if constexpr (QB) qw[c][w] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + qo + 32 * c + 8 * g);
+                else qw[c][w] = *reinterpret_cast<const u32x4*>(static_cast<const float*>(a.q) + qo + (KB ? 32 * c + 8 * g + 4 * w : 16 * c + 4 * g));
+            }
+    }
+    if (row_len < 0) return;
+    const RowPlan rp = plan_row(a, row_len, row_first, seq);
+    if ((int)split >= rp.active) return;
+    const int t_begin = rp.t0 + (int)split * rp.per, t_end = idle ? t_begin : min(rp.t1, t_begin + rp.per);
     bf16x8 qb[KB ? QS : 1][KB ? KC : 1];
     f32x4 qf[KB ? 1 : KC];
     {
         const bool live = n < gn;
-        const long long qo = row * a.qr + (long long)(h0 + (live ? n : 0)) * a.qh;
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
             if constexpr (QB) {
-                u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + qo + 32 * c + 8 * g);
-                if (!live) w = u32x4{0u, 0u, 0u, 0u};
-                qb[0][c] = __builtin_bit_cast(bf16x8, w);
+                qb[0][c] = __builtin_bit_cast(bf16x8, live ? qw[c][0] : u32x4{0u, 0u, 0u, 0u});
             } else if constexpr (KB) {
-                const float* qp = static_cast<const float*>(a.q) + qo + 32 * c + 8 * g;
-                const f32x4 lo = *reinterpret_cast<const f32x4*>(qp), hi = *reinterpret_cast<const f32x4*>(qp + 4);
                 float x[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { x[j] = live ? lo[j] : 0.f; x[4 + j] = live ? hi[j] : 0.f; }
+                for (int j = 0; j < 8; ++j) x[j] = live ? __uint_as_float(qw[c][j >> 2][j & 3]) : 0.f;
                 bf16x8 o[3];
                 to_parts<3>(x, o);
 #pragma unroll
                 for (int s = 0; s < QS; ++s) qb[s][c] = o[s];
             } else {
-                f32x4 w = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + qo + 16 * c + 4 * g);
-                if (!live) w = f32x4{0.f, 0.f, 0.f, 0.f};
-                qf[c] = w;
+                qf[c] = live ? __builtin_bit_cast(f32x4, qw[c][0]) : f32x4{0.f, 0.f, 0.f, 0.f};
             }
         }
     }
@@ -496,8 +503,9 @@ __global__ __launch_bounds__(256) void paged_join_few_kernel(PagedAttnArgs a) {
     const int pair = blockIdx.x * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (pair >= a.rows * a.q_heads) return;
     const int row = pair / a.q_heads, h = pair - row * a.q_heads;
-    if (a.lengths[row] < 0) return;
-    const RowPlan rp = plan_row(a, row, a.seq ? a.seq[row] : row);
+    const int len = a.lengths[row], seq = a.seq ? a.seq[row] : row, first = a.starts ? a.starts[row] : 0;
+    if (len < 0) return;
+    const RowPlan rp = plan_row(a, len, first, seq);
     if (rp.active <= 1) return;
     const long long part = (long long)pair * a.n_split;
     const float2* ml = reinterpret_cast<const float2*>(a.ws + (long long)a.rows * a.q_heads * a.n_split * D) + part;
@@ -541,8 +549,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     __shared__ __attribute__((aligned(16))) float sm_o[NS][D];
     __shared__ float sm_f[kMaxSplit], sm_l;
     const int row = blockIdx.x / a.q_heads, h = blockIdx.x % a.q_heads, tid = threadIdx.x;
-    if (a.lengths[row] < 0) return;
-    const RowPlan rp = plan_row(a, row, a.seq ? a.seq[row] : row);
+    const int len = a.lengths[row], seq = a.seq ? a.seq[row] : row, first = a.starts ? a.starts[row] : 0;
+    if (len < 0) return;
+    const RowPlan rp = plan_row(a, len, first, seq);
     if (rp.active <= 1) return;
     const long long part = (long long)blockIdx.x * a.n_split;
     const int sub = tid / LP, d4 = (tid % LP) * 4;
