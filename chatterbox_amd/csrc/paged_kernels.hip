@@ -372,12 +372,19 @@ __global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
 #pragma unroll
                         for (int u = 0; u < U; ++u) s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[u][c]), qb[part][c], s[u], 0, 0, 0);
             } else {
+                f32x4 part[U][4];                        // four chains: less rounding than one, and none waits for another
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) part[u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < KC; ++c)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int u = 0; u < U; ++u) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, kr[u][c])[i], qf[c][i], s[u], 0, 0, 0);
+                        for (int u = 0; u < U; ++u) part[u][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, kr[u][c])[i], qf[c][i], part[u][i], 0, 0, 0);
+#pragma unroll
+                for (int u = 0; u < U; ++u) s[u] = (part[u][0] + part[u][1]) + (part[u][2] + part[u][3]);
             }
             const Pages next = settle();
             ask(min(t + 2 * kw, t_end - 1));
@@ -390,7 +397,9 @@ __global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
             bool all_in = true;
             if constexpr (PAGES == 0) all_in = pg.ok;
             else all_in = __builtin_amdgcn_ballot_w64(!pg.ok) == 0;
-            if (!(whole && all_in)) {
+            const bool masked = !(whole && all_in);
+            unsigned dead = 0u;                          // bit j: key j of this lane is not to be seen
+            if (masked) {
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
                     const int key = t * TK + 16 * (j >> 2) + 4 * g + (j & 3);
@@ -399,7 +408,7 @@ __global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
                         const int id = key < rp.len ? trow[key >> a.c.page_shift] : -1;
                         live = live && id >= 0 && id < a.c.n_pages;
                     }
-                    p[j] = live ? p[j] : -INFINITY;
+                    if (!live) { p[j] = -INFINITY; dead |= 1u << j; }
 #pragma unroll
                     for (int h = 0; h < VL; ++h)
 #pragma unroll
@@ -417,8 +426,19 @@ __global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
                 for (int e = 0; e < NT; ++e) acc[e] *= keep;
                 m = mx;
             }
+            // Scores of ordinary size: the product with the scale is not rounded before the maximum comes off.  Beyond 2^16 that rounding is what the
+            // maximum itself carries, and has to cancel.
+            if (__builtin_amdgcn_ballot_w64(!(fabsf(ref) < 65536.f)) == 0) {
 #pragma unroll
-            for (int j = 0; j < J; ++j) p[j] = __builtin_amdgcn_exp2f(p[j] - ref);
+                for (int j = 0; j < J; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], scale2, -ref));
+                if (masked) {
+#pragma unroll
+                    for (int j = 0; j < J; ++j) p[j] = (dead >> j) & 1u ? 0.f : p[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < J; ++j) p[j] = __builtin_amdgcn_exp2f(p[j] - ref);
+            }
             if constexpr (U == 2) l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
             else l += (p[0] + p[1]) + (p[2] + p[3]);
             if constexpr (KB) {
