@@ -653,6 +653,12 @@ void launch_attention_d(const PagedAttnArgs& a, unsigned blocks, unsigned thread
 
 }  // namespace
 
+// shared memory of a block: maxima and sums, and the weighted sums of its waves
+static size_t attention_lds(const PagedAttnArgs& a) {
+    const int group = a.q_heads / a.c.kv_heads;
+    return (size_t)a.waves * (32 + (size_t)(group < 16 ? group : 16) * a.c.head_dim) * 4;
+}
+
 void plan_paged_attention(PagedAttnArgs& a) {
     const int group = a.q_heads / a.c.kv_heads, eb = a.c.bf16 ? 2 : 4;
     a.tile_shift = a.c.bf16 ? 5 : 4;
@@ -691,6 +697,7 @@ void plan_paged_attention(PagedAttnArgs& a) {
             a.n_split = (int)std::min((share + a.waves - 1) / a.waves, (long long)(a.waves == 2 ? kMaxSplit / 2 : kMaxSplit));
         }
     }
+    if (attention_lds(a) > 65536) a.waves = 4;   // (8 waves of 16 heads of 128)
     a.min_tiles = 2 * a.waves;
 }
 
@@ -704,7 +711,8 @@ hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s) {
     const long long blocks = (long long)a.rows * ((a.c.kv_heads + a.head_waves - 1) / a.head_waves) * ((group + 15) / 16) * a.n_split;
     if (a.rows <= 0 || a.n_split < 1 || a.n_split > kMaxSplit || a.min_tiles < 1 || a.waves < 1 || a.waves > 8 || blocks > 0x7FFFFFFFLL) return hipErrorInvalidValue;
     if (a.n_split > 1 && a.ws == nullptr) return hipErrorInvalidValue;
-    const size_t lds = (size_t)a.waves * (32 + (size_t)(group < 16 ? group : 16) * a.c.head_dim) * 4;
+    const size_t lds = attention_lds(a);
+    if (lds > 65536) return hipErrorInvalidValue;
     if (a.c.head_dim == 64) launch_attention_d<64>(a, (unsigned)blocks, 64u * a.waves, lds, s);
     else if (a.c.head_dim == 128) launch_attention_d<128>(a, (unsigned)blocks, 64u * a.waves, lds, s);
     else return hipErrorInvalidValue;

@@ -127,6 +127,36 @@ def test_attention_plan_does_not_change_what_is_computed(max_length, q_t, kv_t):
         assert bool((got[r] == 0).all())
 
 
+@pytest.mark.parametrize("q_t,out_t", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("heads,kv_heads,order", [(15, 5, "slots"), (16, 16, "pairs")])
+def test_attention_many_rows_of_neighbouring_heads(q_t, out_t, heads, kv_heads, order):
+    """Enough rows of 128-byte keys that blocks take four neighbouring heads (the last block of 5 heads takes one), whole and split."""
+    rng = np.random.default_rng(kv_heads)
+    rows = 1100 // kv_heads
+    lens = [int(n) for n in rng.integers(0, 80, rows)]
+    lens[3], lens[4], lens[-1] = 0, -1, 700
+    k, v, table, keys, vals = make_cache(lens, 16, kv_heads, 64, "bf16", 21, order)
+    q = torch.randn(rows, heads, 64, generator=torch.Generator().manual_seed(3)).to(DT[q_t]).cuda()
+    lengths = torch.tensor(lens, dtype=torch.int32).cuda()
+    for most in (700, 80):
+        out = torch.full((rows, heads, 64), 5.0, dtype=DT[out_t], device="cuda")
+        cb.paged_attention(q, k, v, table, lengths, out=out, max_length=most)
+        check_rows(out, q, keys, vals, None, range(rows), lens, 0.125, out_t, out_t == "bf16")
+        assert bool((out[4] == 5).all()) and bool((out[3] == 0).all())
+
+
+@pytest.mark.parametrize("q_t,kv_t", [("f32", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("heads", [16, 17, 33])
+def test_attention_wide_groups_over_a_long_row(q_t, kv_t, heads):
+    """One key head for 16 and more query heads of 128: the largest blocks, and groups that end inside a tile of 16."""
+    lens = [9001, 0, 130]
+    k, v, table, keys, vals = make_cache(lens, 128, 1, 128, kv_t, 31)
+    q = torch.randn(3, heads, 128, generator=torch.Generator().manual_seed(4)).to(DT[q_t]).cuda()
+    got = cb.paged_attention(q, k, v, table, torch.tensor(lens, dtype=torch.int32).cuda(), max_length=2 ** 17)
+    check_rows(got, q, keys, vals, None, range(3), lens, 128 ** -0.5, q_t, q_t == "bf16")
+    assert torch.equal(cb.paged_attention(q, k, v, table, torch.tensor(lens, dtype=torch.int32).cuda(), max_length=2 ** 17, out=q), got)   # in place
+
+
 def test_attention_prompt_rows_share_a_sequence():
     """Rows of a prompt: the same sequence at lengths 1, 2, 3, ... , in any order, through `seq`; q and out as strided views."""
     k, v, table, keys, vals = make_cache([70, 9], 16, 2, 64, "bf16", 4)
@@ -465,6 +495,44 @@ def test_logits_match_64_bits(x_t, rows, vocab, cap, n_bias, mask, guide, each):
     assert (np.abs(g[~off] - want[~off]) <= tol[~off]).all()
     cb.process_logits(l, **kw, out=l)                    # in place
     assert torch.equal(l, got)
+
+
+@pytest.mark.parametrize("x_t", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,cap,n_bias", [(300, 12289, 700, 40), (90, 33000, 17000, 1500), (3, 9000, 9000, 4094), (70, 40960, 0, 3)])
+def test_logits_of_many_chunks(x_t, rows, vocab, cap, n_bias):
+    """Blocks of several chunks (tokens sorted, or too many to be), token lists and biases longer than a block holds; vectorised reference."""
+    rng = np.random.default_rng(rows)
+    l = torch.from_numpy((rng.standard_normal((rows, vocab)) * 3).astype(np.float32)).to(DT[x_t]).cuda()
+    tokens = rng.integers(0, vocab, (rows, cap)).astype(np.int32) if cap else None
+    n_tokens = rng.integers(0, cap + 1, rows).astype(np.int32) if cap else None
+    if cap:
+        n_tokens[0] = cap
+    rep, fre, pre = (rng.uniform(lo, hi, rows).astype(np.float32) for lo, hi in ((0.5, 2.0), (0.0, 1.0), (-1.0, 1.0)))
+    ids = rng.integers(0, vocab, (rows, n_bias)).astype(np.int32)
+    ids[:, -1], ids[:, n_bias // 2] = ids[:, 0], ids[:, 0]
+    vals = (rng.standard_normal((rows, n_bias)) * 5).astype(np.float32)
+    allowed = rng.integers(-2 ** 31, 2 ** 31, (rows, (vocab + 31) // 32)).astype(np.int32)
+
+    def dev(x):
+        return None if x is None else torch.from_numpy(x).cuda()
+
+    got = np64(cb.process_logits(l, tokens=dev(tokens), n_tokens=dev(n_tokens), repetition_penalty=dev(rep), frequency_penalty=dev(fre), presence_penalty=dev(pre),
+                                 bias_ids=dev(ids), bias_values=dev(vals), allowed=dev(allowed)))
+    x = np64(l)
+    for r in range(rows):
+        z = x[r].copy()
+        b = dict(zip(ids[r].tolist(), vals[r].tolist()))
+        at = np.fromiter(b, np.int64)
+        z[at] += np.fromiter(b.values(), np.float64)
+        mag = np.abs(x[r]).max() + np.abs(vals).max()
+        if cap:
+            c = np.bincount(tokens[r, : n_tokens[r]], minlength=vocab).astype(np.float64)
+            z = np.where(c > 0, np.where(z > 0, z / np.float64(rep[r]), z * np.float64(rep[r])) - np.float64(fre[r]) * c - np.float64(pre[r]), z)
+            mag = 2 * mag + np.abs(fre[r]) * c.max() * 2 + 1
+        bits = np.unpackbits(allowed[r].view(np.uint8), bitorder="little")[:vocab].astype(bool)
+        tol = 8 * U * mag + (2.0 ** -8 * (np.abs(z) + 8 * U * mag) if x_t == "bf16" else 0.0)
+        assert (np.isneginf(got[r]) == ~bits).all(), r
+        assert (np.abs(got[r] - z)[bits] <= (tol[bits] if x_t == "bf16" else tol)).all(), r
 
 
 def test_logits_without_rules_are_copied_bit_for_bit():
