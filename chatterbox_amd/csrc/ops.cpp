@@ -78,6 +78,8 @@ int take_attention(const char* where, const t3mi_paged_cache* cache, const t3mi_
     if (!at16(a->q) || !at16(a->out) || !steps16(a->q_stride, a->q_dtype) || !steps16(a->out_stride, a->out_dtype))
         return bad(where, "q and out: addresses and strides must be multiples of 16 bytes");
     if (!a->seq && a->rows > cache->n_seqs) return bad(where, "more rows than sequences (seq says which row belongs to which)");
+    if (a->q == a->out && (a->q_dtype != a->out_dtype || a->q_stride[0] != a->out_stride[0] || a->q_stride[1] != a->out_stride[1]))
+        if (a->rows) return bad(where, "out may be q only with the same strides and type");
     o.q = a->q; o.out = a->out;
     o.qr = a->q_stride[0]; o.qh = a->q_stride[1]; o.outr = a->out_stride[0]; o.outh = a->out_stride[1];
     o.lengths = a->lengths; o.starts = a->starts; o.seq = a->seq;
@@ -157,7 +159,7 @@ int t3mi_paged_attention(const t3mi_paged_cache* cache, const t3mi_attention_arg
 int t3mi_process_logits(const t3mi_logits_args* a, void* stream) {
     const char* me = "t3mi_process_logits";
     if (!a) return bad(me, "null arguments");
-    if (a->rows < 0 || a->rows > 65535 || a->vocab <= 0) return bad(me, "rows must be 0..65535, vocab positive");
+    if (a->rows < 0 || a->rows > 65535 || a->vocab <= 0 || a->vocab > (1 << 28)) return bad(me, "rows must be 0..65535, vocab 1..2^28");
     if (!is_type(a->dtype)) return bad(me, "dtype must be T3MI_W_F32 or T3MI_W_BF16");
     if (a->rows && (!a->logits || !a->out)) return bad(me, "null logits or out");
     const uintptr_t low = a->dtype == T3MI_W_BF16 ? 1u : 3u;

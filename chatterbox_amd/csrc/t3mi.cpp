@@ -1469,6 +1469,7 @@ int upload_rules(t3mi_model* m, Session* s, int u) {
 // step launches: the captured graph is dropped and the next step captures another.
 int set_slot_rules(t3mi_model* m, Session* s, const std::vector<int>& utts, const LogitRules& r) {
     if (!s->rules && !r.any()) return T3MI_OK;
+    if (s->cap > 1048575) return fail(T3MI_ERR_ARG, "logit rules: a session under rules may have at most 1048575 tokens an utterance");
     s->slot_rules.resize(s->n_utt);
     for (int u : utts) s->slot_rules[u] = r;
     int rc;

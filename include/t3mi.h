@@ -431,7 +431,7 @@ int t3mi_paged_append(const t3mi_paged_cache* cache, const t3mi_append_args* arg
  * lengths[r] + length_add) of sequence seq[r], head h reading key head h / (q_heads / kv_heads).  Row r of a prompt's queries attends
  * causally when lengths[r] is its position and length_add 1.  A row with no key is written as zeros, a row whose length is negative is left as it
  * was (padding of a batch); lengths beyond the block table end there.  Types: q fp32 over an fp32 or bf16 cache, q bf16 over a bf16
- * cache; out fp32 or bf16. */
+ * cache; out fp32 or bf16, and q itself only with q's type and strides. */
 typedef struct t3mi_attention_args {
     const void* q;               /* [rows, q_heads, head_dim]; strides (row, head)           */
     void* out;
@@ -475,7 +475,7 @@ typedef struct t3mi_logits_args {
     const uint32_t* allowed;     /* [rows, >= ceil(vocab / 32)] or NULL                      */
     int64_t allowed_stride;
     float cfg_weight, repetition, frequency, presence;
-    int32_t rows, vocab, dtype;
+    int32_t rows, vocab, dtype;  /* rows at most 65535, vocab at most 2^28                   */
     int32_t token_cap;           /* at most 1048575                                          */
     int32_t n_bias;              /* at most 4094                                             */
     int32_t device;

@@ -33,7 +33,7 @@ def append(**kw):
 
 
 def attention(**kw):
-    a = _lib.AttentionArgs(q=P, out=P, lengths=P, workspace=P, workspace_bytes=1 << 30, scale=0.125, rows=3, q_heads=4, q_dtype=_lib.W_F32, out_dtype=_lib.W_F32)
+    a = _lib.AttentionArgs(q=P, out=P if "out_stride" in kw or "out_dtype" in kw else 2 * P, lengths=P, workspace=P, workspace_bytes=1 << 30, scale=0.125, rows=3, q_heads=4, q_dtype=_lib.W_F32, out_dtype=_lib.W_F32)
     a.q_stride[:] = a.out_stride[:] = (256, 64)
     return put(a, kw)
 
@@ -72,7 +72,8 @@ def test_bad_appends_are_refused(kw, word):
 @pytest.mark.parametrize("kw,word", [(dict(rows=-2), "q_heads"), (dict(q_heads=3), "multiple"), (dict(q_heads=0), "multiple"), (dict(q_dtype=5), "dtypes"),
                                      (dict(q_dtype=_lib.W_BF16), "bf16 cache"), (dict(length_add=2), "length_add"), (dict(max_length=-1), "max_length"),
                                      (dict(scale=float("inf")), "finite"), (dict(q=None), "null"), (dict(lengths=None), "null"), (dict(out=P + 4), "16 bytes"),
-                                     (dict(out_stride=(256, 63)), "16 bytes"), (dict(rows=4), "sequences"), (dict(rows=1 << 23, seq=P), "pairs")])
+                                     (dict(out_stride=(256, 63)), "16 bytes"), (dict(rows=4), "sequences"), (dict(rows=1 << 23, seq=P), "pairs"), (dict(out_stride=(512, 64)), "same strides"),
+                                     (dict(out_dtype=_lib.W_BF16), "same strides")])
 def test_bad_attentions_are_refused(kw, word):
     L = _lib.load()
     refused(L.t3mi_paged_attention(cache(), attention(**kw), None), word)
@@ -80,7 +81,7 @@ def test_bad_attentions_are_refused(kw, word):
     refused(L.t3mi_paged_attention_workspace(cache(), attention(**kw), n), word)
 
 
-@pytest.mark.parametrize("kw,word", [(dict(rows=-1), "rows"), (dict(rows=65536), "rows"), (dict(vocab=0), "vocab"), (dict(dtype=3), "dtype"), (dict(out=None), "null"),
+@pytest.mark.parametrize("kw,word", [(dict(rows=-1), "rows"), (dict(rows=65536), "rows"), (dict(vocab=0), "vocab"), (dict(vocab=(1 << 28) + 1), "vocab"), (dict(dtype=3), "dtype"), (dict(out=None), "null"),
                                      (dict(logits=P + 2), "aligned"), (dict(out_stride=99), "overlap"), (dict(logits_stride=128, out=P, out_stride=100), "same stride"),
                                      (dict(n_tokens=None), "n_tokens"), (dict(token_cap=1 << 20), "token_cap"), (dict(n_bias=5), "n_bias"),
                                      (dict(n_bias=4095, bias_ids=P, bias_values=P), "n_bias"), (dict(repetition=0.0), "repetition"),
