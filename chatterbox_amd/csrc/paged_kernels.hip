@@ -182,6 +182,10 @@ template <int PARTS> __device__ __forceinline__ void to_parts(const float (&x)[8
     }
 }
 
+// what a part's sums count, its maximum being m and that of all parts top.  A part without a maximum saw no key, and its sums are 0, or it saw
+// NaN scores alone, and they are NaN: taken as they are
+__device__ __forceinline__ float part_factor(float m, float top) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 1.f; }
+
 constexpr int kMaxSplit = 64;      // blocks that share a row's keys at most
 
 // which keys of a row a block works on: key tiles [t0, t1) of 1 << tile_shift, shared by `active` blocks of at most `per` tiles each
@@ -482,7 +486,7 @@ __global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
     float top = -INFINITY;
     for (int w = wh; w < nw; w += hw) top = fmaxf(top, sm_m[w * 16 + n]);
     if (n < gn) {
-        const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.f;
+        const float f = part_factor(m, top);
         float* o = sm_o + (wave * gn + n) * D;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -503,7 +507,7 @@ __global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
         for (int w = ho; w < nw; w += hw) {
             const float mw = sm_m[w * 16 + hn];
-            sum += mw > -INFINITY ? sm_l[w * 16 + hn] * __builtin_amdgcn_exp2f(mw - big) : 0.f;
+            sum += sm_l[w * 16 + hn] * part_factor(mw, big);
             o += *reinterpret_cast<const f32x4*>(sm_o + (w * gn + hn) * D + d4);
         }
         if (rp.active > 1) {
@@ -544,7 +548,7 @@ __global__ __launch_bounds__(256) void paged_join_few_kernel(PagedAttnArgs a) {
     for (int s = 1; s < 8; ++s) big = fmaxf(big, x[s].x);
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-        f[s] = x[s].x > -INFINITY ? __builtin_amdgcn_exp2f(x[s].x - big) : 0.f;
+        f[s] = part_factor(x[s].x, big);
         sum += x[s].y * f[s];
     }
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -581,7 +585,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
         float big = x.x;
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
-        const float f = x.x > -INFINITY ? __builtin_amdgcn_exp2f(x.x - big) : 0.f;
+        const float f = part_factor(x.x, big);
         sm_f[tid] = f;
         float sum = x.y * f;
 #pragma unroll

@@ -157,6 +157,37 @@ def test_attention_wide_groups_over_a_long_row(q_t, kv_t, heads):
     assert torch.equal(cb.paged_attention(q, k, v, table, torch.tensor(lens, dtype=torch.int32).cuda(), max_length=2 ** 17, out=q), got)   # in place
 
 
+@pytest.mark.parametrize("q_t,kv_t", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("most", [64, 20000])
+def test_attention_passes_on_nan(q_t, kv_t, most):
+    """NaN in a query, a live key or a live value comes out, as the formula has it, in one block and split over many; other rows and heads keep theirs."""
+    lens = [3000, 33, 3000, 700, 1]
+    k, v, table, keys, vals = make_cache(lens, 16, 2, 64, kv_t, 41)
+    q = torch.randn(5, 4, 64, generator=torch.Generator().manual_seed(5)).to(DT[q_t])
+    q[0, 1, 7] = float("nan")
+    q[1, 2] = float("nan")
+    q[4, 3, 0] = float("nan")
+    q = q.cuda()
+    at = 2900
+    page, slot = int(table[2, at // 16]), at % 16
+    k[page, slot, 0, 3] = float("nan")
+    v[page, slot, 1, 5] = float("nan")
+    lengths = torch.tensor(lens, dtype=torch.int32).cuda()
+    got = cb.paged_attention(q, k, v, table, lengths, max_length=most)
+    for r, h in ((0, 1), (1, 2), (4, 3), (2, 0), (2, 1)):
+        assert bool(got[r, h].isnan().all()), (r, h)
+    for h in (2, 3):
+        nan = got[2, h].isnan()
+        assert bool(nan[5]) and int(nan.sum()) == 1
+    rest = torch.ones(5, 4, dtype=torch.bool)
+    for r, h in ((0, 1), (1, 2), (4, 3), (2, 0), (2, 1), (2, 2), (2, 3)):
+        rest[r, h] = False
+    clean = torch.nan_to_num(q)
+    k[page, slot, 0, 3] = 0
+    v[page, slot, 1, 5] = 0
+    assert torch.equal(got[rest], cb.paged_attention(clean, k, v, table, lengths, max_length=most)[rest])
+
+
 def test_attention_prompt_rows_share_a_sequence():
     """Rows of a prompt: the same sequence at lengths 1, 2, 3, ... , in any order, through `seq`; q and out as strided views."""
     k, v, table, keys, vals = make_cache([70, 9], 16, 2, 64, "bf16", 4)
