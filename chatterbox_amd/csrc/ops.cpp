@@ -11,7 +11,15 @@ int t3mi_set_error(int code, const std::string& msg);   // t3mi.cpp
 
 namespace {
 
-int bad(const char* where, const char* what) { return t3mi_set_error(T3MI_ERR_ARG, std::string(where) + ": " + what); }
+// (no exception leaves these: without memory for its text an error keeps its code)
+int say(int code, const char* where, const char* what) {
+    try {
+        return t3mi_set_error(code, std::string(where) + ": " + what);
+    } catch (...) {
+        return code;
+    }
+}
+int bad(const char* where, const char* what) { return say(T3MI_ERR_ARG, where, what); }
 
 // the operators' device, for the length of a call; the caller's current device afterwards
 struct OnDevice {
@@ -28,7 +36,7 @@ struct OnDevice {
 
 int done(const char* where, hipError_t e) {
     if (e == hipSuccess) return T3MI_OK;
-    return t3mi_set_error(T3MI_ERR_HIP, std::string(where) + ": " + hipGetErrorString(e));
+    return say(T3MI_ERR_HIP, where, hipGetErrorString(e));
 }
 
 bool is_type(int t) { return t == T3MI_W_F32 || t == T3MI_W_BF16; }
@@ -38,6 +46,24 @@ bool step16(int64_t s, int dtype) { return s >= 0 && ((s * (dtype == T3MI_W_BF16
 template <int N> bool steps16(const int64_t (&s)[N], int dtype) {
     for (int i = 0; i < N; ++i)
         if (!step16(s[i], dtype)) return false;
+    return true;
+}
+
+// whether what is written through N strides never falls on itself: sorted by stride, each dimension steps over all that lies within it
+template <int N> bool disjoint(const int64_t (&stride)[N], const int64_t (&count)[N], int64_t inner) {
+    int by[N];
+    for (int i = 0; i < N; ++i) {
+        int j = i;
+        for (; j > 0 && stride[by[j - 1]] > stride[i]; --j) by[j] = by[j - 1];
+        by[j] = i;
+    }
+    int64_t extent = inner;
+    for (int i = 0; i < N; ++i) {
+        if (count[by[i]] <= 1) continue;
+        if (stride[by[i]] < extent) return false;
+        if (stride[by[i]] > (INT64_MAX - extent) / (count[by[i]] - 1)) return true;   // (past any address)
+        extent += stride[by[i]] * (count[by[i]] - 1);
+    }
     return true;
 }
 
@@ -80,6 +106,7 @@ int take_attention(const char* where, const t3mi_paged_cache* cache, const t3mi_
     if (!a->seq && a->rows > cache->n_seqs) return bad(where, "more rows than sequences (seq says which row belongs to which)");
     if (a->q == a->out && (a->q_dtype != a->out_dtype || a->q_stride[0] != a->out_stride[0] || a->q_stride[1] != a->out_stride[1]))
         if (a->rows) return bad(where, "out may be q only with the same strides and type");
+    if (!disjoint<2>(a->out_stride, {a->rows, a->q_heads}, cache->head_dim)) return bad(where, "the rows and heads of out must not overlap");
     o.q = a->q; o.out = a->out;
     o.qr = a->q_stride[0]; o.qh = a->q_stride[1]; o.outr = a->out_stride[0]; o.outh = a->out_stride[1];
     o.lengths = a->lengths; o.starts = a->starts; o.seq = a->seq;
@@ -117,6 +144,10 @@ int t3mi_paged_append(const t3mi_paged_cache* cache, const t3mi_append_args* a, 
     if (!a->seq && a->rows > cache->n_seqs) return bad(me, "more rows than sequences (seq says which row belongs to which)");
     if ((int64_t)a->rows * ((a->q ? a->q_heads : 0) + 2LL * cache->kv_heads) > 0x8000000LL) return bad(me, "at most 2^27 (row, head) pairs a call");
     if (a->rows == 0) return T3MI_OK;
+    if (a->q && !disjoint<2>(a->q_out_stride, {a->rows, a->q_heads}, cache->head_dim)) return bad(me, "the rows and heads of q_out must not overlap");
+    if (!disjoint<3>(cache->k_stride, {cache->n_pages, cache->page_size, cache->kv_heads}, cache->head_dim) ||
+        !disjoint<3>(cache->v_stride, {cache->n_pages, cache->page_size, cache->kv_heads}, cache->head_dim) || cache->k == cache->v)
+        return bad(me, "the pages, slots and heads of the cache must not overlap");
     o.k = a->k; o.v = a->v; o.q = a->q; o.q_out = a->q_out;
     o.kr = a->k_stride[0]; o.kh = a->k_stride[1]; o.vr = a->v_stride[0]; o.vh = a->v_stride[1];
     o.qr = a->q_stride[0]; o.qh = a->q_stride[1]; o.qor = a->q_out_stride[0]; o.qoh = a->q_out_stride[1];

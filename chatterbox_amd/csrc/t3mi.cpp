@@ -1465,11 +1465,14 @@ int upload_rules(t3mi_model* m, Session* s, int u) {
     return T3MI_OK;
 }
 
+constexpr int kRuleTokens = 1048575;   // (process_logits counts a token's occurrences in 20 bits)
+const char* const kRuleTokensText = "logit rules: a session under rules may have at most 1048575 tokens an utterance";
+
 // the rules of slots `utts` change (the stream is idle).  The first rules of a session, and more biases than its buffers hold, change what a
 // step launches: the captured graph is dropped and the next step captures another.
 int set_slot_rules(t3mi_model* m, Session* s, const std::vector<int>& utts, const LogitRules& r) {
     if (!s->rules && !r.any()) return T3MI_OK;
-    if (s->cap > 1048575) return fail(T3MI_ERR_ARG, "logit rules: a session under rules may have at most 1048575 tokens an utterance");
+    if (s->cap > kRuleTokens) return fail(T3MI_ERR_ARG, kRuleTokensText);
     s->slot_rules.resize(s->n_utt);
     for (int u : utts) s->slot_rules[u] = r;
     int rc;
@@ -2441,6 +2444,7 @@ int t3mi_session_refill(t3mi_model* m, int n, const int32_t* utts, const float* 
     HIPCHK(hipSetDevice(m->device));
     hipStream_t st = m->stream;
     HIPCHK(hipStreamSynchronize(st));   // the steps enqueued so far are over: the slots' tokens were the caller's to read before this call
+    if ((s->rules || m->rules.any()) && s->cap > kRuleTokens) return fail(T3MI_ERR_ARG, kRuleTokensText);   // (before anything is given up)
     if (s->paged) {
         // the pages of the slots that are refilled, and of every other slot whose utterance has ended, go back to the pool first
         std::vector<int32_t> over(s->n_utt);

@@ -76,6 +76,6 @@ def process_logits(logits, *, uncond=None, cfg_weight: float = 0.0, tokens=None,
     allowed: bit t % 32 of allowed[r, t // 32] (int32 words) is 0: z = -inf, whatever it was.
 
     bias_ids / bias_values [rows or 1, n] and allowed [rows or 1, words]: one row serves all.  A row that allows nothing is all -inf.
-    Returns out (new by default; may be logits itself)."""
+    Returns out (new by default; may be logits itself, and shares memory with no other argument)."""
     return (_ops or _bind()).logits(logits, uncond, cfg_weight, tokens, n_tokens, repetition_penalty, frequency_penalty, presence_penalty,
                                     bias_ids, bias_values, allowed, out)

@@ -410,7 +410,8 @@ typedef struct t3mi_paged_cache {
  * head_dim / 2] fp32, 4-byte aligned) keys and queries are rotated by their position's angle on the way, element i with element
  * i + head_dim / 2 (apply_rotary_pos_emb, R/llama.R:155-188): (a, b) -> (a cos - b sin, b cos + a sin); the rotated queries go to
  * q_out (may be q itself, with the same strides).  A row whose position is negative, beyond the tables or on no page is skipped: neither
- * the cache nor its q_out row is written.  No two rows of a call may name the same place. */
+ * the cache nor its q_out row is written.  No two rows of a call may name the same place, and no two elements of the cache or of q_out may be
+ * the same memory. */
 typedef struct t3mi_append_args {
     const void* k;               /* [rows, kv_heads, head_dim], type dtype; strides (row, head) */
     const void* v;
@@ -457,7 +458,7 @@ int t3mi_paged_attention(const t3mi_paged_cache* cache, const t3mi_attention_arg
  *   z -= frequency * occurrences + presence        likewise
  *   z = -inf                                       where bit (t & 31) of allowed[r, t >> 5] is 0, whatever z was
  * A row whose mask allows nothing is all -inf.  Row strides are in elements; 0 shares one bias list or mask among the rows.  out may
- * be logits.  Addresses are aligned to their elements only. */
+ * be logits (with the same stride) and shares memory with no other argument.  Addresses are aligned to their elements only. */
 typedef struct t3mi_logits_args {
     const void* logits;          /* [rows, vocab]                                            */
     const void* uncond;          /* [rows, vocab] or NULL                                    */

@@ -640,3 +640,85 @@ def test_work_on_another_stream_is_ordered_with_it():
             v.fill_(-1.0)
             st.synchronize()
             assert torch.allclose(kept, torch.full_like(kept, float(i)), rtol=4100 * U, atol=0)
+
+
+def small_calls(seed):
+    """One call of each operator over a ragged cache, and what they give."""
+    k, v, table, _, _ = make_cache([700, 3, 1200], 16, 2, 64, "bf16", seed)
+    gen = torch.Generator().manual_seed(seed)
+    q, kn, vn = (torch.randn(3, h, 64, generator=gen).cuda() for h in (4, 2, 2))
+    lengths = torch.tensor([700, 3, 1200], dtype=torch.int32).cuda()
+    pos = lengths - 1
+    l = torch.randn(5, 9001, generator=gen).cuda()
+    tok = torch.randint(0, 9001, (5, 40), generator=gen).int().cuda()
+    n_tok = torch.tensor([40, 0, 7, 1, 40], dtype=torch.int32).cuda()
+
+    def run():
+        turned = cb.paged_kv_append(kn, vn, k, v, table, pos, q=q)
+        out = cb.paged_attention(turned, k, v, table, lengths, max_length=1200)
+        return out, cb.process_logits(l, tokens=tok, n_tokens=n_tok, repetition_penalty=1.3, frequency_penalty=0.25)
+
+    return run, (q, kn, vn, k, v, table, pos, lengths, l, tok, n_tok)
+
+
+def test_calls_from_two_threads_on_two_streams():
+    """The lock of the interpreter is given up while a call enqueues: two loops side by side get what each gets alone."""
+    import threading
+    runs = [small_calls(s)[0] for s in (1, 2)]
+    want = [r() for r in runs]
+    torch.cuda.synchronize()
+    streams, wrong = [torch.cuda.Stream() for _ in runs], []
+
+    def loop(i):
+        try:
+            with torch.cuda.stream(streams[i]):
+                for _ in range(200):
+                    got = runs[i]()
+                streams[i].synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+                for _ in range(20):
+                    try:
+                        cb.process_logits(torch.zeros(2, 10, device="cuda"), repetition_penalty=0.0)
+                        wrong.append("no refusal")
+                    except RuntimeError as e:
+                        if "repetition" not in str(e):
+                            wrong.append(str(e))
+        except BaseException as e:
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=loop, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
+
+
+def test_calls_and_refusals_keep_no_reference():
+    import sys
+    run, tensors = small_calls(3)
+    q, kn, vn, k, v, table, pos, lengths, l, tok, n_tok = tensors
+    objects = list(tensors) + [torch.float32, torch.bfloat16, torch.int32, torch.uint8, q.device]
+
+    def refusals():
+        for bad in (lambda: cb.paged_attention(q, k, v, table, lengths[:2]), lambda: cb.paged_attention(q, k, v, table, lengths, out=q[:2]),
+                    lambda: cb.paged_attention(q, k, v, table, lengths, out_dtype=torch.float16), lambda: cb.paged_attention(q[:, :3], k, v, table, lengths),
+                    lambda: cb.paged_attention(q, k, v, table, lengths, scale=float("nan")), lambda: cb.paged_kv_append(kn, vn, k, v, table, pos, q=q, q_out=q[:1]),
+                    lambda: cb.paged_kv_append(kn, vn, k, v, table, pos.cpu()), lambda: cb.process_logits(l, tokens=tok), lambda: cb.process_logits(l, out=l[:2]),
+                    lambda: cb.process_logits(l, repetition_penalty=0.0), lambda: cb.process_logits(l, allowed=tok)):
+            with pytest.raises((ValueError, RuntimeError)):
+                bad()
+
+    for _ in range(3):
+        run()
+        refusals()
+    torch.cuda.synchronize()
+    before, memory = [sys.getrefcount(o) for o in objects], torch.cuda.memory_allocated()
+    for _ in range(30):
+        run()
+        refusals()
+    torch.cuda.synchronize()
+    after = [sys.getrefcount(o) for o in objects]
+    assert all(abs(a - b) <= 5 for a, b in zip(after, before)), list(zip(before, after))   # (30 turns: a reference kept once a turn shows)
+    assert torch.cuda.memory_allocated() == memory

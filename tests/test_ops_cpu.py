@@ -33,7 +33,7 @@ def append(**kw):
 
 
 def attention(**kw):
-    a = _lib.AttentionArgs(q=P, out=P if "out_stride" in kw or "out_dtype" in kw else 2 * P, lengths=P, workspace=P, workspace_bytes=1 << 30, scale=0.125, rows=3, q_heads=4, q_dtype=_lib.W_F32, out_dtype=_lib.W_F32)
+    a = _lib.AttentionArgs(q=P, out=P, lengths=P, workspace=P, workspace_bytes=1 << 30, scale=0.125, rows=3, q_heads=4, q_dtype=_lib.W_F32, out_dtype=_lib.W_F32)
     a.q_stride[:] = a.out_stride[:] = (256, 64)
     return put(a, kw)
 
@@ -67,6 +67,16 @@ def test_bad_caches_are_refused(kw, word):
                                      (dict(q_out_stride=(512, 64)), "same strides"), (dict(rows=4), "sequences"), (dict(rows=1 << 27, seq=P), "pairs")])
 def test_bad_appends_are_refused(kw, word):
     refused(_lib.load().t3mi_paged_append(cache(), append(**kw), None), word)
+
+
+def test_outputs_that_overlap_are_refused():
+    """Written tensors whose strides put two elements in one place: a broadcast row or head, heads closer than head_dim, a shared page."""
+    L = _lib.load()
+    for stride in ((0, 64), (256, 0), (64, 64), (128, 64), (32, 256)):
+        refused(L.t3mi_paged_attention(cache(), attention(rows=3, q_heads=4, out=2 * P, out_stride=stride), None), "out must not overlap")
+        refused(L.t3mi_paged_append(cache(v=2 * P), append(rows=3, q_heads=4, q_out=2 * P, q_out_stride=stride), None), "q_out must not overlap")
+    for kw in (dict(k_stride=(0, 128, 64)), dict(v_stride=(1024, 64, 64)), dict(k_stride=(2048, 128, 32)), dict(v=P)):
+        refused(L.t3mi_paged_append(cache(**{"v": 2 * P, **kw}), append(), None), "cache must not overlap")
 
 
 @pytest.mark.parametrize("kw,word", [(dict(rows=-2), "q_heads"), (dict(q_heads=3), "multiple"), (dict(q_heads=0), "multiple"), (dict(q_dtype=5), "dtypes"),
