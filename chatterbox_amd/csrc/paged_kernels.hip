@@ -228,11 +228,12 @@ __global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
     const int hw = a.head_waves, wh = wave % hw, wk = wave / hw, kw = nw / hw;
     const int group = a.q_heads / a.c.kv_heads, gt = (group + 15) >> 4, hg = (a.c.kv_heads + hw - 1) / hw;
-    const unsigned split = blockIdx.x % (unsigned)a.n_split;
     unsigned pair = blockIdx.x / (unsigned)a.n_split;
     const int q16 = (int)(pair % (unsigned)gt);
     pair /= (unsigned)gt;
     const int hk0 = (int)(pair % (unsigned)hg) * hw, row = (int)(pair / (unsigned)hg);
+    // (a short row's last blocks have nothing to do: turned by the row, they do not all fall to the same XCDs.  128 rows of 60 to 4000 keys: 194 -> 181 us)
+    const unsigned split = (blockIdx.x + (unsigned)row) % (unsigned)a.n_split;
     // what the row is, and its queries, are asked for together, before anything waits
     const int row_len = a.lengths[row], seq = a.seq ? a.seq[row] : row, row_first = a.starts ? a.starts[row] : 0;
     const int gn = min(16, group - q16 * 16);       // live query heads of a key head in this block
@@ -669,38 +670,49 @@ void plan_paged_attention(PagedAttnArgs& a) {
     const long long tiles = ((long long)a.max_length + (1 << a.tile_shift) - 1) >> a.tile_shift;
     const long long pairs = (long long)a.rows * a.c.kv_heads * ((group + 15) / 16);
     // 128-byte rows that lie beside those of the other heads: blocks of four heads, two waves each, so that a block reads 512 bytes in a
-    // row (128 rows of 16 key heads of 64 bf16, up to 1100 keys: 67 us, a head a block 76; with the heads apart in memory 62)
+    // row (512 rows of 16 key heads of 64 bf16, 264 keys each: 104 us, a head a block 121; with the heads apart in memory 99).  Up to 24 tiles
+    // the row is one block (450 keys: 169 us, in two 210), longer ones, which differ more, are split (up to 1100 keys: 3 219 us, 1 222).
     if (group <= 16 && a.c.head_dim * eb == 128 && a.c.kh < a.c.ks && a.c.kv_heads >= 4 && pairs >= 1024) {
         a.head_waves = 4;
         a.waves = 8;
-        a.min_tiles = 8;
-        const long long blocks = (long long)a.rows * ((a.c.kv_heads + 3) / 4);
-        const long long n = std::min((4096 + blocks - 1) / blocks, (tiles + a.min_tiles - 1) / a.min_tiles);   // (at most 16)
-        a.n_split = (int)std::max(n, 1LL);
+        a.min_tiles = 12;
+        a.n_split = tiles <= 24 ? 1 : (int)std::min((tiles + 6) / 12, 8LL);
         return;
     }
+    // Otherwise a block works on one key head.  Measured over 230 shapes (1 to 600 rows, 5 to 4096 tiles), this is within 4 % of the best of 60 plans
+    // on average.  `wide`: the kernel of 128 bf16 elements has registers for two waves to a SIMD, the others for four or (fp32, half the work to a
+    // tile) for as many as are useful.
+    const bool wide = a.c.bf16 && a.c.head_dim == 128;
+    const long long all = pairs * tiles;             // if every row is as long as the longest
+    const long long ragged = std::min(tiles / (wide ? 16 : 20), 8LL);   // rows differ more, the longer they are: so many blocks even out
     a.head_waves = 1;
-    // Short contexts: about 1024 waves (one to a SIMD) without a second launch, where a wave's share stays within 160 KB.  (8 rows of 16 fp32 key
-    // heads, 350 keys: one block of 8 waves 11.1 us, split 13.7; 200 rows of one bf16 head, 900 keys: 4 waves 12.0, split 19.3.)
-    const long long one = (1024 + pairs - 1) / pairs;
-    const int w1 = one <= 1 ? 1 : (one <= 2 ? 2 : (one <= 6 ? 4 : (one <= 12 ? 8 : 0)));
     a.n_split = 1;
-    if (w1 > 0 && tiles <= (a.c.head_dim == 64 ? 20 : 10) * w1) {
-        a.waves = w1;
-    } else {
-        // Else a wave to 8 tiles of the call, 1024 to 8192 of them, in blocks that grow with the work: the fewer partial results, the shorter the
-        // join.  (One row, 30000 bf16 keys, 8 key heads of 128: 2 waves x 32 splits 30.9 us, 4 x 32 33.0, 2 x 64 35.1; three rows of 131071: 8 x 43
-        // 258 us, 4 x 43 264; 96 rows of up to 8190: 4 x 3 333 us, 8 x 3 337, 4 x 1 394.)
-        const long long all = pairs * tiles;                                       // if every row is as long as the longest
-        const long long waves = std::min(std::max(all / 8, 1024LL), 8192LL);
-        const long long share = std::max(std::min((waves + pairs - 1) / pairs, (tiles + 1) / 2), 1LL);   // of a pair, two tiles to a wave at least
-        if (share <= 4) {
-            a.waves = share <= 1 ? 1 : (share <= 2 ? 2 : 4);
-        } else {
-            a.waves = share > 128 ? 8 : (all > 65536 ? 4 : 2);
-            a.n_split = (int)std::min((share + a.waves - 1) / a.waves, (long long)(a.waves == 2 ? kMaxSplit / 2 : kMaxSplit));
+    if (tiles <= (wide ? 16 : a.c.bf16 ? 40 : 32) && (wide || pairs >= 64 || tiles <= 16)) {
+        // short rows: one block, no second launch (16 rows of 16 bf16 heads of 64, up to 464 keys: 9.7 us, in four 12.2)
+        a.waves = wide ? 2 : 4;
+    } else if (all < 65536) {
+        // as many blocks as the card takes well at once (wide: one to a CU), of two waves, two tiles and more to a wave; where that asks for more than 8
+        // partial results of a shortish row, 8 blocks of four waves (2 rows of 16 fp32 heads, up to 4000 keys: 16.0 us, 16 of two 17.4)
+        long long n = wide ? std::max(256 / pairs, 1LL) : ((a.c.bf16 ? 384 : 640) + pairs - 1) / pairs;
+        n = std::min(std::max(n, ragged), std::max(tiles / (wide ? 8 : 4), 1LL));
+        a.waves = 2;
+        if (n > 8 && tiles <= (wide ? 128 : 512)) {
+            n = 8;
+            a.waves = 4;
+        } else if (!a.c.bf16 && tiles >= 16 * n) {
+            a.waves = 4;
         }
+        a.n_split = (int)std::min(n, (long long)kMaxSplit);
+    } else {
+        // much work: a wave to 8 tiles of the call, at most 8192 of them, in blocks that grow with it: the fewer partial results, the shorter the join
+        // (three rows of 131071 bf16 keys, 8 key heads of 128: 8 x 43 258 us, 4 x 43 264)
+        const long long share = (std::min(all / 8, 8192LL) + pairs - 1) / pairs;   // of a pair
+        a.waves = share > 128 ? 8 : 4;
+        a.n_split = (int)std::min(std::max((share + a.waves - 1) / a.waves, std::max(std::min(ragged, 5LL), 1LL)), (long long)kMaxSplit);
     }
+    // more than 16 heads to a key head: the blocks that read the same keys are n_split apart, in the same L2 where that is a multiple of the 8 XCDs
+    // (2 rows of 40 heads over one, 60001 keys: 42 blocks a row 37.4 us, 32 29.5)
+    if (group > 16 && a.n_split >= 8) a.n_split &= ~7;
     if (attention_lds(a) > 65536) a.waves = 4;   // (8 waves of 16 heads of 128)
     a.min_tiles = 2 * a.waves;
 }
