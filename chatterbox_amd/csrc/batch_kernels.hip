@@ -685,7 +685,7 @@ template <typename T> __device__ __forceinline__ float act_tanh(float v) {
 // Everything the epilogues READ from global memory is fetched before their first store: the stores may alias the
 // tables as far as the compiler knows, so a load inside the store loop waits for the previous store and the loop
 // runs at one memory latency per row (qkv at 1024 rows: 6.5 us of epilogue for 16 rows per lane).
-struct EpiRow { int pos, crow; };          // cache position and cache row of an activation row (EPI_ROPE_KV)
+struct EpiRow { int pos, crow; };          // cache position and cache row (or page) of an activation row (EPI_ROPE_KV)
 struct EpiCol { float b0, b1; };           // bias of the two partner features of a column (0 without bias)
 
 template <int EPI>
@@ -694,6 +694,10 @@ __device__ __forceinline__ EpiRow rows_pos(const GemmArgs& a, int mi) {
     if (EPI == EPI_ROPE_KV && mi < a.M) {
         e.pos = a.posmap[mi];
         if (a.rowmap) e.crow = a.rowmap[mi];
+        if (a.page_table != nullptr && e.pos >= 0) {
+            e.crow = a.page_table[(size_t)e.crow * a.page_stride + (e.pos >> a.page_shift)];
+            if (e.crow < 0 || e.crow >= a.n_pages) e.pos = -1;
+        }
     }
     return e;
 }
@@ -772,7 +776,7 @@ __device__ __forceinline__ void rows_epilogue(const GemmArgs& a, int tile, int n
             float* q = a.q + (size_t)mi * (H * kHeadDim) + head * kHeadDim;
             q[i] = lo; q[i + 32] = hi;
         } else {
-            const size_t co = (((size_t)er.crow * H + head) * a.max_len + pos) * kHeadDim;
+            const size_t co = (((size_t)er.crow * H + head) * a.max_len + (pos & a.slot_mask)) * kHeadDim;
             if (a.kv_bf16) {
                 uint16_t* cb = static_cast<uint16_t*>(kind == 1 ? a.kcache : a.vcache) + co;
                 cb[i] = f2bf(lo); cb[i + 32] = f2bf(hi);
@@ -1756,6 +1760,9 @@ int gemm_as_plan(int M, int N, int K, int epilogue, bool splittable, int* gz_out
     return as_four(tiles32, chunks, gz) ? 4 : 2;
 }
 
+// whether launch_gemm writes EPI_ROPE_KV into pages for M rows of K: every kernel but the 16-feature one (fp32 operands below 64 rows)
+bool gemm_takes_pages(int M, int K, int wdtype) { return (wdtype == 1 || (wdtype == 0 && M >= 64)) && K % 256 == 0; }
+
 hipError_t launch_gemm(const GemmArgs& a, int epilogue, int wdtype, hipStream_t s) {
     if (!a.W || !a.A || a.M <= 0 || a.N <= 0 || a.K <= 0) return hipErrorInvalidValue;
     if ((epilogue == EPI_STORE || epilogue == EPI_RESID) && (!a.y || a.ldy <= 0)) return hipErrorInvalidValue;
@@ -1806,6 +1813,7 @@ hipError_t launch_gemm(const GemmArgs& a, int epilogue, int wdtype, hipStream_t 
             }
         }
     }
+    if (a.page_table != nullptr) return hipErrorInvalidValue;
     if (wdtype == 2) return launch_gemm_g<GemmBF16W>(a, epilogue, s);   // bf16 weights, fp32 activation rows
     return wdtype == 1 ? launch_gemm_g<GemmBF16>(a, epilogue, s) : launch_gemm_g<GemmF32>(a, epilogue, s);
 }

@@ -142,6 +142,10 @@ struct GemmArgs {
                                   // leaves the fold of its partial slabs to the caller (launch_*norm_rows / launch_fold_partials)
     unsigned long long* dbg = nullptr;  // diagnostic builds (-DT3K_STAMPS; scripts/micro/gemm_micro.cpp): [block][4] clock stamps; ignored otherwise
     PfArgs pf;                    // activation-stationary kernel, one row chunk, K unsplit: see PfArgs (last: the other offsets stay)
+    // EPI_ROPE_KV into a paged cache (not the 16-feature kernel: launch_gemm says so): kcache / vcache are pools [page][H][slot][64], max_len the
+    // slots of a page, and row r's position p is in slot p & slot_mask of page page_table[r * page_stride + (p >> page_shift)]
+    const int* page_table = nullptr;
+    int page_stride = 0, page_shift = 0, n_pages = 0, slot_mask = -1;
 };
 
 struct EmbedArgs {                // token-by-token prefill input (R/t3.R:494, :505)
@@ -202,6 +206,7 @@ hipError_t launch_attn_decode(const AttnArgs& a, hipStream_t s);
 hipError_t launch_prefill_embed(const EmbedArgs& a, hipStream_t s);
 hipError_t launch_sampler(const SamplerArgs& a, hipStream_t s);
 hipError_t launch_gemm(const GemmArgs& a, int epilogue, int wdtype, hipStream_t s);
+bool gemm_takes_pages(int M, int K, int wdtype);
 // 16-feature sub-tiles per block column (2 or 4; 0: not an activation-stationary shape) and K layers of the activation-stationary
 // launch of this shape with bf16 operands: what a prefetch for that launch has to know (PfArgs::unit)
 int gemm_as_plan(int M, int N, int K, int epilogue, bool splittable, int* gz_out);

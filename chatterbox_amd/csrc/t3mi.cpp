@@ -1025,7 +1025,7 @@ int run_layers_gemm(t3mi_model* m, Session* s, GemmCtx& c, StepTimer* tm) {
     // pf_attn: the attention launch has idle CUs (at most pf_max_blocks (item, head) blocks) and fetches o_proj's and gate_up's
     // matrices; otherwise, up to pf_max_rows rows, the qkv launch does.
     const bool pf_any = m->pf_blocks > 0 && as_ok && c.M <= m->pf_max_rows && ((c.M * H) & 7) == 0;
-    const bool pf_attn = pf_any && (long long)c.M * H <= m->pf_max_blocks && !(m->pf_mask & 32);
+    const bool pf_attn = pf_any && !s->paged && (long long)c.M * H <= m->pf_max_blocks && !(m->pf_mask & 32);
     const bool pf_q = pf_any && !pf_attn && (m->pf_mask & 16);
     const size_t pf_eb = 2;   // bf16 (as the instantiations that carry it)
     auto pf_region = [&](t3k::PfArgs& f, int slot, int bit, const void* w_frag, int N, int K, int epi, bool splittable, bool remap) {
@@ -1047,6 +1047,8 @@ int run_layers_gemm(t3mi_model* m, Session* s, GemmCtx& c, StepTimer* tm) {
         f.n_blocks = blocks;
         f.sink = m->pf_sink.as<unsigned>();
     };
+    // paged cache: the qkv epilogue writes into the pages where its kernel knows them, otherwise projections and append are two launches
+    const bool fused_qkv = !s->paged || t3k::gemm_takes_pages(c.M, d, wdt);
     bool ln1_done = false;
     for (int l = 0; l < m->n_layers; ++l) {
         const LayerW& lw = m->layers[l];
@@ -1077,9 +1079,26 @@ int run_layers_gemm(t3mi_model* m, Session* s, GemmCtx& c, StepTimer* tm) {
                                               split_ln2 ? c.row_mu : nullptr));
         else if (!ln1_done) HIPCHK(t3k::launch_rmsnorm_rows(c.x, lw.ln1, m->eps, c.xn, c.M, d, abf, st, gp, c.pend_ks, c.pend_bias));
         c.pend_ks = 0;
-        if (s->paged) {
-            // projections, append (rotation on the way) and attention as launches of their own: the slab path's fused epilogue writes
-            // to rows of contiguous positions
+        if (fused_qkv) {
+            t3k::GemmArgs a;
+            a.W = lw.wqkv; a.Wf = as_ok ? m->frag(lw.wqkv, 1, c.M) : nullptr; a.A = c.xn; a.M = c.M; a.N = 3 * d; a.K = d;
+            a.posmap = c.posmap; a.rowmap = c.rowmap;
+            a.rope_cos = m->rope_cos.as<float>(); a.rope_sin = m->rope_sin.as<float>();
+            a.q = c.q; a.kcache = kc; a.vcache = vc; a.kv_bf16 = s->kv_bf16 ? 1 : 0; a.n_heads = H; a.max_len = s->max_len;
+            if (s->paged) {
+                const t3k::PagedCache p = paged_layer(m, s, l);
+                a.kcache = p.k; a.vcache = p.v; a.max_len = s->page_size;
+                a.page_table = p.table; a.page_stride = s->table_w; a.page_shift = p.page_shift; a.n_pages = p.n_pages; a.slot_mask = s->page_size - 1;
+            }
+            if (turbo) { a.bias = lw.b_qkv; a.rope = 0; }
+            if (ln1_done) { a.row_ss = c.row_ss; a.row_ss_tiles = d / 32; a.norm_eps = m->eps; }
+            if (pf_q && a.Wf) {
+                pf_region(a.pf, 0, 1, wo_f, d, d, t3k::EPI_RESID, true, split_ln2);
+                pf_region(a.pf, 1, 2, gu_f, turbo ? F : 2 * F, d, turbo ? t3k::EPI_GELU : t3k::EPI_SWIGLU, false, false);
+                pf_arm(a.pf, m->pf_gblocks);
+            }
+            HIPCHK(t3k::launch_gemm(a, t3k::EPI_ROPE_KV, wdt, st));
+        } else {
             t3k::GemmArgs a;
             a.W = lw.wqkv; a.A = c.xn; a.M = c.M; a.N = 3 * d; a.K = d; a.y = c.qkv; a.ldy = 3 * d;
             if (turbo) a.bias = lw.b_qkv;
@@ -1092,40 +1111,24 @@ int run_layers_gemm(t3mi_model* m, Session* s, GemmCtx& c, StepTimer* tm) {
             if (!turbo) { p.cos = m->rope_cos.as<float>(); p.sin = m->rope_sin.as<float>(); p.rope_stride = 64; p.rope_len = m->rope_len; }
             p.positions = c.posmap; p.seq = c.rowmap; p.rows = c.M; p.q_heads = H; p.in_bf16 = 0;
             HIPCHK(t3k::launch_paged_append(p, st));
-            if (tm) tm->mark(K_QKV);
+        }
+        if (tm) tm->mark(K_QKV);
+        if (s->paged) {
             t3k::PagedAttnArgs t = paged_attn(m, s, l, c.M, abf);
             t.q = c.q; t.out = c.attn_out; t.lengths = c.posmap; t.seq = c.rowmap; t.ws = static_cast<float*>(c.ws);
             HIPCHK(t3k::launch_paged_attention(t, st));
         } else {
-            {
-                t3k::GemmArgs a;
-                a.W = lw.wqkv; a.Wf = as_ok ? m->frag(lw.wqkv, 1, c.M) : nullptr; a.A = c.xn; a.M = c.M; a.N = 3 * d; a.K = d;
-                a.posmap = c.posmap; a.rowmap = c.rowmap;
-                a.rope_cos = m->rope_cos.as<float>(); a.rope_sin = m->rope_sin.as<float>();
-                a.q = c.q; a.kcache = kc; a.vcache = vc; a.kv_bf16 = s->kv_bf16 ? 1 : 0; a.n_heads = H; a.max_len = s->max_len;
-                if (turbo) { a.bias = lw.b_qkv; a.rope = 0; }
-                if (ln1_done) { a.row_ss = c.row_ss; a.row_ss_tiles = d / 32; a.norm_eps = m->eps; }
-                if (pf_q && a.Wf) {
-                    pf_region(a.pf, 0, 1, wo_f, d, d, t3k::EPI_RESID, true, split_ln2);
-                    pf_region(a.pf, 1, 2, gu_f, turbo ? F : 2 * F, d, turbo ? t3k::EPI_GELU : t3k::EPI_SWIGLU, false, false);
-                    pf_arm(a.pf, m->pf_gblocks);
-                }
-                HIPCHK(t3k::launch_gemm(a, t3k::EPI_ROPE_KV, wdt, st));
+            t3k::AttnRowsArgs a;
+            a.q = c.q; a.kcache = kc; a.vcache = vc; a.posmap = c.posmap; a.rowmap = c.rowmap;
+            a.out = c.attn_out; a.M = c.M; a.n_heads = H; a.max_len = s->max_len;
+            a.kv_bf16 = s->kv_bf16 ? 1 : 0; a.out_bf16 = abf;
+            if (split_ln2 && turbo) { a.dot_vec = lw.o_colmean; a.dot_out = c.row_mu + t3k::kAsMaxRows; }
+            if (pf_attn) {   // the idle CUs fetch o_proj's and gate_up's weights
+                pf_region(a.pf, 0, 1, wo_f, d, d, t3k::EPI_RESID, true, split_ln2);
+                pf_region(a.pf, 1, 2, gu_f, turbo ? F : 2 * F, d, turbo ? t3k::EPI_GELU : t3k::EPI_SWIGLU, false, false);
+                pf_arm(a.pf, m->pf_blocks);
             }
-            if (tm) tm->mark(K_QKV);
-            {
-                t3k::AttnRowsArgs a;
-                a.q = c.q; a.kcache = kc; a.vcache = vc; a.posmap = c.posmap; a.rowmap = c.rowmap;
-                a.out = c.attn_out; a.M = c.M; a.n_heads = H; a.max_len = s->max_len;
-                a.kv_bf16 = s->kv_bf16 ? 1 : 0; a.out_bf16 = abf;
-                if (split_ln2 && turbo) { a.dot_vec = lw.o_colmean; a.dot_out = c.row_mu + t3k::kAsMaxRows; }
-                if (pf_attn) {   // the idle CUs fetch o_proj's and gate_up's weights
-                    pf_region(a.pf, 0, 1, wo_f, d, d, t3k::EPI_RESID, true, split_ln2);
-                    pf_region(a.pf, 1, 2, gu_f, turbo ? F : 2 * F, d, turbo ? t3k::EPI_GELU : t3k::EPI_SWIGLU, false, false);
-                    pf_arm(a.pf, m->pf_blocks);
-                }
-                HIPCHK(t3k::launch_attn_rows(a, st));
-            }
+            HIPCHK(t3k::launch_attn_rows(a, st));
         }
         if (tm) tm->mark(K_ATTN);
         {
@@ -1172,7 +1175,7 @@ int run_layers_gemm(t3mi_model* m, Session* s, GemmCtx& c, StepTimer* tm) {
             // of K in LDS) writes x, w_ln1 * x in the activation type and per-tile sums of squares; the next qkv scales its rows before
             // RoPE.  Removes the norm launch and down_proj's partial slabs -- and measured SLOWER (64 utterances 1.758 -> 1.770 ms per step,
             // 16 utterances 1.007 -> 1.074: down_proj 6.7 -> 10.1 us, qkv 6.5 -> 7.5, against 4.9 for the norm launch), so it is off by default.
-            ln1_done = (m->norm_split & 2) && !s->paged && !turbo && abf && c.row_ss != nullptr && l + 1 < m->n_layers && F == 4096 && d % 32 == 0 &&
+            ln1_done = (m->norm_split & 2) && fused_qkv && !turbo && abf && c.row_ss != nullptr && l + 1 < m->n_layers && F == 4096 && d % 32 == 0 &&
                        d / 32 <= 32 && c.M >= m->ln1_lo && c.M <= m->ln1_hi && c.M <= 128 && a.Wf != nullptr &&
                        m->frag(m->layers[l + 1].wqkv, 1, c.M) != nullptr;
             if (ln1_done) { a.part = nullptr; a.part_floats = 0; a.next_act = c.xn; a.next_norm_w = m->layers[l + 1].ln1; a.next_ss = c.row_ss; }
