@@ -188,6 +188,28 @@ def test_attention_passes_on_nan(q_t, kv_t, most):
     assert torch.equal(got[rest], cb.paged_attention(clean, k, v, table, lengths, max_length=most)[rest])
 
 
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,q_t,kv_t,longest", [
+    (220, 15, 5, 64, "f32", "bf16", 1500),     # blocks of four heads, rows in four parts
+    (2, 40, 1, 128, "bf16", "bf16", 9000),     # three blocks to a key head, many parts
+    (70, 4, 1, 64, "f32", "f32", 900),         # eight parts of four waves
+    (300, 8, 4, 128, "f32", "f32", 700),       # two parts of four waves
+    (40, 8, 8, 64, "f32", "bf16", 20000),      # much work: parts of eight waves
+    (128, 2, 1, 128, "bf16", "bf16", 500),     # one block of two waves
+    (12, 12, 2, 128, "f32", "bf16", 2500)])    # parts of two waves
+def test_attention_plans(rows, heads, kv_heads, dim, q_t, kv_t, longest):
+    """Each way to share a call's keys among blocks and waves, with rows of every length below the longest, none and padding among them."""
+    rng = np.random.default_rng(longest)
+    lens = [int(n) for n in rng.integers(0, min(longest, 200), rows)]
+    lens[0], lens[1 % rows], lens[-1] = (0, -3, longest) if rows > 2 else (longest, longest - 1, longest)
+    k, v, table, keys, vals = make_cache(lens, 32, kv_heads, dim, kv_t, 51)
+    q = torch.randn(rows, heads, dim, generator=torch.Generator().manual_seed(6)).to(DT[q_t]).cuda()
+    out = torch.full((rows, heads, dim), 5.0, dtype=DT[q_t], device="cuda")
+    cb.paged_attention(q, k, v, table, torch.tensor(lens, dtype=torch.int32).cuda(), out=out)
+    check_rows(out, q, keys, vals, None, range(rows), lens, dim ** -0.5, q_t, q_t == "bf16")
+    if rows > 2:
+        assert bool((out[1] == 5).all()) and bool((out[0] == 0).all())
+
+
 def test_attention_prompt_rows_share_a_sequence():
     """Rows of a prompt: the same sequence at lengths 1, 2, 3, ... , in any order, through `seq`; q and out as strided views."""
     k, v, table, keys, vals = make_cache([70, 9], 16, 2, 64, "bf16", 4)
