@@ -1,14 +1,21 @@
 /* CPython side of the serving operators (chatterbox_amd/ops.py): torch tensors to the structs of include/t3mi.h.
  *
  * A decode step calls these operators on a few rows, where the GPU needs 3-10 us and taking tensors apart in Python code took 12-17: the
- * attributes are read here instead (through the tensors' public methods: nothing of torch is linked).  What a tensor has to be is
- * checked here, with ValueError; what the sizes have to be is checked by the C entry points, whose status goes to _lib.check.
+ * attributes are read here instead: by torch's DLPack exchange table where it has one (a tensor in 0.05 us), by the tensors' methods
+ * otherwise (0.4 us); nothing of torch is linked.  What a tensor has to be is checked here, with ValueError; what the sizes have to be is
+ * checked by the C entry points, whose status goes to _lib.check.
  * The entry points' addresses come from the ctypes binding (bind), so that this module and it use one library. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <stdint.h>
 
 #include "t3mi.h"
+
+#ifdef T3MI_DLPACK
+#include <ATen/dlpack.h>
+static int (*f_dltensor)(void*, DLTensor*);   /* of torch's table, or NULL */
+static PyObject* t_tensor;
+#endif
 
 static int (*f_append)(const t3mi_paged_cache*, const t3mi_append_args*, void*);
 static int (*f_workspace)(const t3mi_paged_cache*, const t3mi_attention_args*, size_t*);
@@ -39,22 +46,80 @@ static int ints_of(PyObject* tuple, int64_t* o, int dim) {
 
 static const char* word_of(int types) { return types == I32 ? "int32" : types == F32 ? "float32" : "float32 or bfloat16"; }
 
+static int need_gpu(const char* name, int device, int wanted_device) {
+    if (device < 0)
+        PyErr_Format(PyExc_ValueError, "%s is on the host: the operators run on the GPU, and all tensors of a call are on the same one", name);
+    else if (wanted_device >= 0 && device != wanted_device)
+        PyErr_Format(PyExc_ValueError, "%s is on GPU %d, not on GPU %d", name, device, wanted_device);
+    else
+        return 0;
+    return -1;
+}
+
+static int wants_no_gradient(const char* name, PyObject* t) {
+    PyObject* r = PyObject_GetAttr(t, s_requires_grad);
+    if (!r) return -1;
+    const int grad = PyObject_IsTrue(r);
+    Py_DECREF(r);
+    if (grad <= 0) return grad;
+    if (!(r = PyObject_CallNoArgs(c_grad))) return -1;
+    const int on = PyObject_IsTrue(r);
+    Py_DECREF(r);
+    if (on > 0) PyErr_Format(PyExc_ValueError, "%s requires gradients: this operator has no backward pass", name);
+    return on ? -1 : 0;
+}
+
+#ifdef T3MI_DLPACK
+/* `take` by the exchange table: 1 if it could say nothing about this object (the methods then do) */
+static int take_dl(const char* name, PyObject* t, int types, int dim, int device, Ten* o) {
+    DLTensor d;
+    if (!f_dltensor || !PyObject_TypeCheck(t, (PyTypeObject*)t_tensor)) return 1;
+    if (f_dltensor(t, &d)) {
+        PyErr_Clear();
+        return 1;
+    }
+    o->device = d.device.device_type == kDLROCM || d.device.device_type == kDLCUDA ? d.device.device_id : -1;
+    if (need_gpu(name, o->device, device)) return -1;
+    const DLDataType y = d.dtype;
+    o->dtype = y.lanes != 1 ? 0 : y.code == kDLFloat && y.bits == 32 ? F32 : y.code == kDLBfloat && y.bits == 16 ? BF16 : y.code == kDLInt && y.bits == 32 ? I32 : 0;
+    if (!(o->dtype & types) || d.ndim != dim || !d.strides) return 1;   /* (the methods find the words) */
+    for (int i = 0; i < dim; ++i) {
+        o->shape[i] = d.shape[i];
+        o->stride[i] = d.strides[i];
+    }
+    o->dim = dim;
+    o->p = d.data ? (char*)d.data + d.byte_offset : NULL;
+    return 0;
+}
+#endif
+
+static int take_methods(const char* name, PyObject* t, int types, int dim, int device, Ten* o);
+
 /* A tensor of `dim` dimensions on GPU `device` (-1: any GPU) of one of `types`, its last dimension contiguous, no gradients asked for.
  * A dimension of one entry has no stride worth the name: 0. */
 static int take(const char* name, PyObject* t, int types, int dim, int device, Ten* o) {
+    int rc = 1;
+#ifdef T3MI_DLPACK
+    rc = take_dl(name, t, types, dim, device, o);
+#endif
+    if (rc > 0) rc = take_methods(name, t, types, dim, device, o);
+    if (rc) return -1;
+    if (o->stride[dim - 1] != 1 && o->shape[dim - 1] > 1) {
+        PyErr_Format(PyExc_ValueError, "%s: the last dimension must be contiguous", name);
+        return -1;
+    }
+    for (int i = 0; i < dim; ++i)
+        if (o->shape[i] <= 1) o->stride[i] = 0;
+    return types == I32 ? 0 : wants_no_gradient(name, t);
+}
+
+static int take_methods(const char* name, PyObject* t, int types, int dim, int device, Ten* o) {
     PyObject* r = PyObject_CallMethodNoArgs(t, s_get_device);
     if (!r) return -1;
     o->device = (int)PyLong_AsLong(r);
     Py_DECREF(r);
     if (o->device == -1 && PyErr_Occurred()) return -1;
-    if (o->device < 0) {
-        PyErr_Format(PyExc_ValueError, "%s is on the host: the operators run on the GPU, and all tensors of a call are on the same one", name);
-        return -1;
-    }
-    if (device >= 0 && o->device != device) {
-        PyErr_Format(PyExc_ValueError, "%s is on GPU %d, not on GPU %d", name, o->device, device);
-        return -1;
-    }
+    if (need_gpu(name, o->device, device)) return -1;
     if (!(r = PyObject_GetAttr(t, s_dtype))) return -1;
     o->dtype = r == t_f32 ? F32 : r == t_bf16 ? BF16 : r == t_i32 ? I32 : 0;
     if (!(o->dtype & types)) PyErr_Format(PyExc_ValueError, "%s has dtype %S: %s wanted", name, r, word_of(types));
@@ -75,27 +140,6 @@ static int take(const char* name, PyObject* t, int types, int dim, int device, T
     if (bad) {
         if (!PyErr_Occurred()) PyErr_Format(PyExc_ValueError, "%s has no strides", name);
         return -1;
-    }
-    if (o->stride[dim - 1] != 1 && o->shape[dim - 1] > 1) {
-        PyErr_Format(PyExc_ValueError, "%s: the last dimension must be contiguous", name);
-        return -1;
-    }
-    for (int i = 0; i < dim; ++i)
-        if (o->shape[i] <= 1) o->stride[i] = 0;
-    if (types != I32) {
-        if (!(r = PyObject_GetAttr(t, s_requires_grad))) return -1;
-        const int grad = PyObject_IsTrue(r);
-        Py_DECREF(r);
-        if (grad < 0) return -1;
-        if (grad) {
-            if (!(r = PyObject_CallNoArgs(c_grad))) return -1;
-            const int on = PyObject_IsTrue(r);
-            Py_DECREF(r);
-            if (on) {
-                if (on > 0) PyErr_Format(PyExc_ValueError, "%s requires gradients: this operator has no backward pass", name);
-                return -1;
-            }
-        }
     }
     if (!(r = PyObject_CallMethodNoArgs(t, s_data_ptr))) return -1;
     o->p = PyLong_AsVoidPtr(r);
@@ -435,10 +479,11 @@ fail:
     return NULL;
 }
 
-/* bind(4 addresses, float32, bfloat16, int32, uint8, empty, empty_like, raw stream of a device, is_grad_enabled, check) */
+/* bind(4 addresses, float32, bfloat16, int32, uint8, empty, empty_like, raw stream of a device, is_grad_enabled, check, torch.Tensor, its DLPack
+ * exchange capsule or None) */
 static PyObject* py_bind(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     (void)self;
-    if (wanted("bind", n, 13)) return NULL;
+    if (wanted("bind", n, 15)) return NULL;
     void* p[4];
     for (int i = 0; i < 4; ++i) {
         p[i] = PyLong_AsVoidPtr(a[i]);
@@ -453,6 +498,17 @@ static PyObject* py_bind(PyObject* self, PyObject* const* a, Py_ssize_t n) {
         Py_INCREF(a[4 + i]);
         Py_XSETREF(*keep[i], a[4 + i]);
     }
+#ifdef T3MI_DLPACK
+    f_dltensor = NULL;
+    if (PyType_Check(a[13]) && PyCapsule_IsValid(a[14], "dlpack_exchange_api")) {
+        const DLPackExchangeAPI* x = PyCapsule_GetPointer(a[14], "dlpack_exchange_api");
+        if (x->header.version.major == DLPACK_MAJOR_VERSION) {   /* (the table lives as long as torch does) */
+            Py_INCREF(a[13]);
+            Py_XSETREF(t_tensor, a[13]);
+            f_dltensor = x->dltensor_from_py_object_no_sync;
+        }
+    }
+#endif
     Py_RETURN_NONE;
 }
 

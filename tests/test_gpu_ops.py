@@ -744,3 +744,42 @@ def test_calls_and_refusals_keep_no_reference():
     after = [sys.getrefcount(o) for o in objects]
     assert all(abs(a - b) <= 5 for a, b in zip(after, before)), list(zip(before, after))   # (30 turns: a reference kept once a turn shows)
     assert torch.cuda.memory_allocated() == memory
+
+
+def test_tensors_are_read_alike_without_the_exchange_table(monkeypatch):
+    """torch versions without the DLPack exchange table: the tensors' own methods say the same of them, strides, refusals and all."""
+    from chatterbox_amd import ops
+    run, tensors = small_calls(4)
+    q, _, _, k, v, table, _, lengths, l, _, _ = tensors
+    wide = torch.randn(3, 8, 64, device="cuda")
+    calls = [lambda: cb.paged_attention(wide[:, ::2], k, v, table, lengths), lambda: cb.paged_attention(wide[:, 1::2].bfloat16(), k, v, table, lengths),
+             lambda: cb.process_logits(l[1:2, 5:], bias_ids=torch.tensor([[3, 7]], dtype=torch.int32, device="cuda"), bias_values=torch.ones(1, 2, device="cuda")),
+             lambda: cb.process_logits(l.t()[:5].t(), frequency_penalty=torch.ones(5, device="cuda"))]
+    bad = [lambda: cb.paged_attention(wide.transpose(1, 2), k, v, table, lengths), lambda: cb.paged_attention(q.double(), k, v, table, lengths),
+           lambda: cb.paged_attention(q, k, v, table.cpu(), lengths), lambda: cb.paged_attention(q[0], k, v, table, lengths),
+           lambda: cb.paged_attention(q.clone().requires_grad_(), k, v, table, lengths), lambda: cb.process_logits(l, tokens=l.long(), n_tokens=lengths)]
+
+    def all_of_them():
+        out, words = list(run()), []
+        for c in calls:
+            try:
+                out.append(c())
+            except ValueError as e:
+                words.append(str(e))
+        for c in bad:
+            with pytest.raises(ValueError) as e:
+                c()
+            words.append(str(e.value))
+        return out, words
+
+    with_table = all_of_them()
+    try:
+        with monkeypatch.context() as m:
+            m.delattr(torch.Tensor, "__dlpack_c_exchange_api__", raising=False)
+            ops._bind()
+            without = all_of_them()
+    finally:
+        ops._bind()
+    assert with_table[1] == without[1] and len(with_table[0]) == len(without[0])
+    for a, b in zip(with_table[0], without[0]):
+        assert a.dtype == b.dtype and torch.equal(a, b)
