@@ -98,7 +98,7 @@ template <int TH, bool HOLD> struct IdList {
 };
 
 // Chunks [c0, c1) of CH entries of one row, one after the other, TH threads.  Bound: the logits are read and written once (256 rows of 131072
-// fp32 entries in 62 us: 4.4 TB/s); everything else is kept off that stream.  The entries go to LDS as they arrive, the next
+// fp32 entries in 60 us: 4.6 TB/s); everything else is kept off that stream.  The entries go to LDS as they arrive, the next
 // chunk's already asked for.  How often each entry occurs among the row's tokens and which bias names it is noted in LDS (integer atomics: the
 // result does not depend on their order; of two biases with one id the later counts).  Few entries have a note: a second walk over the
 // tokens and biases lets the first thread that comes to one take the note (which leaves it clear for the next chunk) and change the
@@ -153,7 +153,7 @@ __device__ __forceinline__ void process_chunks(const LogitsArgs& a, const Logits
     const bool notes = n_tok > 0 || a.n_bias > 0;   // (block-uniform)
     int bid = -1;                                    // the first TH biases are held, a longer list is read again for every chunk
     float bval = 0.f;
-    IdList<TH, !MANY> tok;
+    IdList<TH, true> tok;
     float rep = 1.f, fre = 0.f, pre = 0.f;
     if (notes) {
         tok.take(a.tokens + row * a.tr, n_tok);
@@ -167,8 +167,8 @@ __device__ __forceinline__ void process_chunks(const LogitsArgs& a, const Logits
 #pragma unroll
         for (int i = 0; i < CH / (TH * 4); ++i) *reinterpret_cast<uint4*>(&note[(i * TH + tid) * 4]) = uint4{0u, 0u, 0u, 0u};
     }
-    // a block of several chunks sorts the tokens by chunk first: each chunk then walks its own few, not the whole list (as in
-    // launch_logits: 83 -> 62 us)
+    // a block of several chunks sorts the tokens by chunk first: each chunk then walks its own few, not the whole list (the call in
+    // launch_logits: 78 us without it, 49 with)
     const bool sorted = MANY && n_tok > 0 && n_tok <= kListed;
     if (sorted) {
         if (tid < kMaxRun) fill[tid] = 0;
@@ -178,14 +178,17 @@ __device__ __forceinline__ void process_chunks(const LogitsArgs& a, const Logits
             if (v / CH < (unsigned)(c1 - c0) && t < a.vocab) atomicAdd(&fill[v / CH], 1);
         });
         lds_barrier();
-        if (tid == 0) {
-            int at = 0;
-            for (int k = 0; k < c1 - c0; ++k) {
-                from[k] = at;
-                at += fill[k];
-                fill[k] = from[k];
+        if (tid < 64) {                              // kMaxRun = 64: a lane each; where each chunk's tokens begin
+            const int count = fill[tid];
+            int at = count;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int left = __shfl_up(at, d, 64);
+                if (tid >= d) at += left;
             }
-            from[c1 - c0] = at;
+            if (tid == 0) from[0] = 0;
+            from[tid + 1] = at;
+            fill[tid] = at - count;
         }
         lds_barrier();
         tok.each([&](int t) {
@@ -209,7 +212,7 @@ __device__ __forceinline__ void process_chunks(const LogitsArgs& a, const Logits
         }
         if (MANY) ask(min(c + 1, c1 - 1));           // (the last chunk once more, not used: no branch around the loads, or the loop would wait for them)
         if (notes) {
-            lds_barrier();                       // the notes are clear
+            if (c == c0) lds_barrier();          // the notes are clear, the tokens sorted (later chunks: since the last barrier)
             if (a.n_bias > 0) {
                 const auto mark = [&](int j, int id) {
                     const unsigned v = (unsigned)id - (unsigned)v0;
@@ -309,7 +312,7 @@ template <typename T> void launch_logits(const LogitsArgs& a, hipStream_t s) {
     constexpr int CH = 4096, TH = 512;
     // Blocks of a row: two blocks fit a CU at a time (LDS), 512 the chip; the time goes as the rounds they make times the chunks of one,
     // and a block starts for about three chunks' time (it sorts the row's tokens).  256 rows of 131072 fp32 entries with 2000 tokens and
-    // 300 biases each, 1 / 2 / 3 / 4 blocks a row: 104 / 62 / 74 / 73 us; a block for every chunk, unsorted: 84 us.
+    // 300 biases each, in a loop over four inputs, 1 / 2 / 3 / 4 blocks a row: 75 / 49 / 63 / 62 us; a block for every chunk, unsorted: 78 us.
     const int whole = a.vocab / CH;
     int run = 1;
     if ((long long)whole * a.rows > 512) {
