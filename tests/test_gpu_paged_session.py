@@ -117,6 +117,41 @@ def test_full_size_bf16_many_rows():
         assert paged < 1.1 * slab and paged < np.sqrt(120) * 2.0 ** -8, (i, slab, paged)
 
 
+@pytest.mark.parametrize("turbo_model", [False, True])
+@pytest.mark.parametrize("dtype,U,page", [("f32", 3, 32), ("f32", 40, 4), ("f32", 72, 64), ("bf16", 2, 4), ("bf16", 10, 128), ("bf16", 70, 16), ("bf16", 290, 8)])
+def test_every_product_writes_into_the_pages(dtype, U, page, turbo_model):
+    """Row counts that take each kernel of the qkv product (fp32 below 64 rows: product and append apart), Llama and Turbo, ragged, teacher-forced, from
+    pages and from slabs.  fp32: the slab path's bar.  bf16: the distance from the fp32 model, over U x vocabulary logits, at most a tenth above the
+    slab path's (the two round at the same places; only the attention's sums differ) and below what the 8 roundings of two layers come to.  Up to 4 rows
+    the slab session computes in fp32 on bf16 weights and rounds at none of those places, so there the second bar alone says something."""
+    dims = synth.TURBO_TINY if turbo_model else synth.TINY
+    rows = 1 if turbo_model else 2
+    path = synth.ensure_turbo_checkpoint(dims, 4321) if turbo_model else synth.ensure_checkpoint(dims, 1234)
+    load = cb.load_t3_turbo if turbo_model else cb.load_t3
+    embs = [_emb(dims, 4 + (u * 5) % 13, 900 + u, rows) for u in range(U)]
+    forced = np.random.default_rng(U).integers(0, 600, (U, 24)).astype(np.int32)
+    kw = dict(max_new_tokens=24, mask_stop=True, forced=forced, **(dict(top_k=50, top_p=0.9) if turbo_model else dict(top_p=0.0)))
+    got = {}
+    for dt in {"f32", dtype}:
+        m = load(path, device=0, dtype=dt, start_speech_token=dims.start_speech_token, stop_speech_token=dims.stop_speech_token)
+        try:
+            for p in (0, page):
+                m.set_paged_kv(p)
+                with cb.Session(m, embs, **kw) as s:
+                    first = s.logits()
+                    s.decode(20)
+                    got[dt, p] = first, s.logits()
+        finally:
+            m.close()
+    for i in range(2):
+        ref = got["f32", 0][i].astype(np.float64)
+        if dtype == "f32":
+            assert rel_err(got["f32", page][i], ref) < LOGIT_TOL, i
+        else:
+            slab, paged = (float(np.sqrt(np.mean((got["bf16", p][i] - ref) ** 2) / np.mean(ref ** 2))) for p in (0, page))
+            assert (paged < 1.1 * slab or U * rows <= 4) and paged < np.sqrt(8) * 2.0 ** -8, (i, slab, paged)
+
+
 def test_pool_is_shared_and_refill_takes_freed_pages(tiny):
     """A pool for less than the worst case: refill refuses what does not fit and leaves the session as it was; an ended utterance's pages serve
     the next; tokens are those of slabs."""
