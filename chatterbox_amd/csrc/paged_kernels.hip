@@ -651,7 +651,7 @@ void launch_attention_d(const PagedAttnArgs& a, unsigned blocks, unsigned thread
     else if (a.q_bf16) launch_attention_p<true, true, D, 32, 3>(a, blocks, threads, lds, s);
     else if (a.out_bf16) launch_attention_p<false, true, D, 32, 1>(a, blocks, threads, lds, s);
     else launch_attention_p<false, true, D, 32, 3>(a, blocks, threads, lds, s);
-    // (3072 pairs of 3 partial results: 8.3 us with a block to each, 5.1 with a wave)
+    // (96 rows of 32 heads, 3 partial results each: 8.3 us with a block to each, 5.1 with a wave)
     if (a.n_split > 8) hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)(a.rows * a.q_heads)), dim3(256), 0, s, a);
     else if (a.n_split > 1) hipLaunchKernelGGL((paged_join_few_kernel<D>), dim3((unsigned)(a.rows * a.q_heads + 3) / 4), dim3(256), 0, s, a);
 }

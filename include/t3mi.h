@@ -198,8 +198,8 @@ int t3mi_session_begin_tokens(t3mi_model* m, int n_utt, const t3mi_cond* conds, 
  * or another is refilled, instead of a slab as long as the longest utterance may get: with n_pages below the worst case, a batch of
  * ragged utterances runs in the memory it needs.  t3mi_session_begin refuses (T3MI_ERR_ARG) what does not fit the pool, t3mi_session_refill
  * likewise (T3MI_ERR_STATE, the session is as it was); t3mi_generate_continuous opens as many slots as the pool serves and starts a
- * waiting utterance when enough pages are free.  Arithmetic is the batched path's (whatever the number of rows); keys and values go through
- * t3mi_paged_append and are read by t3mi_paged_attention. */
+ * waiting utterance when enough pages are free.  Arithmetic is the batched path's (whatever the number of rows); keys and values are written
+ * by the qkv product itself (fp32 weights below 64 rows: by t3mi_paged_append's kernel) and read by t3mi_paged_attention's. */
 int t3mi_set_paged_kv(t3mi_model* m, int page_size, int n_pages);
 /* pages of the running session's pool, and how many no utterance holds (0, 0 without pages) */
 int t3mi_session_pages(t3mi_model* m, int32_t* total, int32_t* free_pages);
