@@ -529,21 +529,24 @@ __global__ __launch_bounds__(256) void paged_join_few_kernel(PagedAttnArgs a) {
     if (pair >= a.rows * a.q_heads) return;
     const int row = pair / a.q_heads, h = pair - row * a.q_heads;
     const int len = a.lengths[row], seq = a.seq ? a.seq[row] : row, first = a.starts ? a.starts[row] : 0;
-    if (len < 0) return;
-    const RowPlan rp = plan_row(a, len, first, seq);
-    if (rp.active <= 1) return;
     const long long part = (long long)pair * a.n_split;
     const float2* ml = reinterpret_cast<const float2*>(a.ws + (long long)a.rows * a.q_heads * a.n_split * D) + part;
     const int sub = lane / LP, d4 = (lane % LP) * 4;
+    // everything is asked for at once, the row's plan and the partial results; those that no block has written hold anything and are dropped
     float2 x[8];
     f32x4 v[8 / NS];
 #pragma unroll
-    for (int s = 0; s < 8; ++s) x[s] = s < rp.active ? ml[s] : float2{-INFINITY, 0.f};
+    for (int s = 0; s < 8; ++s) x[s] = ml[min(s, a.n_split - 1)];
 #pragma unroll
-    for (int k = 0; k < 8 / NS; ++k) {
-        const int s = k * NS + sub;
-        v[k] = s < rp.active ? *reinterpret_cast<const f32x4*>(a.ws + (part + s) * D + d4) : f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int k = 0; k < 8 / NS; ++k) v[k] = *reinterpret_cast<const f32x4*>(a.ws + (part + min(k * NS + sub, a.n_split - 1)) * D + d4);
+    __builtin_amdgcn_sched_barrier(0);
+    if (len < 0) return;
+    const RowPlan rp = plan_row(a, len, first, seq);
+    if (rp.active <= 1) return;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) x[s] = s < rp.active ? x[s] : float2{-INFINITY, 0.f};
+#pragma unroll
+    for (int k = 0; k < 8 / NS; ++k) v[k] = k * NS + sub < rp.active ? v[k] : f32x4{0.f, 0.f, 0.f, 0.f};
     float big = x[0].x, sum = 0.f, f[8];
 #pragma unroll
     for (int s = 1; s < 8; ++s) big = fmaxf(big, x[s].x);
