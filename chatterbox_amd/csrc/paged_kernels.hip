@@ -674,12 +674,13 @@ void plan_paged_attention(PagedAttnArgs& a) {
     const long long pairs = (long long)a.rows * a.c.kv_heads * ((group + 15) / 16);
     // 128-byte rows that lie beside those of the other heads: blocks of four heads, two waves each, so that a block reads 512 bytes in a
     // row (512 rows of 16 key heads of 64 bf16, 264 keys each: 104 us, a head a block 121; with the heads apart in memory 99).  Up to 24 tiles
-    // the row is one block (450 keys: 169 us, in two 210), longer ones, which differ more, are split (up to 1100 keys: 3 219 us, 1 222).
+    // the row is one block (450 keys: 169 us, in two 210), longer ones, which differ more, are split (128 rows of 60 to 1100 keys: 3 blocks 68 us,
+    // 1 73; up to 4000 keys: 8 211 us, 1 254), where there are not so many that they even out by themselves (2048 rows of 60 to 1100: 1 856 us, 3 873).
     if (group <= 16 && a.c.head_dim * eb == 128 && a.c.kh < a.c.ks && a.c.kv_heads >= 4 && pairs >= 1024) {
         a.head_waves = 4;
         a.waves = 8;
         a.min_tiles = 12;
-        a.n_split = tiles <= 24 ? 1 : (int)std::min((tiles + 6) / 12, 8LL);
+        a.n_split = tiles <= 24 || pairs >= 4096 ? 1 : (int)std::min((tiles + 6) / 12, 8LL);
         return;
     }
     // Otherwise a block works on one key head.  Measured over 230 shapes (1 to 600 rows, 5 to 4096 tiles), this is within 4 % of the best of 60 plans
@@ -687,7 +688,9 @@ void plan_paged_attention(PagedAttnArgs& a) {
     // tile) for as many as are useful.
     const bool wide = a.c.bf16 && a.c.head_dim == 128;
     const long long all = pairs * tiles;             // if every row is as long as the longest
-    const long long ragged = std::min(tiles / (wide ? 16 : 20), 8LL);   // rows differ more, the longer they are: so many blocks even out
+    // rows differ more, the longer they are: so many blocks even out, unless the rows do so by their number (a prompt of 4096 rows, 8 key heads of
+    // 128: 1 block a row 2377 us, 5 3761; 1024 rows of 400 to 2000 keys: 1 912, 3 943)
+    const long long ragged = pairs >= 4096 ? 1 : std::min(tiles / (wide ? 16 : 20), 8LL);
     a.head_waves = 1;
     a.n_split = 1;
     if (tiles <= (wide ? 16 : a.c.bf16 ? 40 : 32) && (wide || pairs >= 64 || tiles <= 16)) {
