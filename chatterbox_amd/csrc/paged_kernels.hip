@@ -723,6 +723,7 @@ void plan_paged_attention(PagedAttnArgs& a) {
     // (2 rows of 40 heads over one, 60001 keys: 42 blocks a row 37.4 us, 32 29.5)
     if (group > 16 && a.n_split >= 8) a.n_split &= ~7;
     if (attention_lds(a) > 65536) a.waves = 4;   // (8 waves of 16 heads of 128)
+    if (pairs > 1 << 22) a.waves = 1;            // (a launch has at most 2^32 threads)
     a.min_tiles = 2 * a.waves;
 }
 

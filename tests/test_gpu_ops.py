@@ -210,6 +210,24 @@ def test_attention_plans(rows, heads, kv_heads, dim, q_t, kv_t, longest):
         assert bool((out[1] == 5).all()) and bool((out[0] == 0).all())
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 16, 64), (16, 8, 128)])
+def test_attention_of_the_most_rows(heads, kv_heads, dim):
+    """2^24 (row, head) pairs, the most a call takes: rows of one key give its value exactly, rows of none zeros; one more row is refused."""
+    rows = 1 << 20
+    k, v, table, _, vals = make_cache([1, 1, 1], 16, kv_heads, dim, "bf16", 61)
+    q = torch.zeros(rows, heads, dim, dtype=torch.bfloat16, device="cuda")
+    seq = (torch.arange(rows, device="cuda", dtype=torch.int32) * 7) % 3
+    lengths = (torch.arange(rows, device="cuda", dtype=torch.int32) % 5 != 0).int()
+    out = cb.paged_attention(q, k, v, table, lengths, seq=seq)
+    want = torch.from_numpy(np.stack(vals)[:, 0]).to(torch.bfloat16).cuda().repeat_interleave(heads // kv_heads, 1)
+    for r0 in range(0, rows, 1 << 17):
+        part = slice(r0, r0 + (1 << 17))
+        assert torch.equal(out[part], want[seq[part].long()] * lengths[part].view(-1, 1, 1))
+    more = torch.zeros(rows + 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="pairs"):
+        cb.paged_attention(q[:1].expand(rows + 1, heads, dim), k, v, table, more, seq=more, out=torch.empty(rows + 1, heads, dim, dtype=torch.bfloat16, device="cuda"))
+
+
 def test_attention_prompt_rows_share_a_sequence():
     """Rows of a prompt: the same sequence at lengths 1, 2, 3, ... , in any order, through `seq`; q and out as strided views."""
     k, v, table, keys, vals = make_cache([70, 9], 16, 2, 64, "bf16", 4)
