@@ -93,7 +93,7 @@ class AttentionArgs(C.Structure):
     """t3mi_attention_args"""
     _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64 * 2), ("out_stride", C.c_int64 * 2), ("lengths", C.c_void_p),
                 ("starts", C.c_void_p), ("seq", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("scale", C.c_float)] + \
-               [(n, C.c_int32) for n in ("rows", "q_heads", "q_dtype", "out_dtype", "length_add", "max_length")]
+               [(n, C.c_int32) for n in ("rows", "q_heads", "q_dtype", "out_dtype", "length_add", "max_length", "prompt")]
 
 
 class LogitsArgs(C.Structure):

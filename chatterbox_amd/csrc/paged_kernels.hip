@@ -521,6 +521,306 @@ __global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
     }
 }
 
+// ---- attention of a prompt's rows -------------------------------------------------------------------------------------------------
+// The same sums where neighbouring rows belong to one sequence: the 16 columns of a tile are 16 / G rows with the G heads of one key head, so a key
+// is read once for all of them (from L2: the blocks that read it are kv_heads apart).  Bound: the matrix and vector work of a tile, a few hundred
+// cycles for 32 keys x 16 columns.  Rows of a block that belong to other sequences are taken in turn (a column that is not in turn has weight
+// zero), so any rows come out right.  A key that some of the rows see and others do not has weight zero for the others; only if such a tile holds a
+// value that is not finite (0 times it is not 0) are its rows summed one by one.
+// SMALL: pages of fewer than TK keys.
+template <bool QB, bool KB, int D, int TK, bool SMALL, int PARTS>
+__global__ __launch_bounds__(256, D == 64 && !(SMALL && KB && !QB) ? 3 : 2) void paged_prompt_kernel(PagedAttnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) float sm[];
+    constexpr int EB = KB ? 2 : 4, KC = KB ? D / 32 : D / 16, VL = KB ? 1 : D / 64, NT = D / 16, QS = QB ? 1 : 3, U = TK / 16, J = 4 * U;
+    using VT = std::conditional_t<KB && D == 64, u32x2, u32x4>;
+    constexpr int VW = (int)sizeof(VT) / 4;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
+    const int group = a.q_heads / a.c.kv_heads, R = 16 / group, cols = R * group;
+    const int hk = (int)(blockIdx.x % (unsigned)a.c.kv_heads), r0 = (int)(blockIdx.x / (unsigned)a.c.kv_heads) * R;
+    const int rn = n / group;                       // this column's row and head
+    const bool col = n < cols && r0 + rn < a.rows;
+    const int row = col ? r0 + rn : r0, h = hk * group + (col ? n - rn * group : 0);
+    const int row_len = a.lengths[row], seq = a.seq ? a.seq[row] : row, first = a.starts ? max(a.starts[row], 0) : 0;
+    bf16x8 qb[KB ? QS : 1][KB ? KC : 1];
+    f32x4 qf[KB ? 1 : KC];
+    {
+        const long long qo = row * a.qr + h * a.qh;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            if constexpr (QB) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + qo + 32 * c + 8 * g);
+                qb[0][c] = __builtin_bit_cast(bf16x8, col ? w : u32x4{0u, 0u, 0u, 0u});
+            } else if constexpr (KB) {
+                float x[8];
+                load_row<float, 4>(a.q, qo + 32 * c + 8 * g, *reinterpret_cast<float(*)[4]>(x));
+                load_row<float, 4>(a.q, qo + 32 * c + 8 * g + 4, *reinterpret_cast<float(*)[4]>(x + 4));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = col ? x[j] : 0.f;
+                bf16x8 o[3];
+                to_parts<3>(x, o);
+#pragma unroll
+                for (int s = 0; s < QS; ++s) qb[s][c] = o[s];
+            } else {
+                const f32x4 w = *reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + qo + 16 * c + 4 * g);
+                qf[c] = col ? w : f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+    }
+    int len = 0;
+    if (col && row_len >= 0 && seq >= 0 && seq < a.c.n_seqs) {
+        const long long most = (long long)a.c.max_pages << a.c.page_shift, k = (long long)row_len + a.length_add;
+        len = (int)(k > most ? most : k);
+    }
+    const bool has = len > first;
+
+    const unsigned ksb = (unsigned)a.c.ks * EB, vsb = (unsigned)a.c.vs * EB;
+    const char* kbase = static_cast<const char*>(a.c.k) + (long long)hk * a.c.kh * EB;
+    const char* vbase = static_cast<const char*>(a.c.v) + (long long)hk * a.c.vh * EB;
+    const int in_page = (1 << a.c.page_shift) - 1;
+    constexpr int NP = SMALL ? U + J : 1;           // page numbers of a tile: of each key a lane loads, or one
+    f32x4 acc[NT];
+#pragma unroll
+    for (int e = 0; e < NT; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    const float scale2 = a.scale * 1.4426950408889634f;
+    const unsigned alive = (unsigned)__builtin_amdgcn_ballot_w64(has) & 0xFFFFu;
+    unsigned pending = alive;
+    while (pending != 0u) {
+        // the columns of the first pending one's sequence, and the keys they span: [lo, hi), all of them see [lo_all, hi_all)
+        const int sq = __builtin_amdgcn_readlane(seq, __builtin_ctz(pending));
+        const unsigned in = (unsigned)__builtin_amdgcn_ballot_w64(has && seq == sq) & 0xFFFFu;
+        pending &= ~in;
+        const bool mine = (in >> n) & 1u;
+        int lo = mine ? first : 0x7FFFFFFF, lo_all = mine ? first : 0, hi = mine ? len : 0, hi_all = mine ? len : 0x7FFFFFFF;
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) {
+            lo = min(lo, __shfl_xor(lo, d, 64));
+            lo_all = max(lo_all, __shfl_xor(lo_all, d, 64));
+            hi = max(hi, __shfl_xor(hi, d, 64));
+            hi_all = min(hi_all, __shfl_xor(hi_all, d, 64));
+        }
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        lo_all = __builtin_amdgcn_readfirstlane(lo_all);
+        hi = __builtin_amdgcn_readfirstlane(hi);
+        hi_all = __builtin_amdgcn_readfirstlane(hi_all);
+        const int* trow = a.c.table + (long long)sq * a.c.table_stride;
+        const int t_end = (hi + TK - 1) / TK;
+        int t = lo / TK + wave;
+        if (t >= t_end) continue;
+        auto key_of = [&](int at, int x) {           // (clamped to the last: entries past it may hold anything)
+            int k = at * TK;
+            if (SMALL) k += x < U ? 16 * x + n : 16 * ((x - U) >> 2) + 4 * g + ((x - U) & 3);
+            return min(k, hi - 1);
+        };
+        int ids[NP];
+        auto ask = [&](int at) {
+#pragma unroll
+            for (int x = 0; x < NP; ++x) ids[x] = trow[key_of(at, x) >> a.c.page_shift];
+        };
+        struct Pages { int id[NP]; unsigned ok; };   // clamped into the pool; ok: bit j, key j of this lane's values has a page
+        auto settle = [&]() {
+            Pages p;
+            p.ok = 0u;
+#pragma unroll
+            for (int x = 0; x < NP; ++x) {
+                const bool good = ids[x] >= 0 && ids[x] < a.c.n_pages;
+                p.id[x] = good ? ids[x] : 0;
+                if (!SMALL) p.ok = good ? 0xFFu : 0u;
+                else if (x >= U) p.ok |= good ? 1u << (x - U) : 0u;
+            }
+            return p;
+        };
+        u32x4 kr[U][KC];
+        VT vr[J][VL];
+        auto load_k = [&](int at, const Pages& p) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int slot = SMALL ? key_of(at, u) & in_page : ((at * TK) & in_page) + 16 * u + n;
+                const char* base = kbase + (long long)p.id[SMALL ? u : 0] * a.c.kp * EB + (long long)slot * ksb + 16 * g;
+#pragma unroll
+                for (int c = 0; c < KC; ++c) kr[u][c] = *reinterpret_cast<const u32x4*>(base + 64 * c);
+            }
+        };
+        auto load_v = [&](int at, const Pages& p) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int slot = SMALL ? key_of(at, U + j) & in_page : ((at * TK) & in_page) + 16 * (j >> 2) + 4 * g + (j & 3);
+                const char* base = vbase + (long long)p.id[SMALL ? U + j : 0] * a.c.vp * EB + (long long)slot * vsb + sizeof(VT) * n;
+#pragma unroll
+                for (int x = 0; x < VL; ++x) vr[j][x] = *reinterpret_cast<const VT*>(base + 256 * x);
+            }
+        };
+        ask(t);
+        Pages pg = settle();
+        ask(min(t + nw, t_end - 1));
+        load_k(t, pg);
+        load_v(t, pg);
+        while (true) {
+            const int t_next = min(t + nw, t_end - 1);
+            f32x4 s[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (KB) {
+#pragma unroll
+                for (int part = QS - 1; part >= 0; --part)
+#pragma unroll
+                    for (int c = 0; c < KC; ++c)
+#pragma unroll
+                        for (int u = 0; u < U; ++u) s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[u][c]), qb[part][c], s[u], 0, 0, 0);
+            } else {
+                f32x4 part[U][4];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) part[u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int u = 0; u < U; ++u) part[u][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, kr[u][c])[i], qf[c][i], part[u][i], 0, 0, 0);
+#pragma unroll
+                for (int u = 0; u < U; ++u) s[u] = (part[u][0] + part[u][1]) + (part[u][2] + part[u][3]);
+            }
+            const Pages next = settle();
+            ask(min(t + 2 * nw, t_end - 1));
+            load_k(t_next, next);
+            float p[J];
+#pragma unroll
+            for (int j = 0; j < J; ++j) p[j] = s[j >> 2][j & 3] * scale2;
+            const bool masked = !(in == alive && t * TK >= lo_all && t * TK + TK <= hi_all && __builtin_amdgcn_ballot_w64((~pg.ok & ((1u << J) - 1)) != 0u) == 0);
+            unsigned dead = 0u;
+            bool odd = false;                        // a value that is not finite in a tile that not all rows see
+            if (masked) {
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    const int key = t * TK + 16 * (j >> 2) + 4 * g + (j & 3);
+                    const bool there = key >= lo && key < hi && ((pg.ok >> j) & 1u);
+                    if (!(there && mine && key >= first && key < len)) { p[j] = -INFINITY; dead |= 1u << j; }
+#pragma unroll
+                    for (int x = 0; x < VL; ++x)
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) {
+                            const unsigned v = there ? vr[j][x][w] : 0u;
+                            vr[j][x][w] = v;
+                            if (KB) odd = odd || (v & 0x7F80u) == 0x7F80u || (v & 0x7F800000u) == 0x7F800000u;
+                            else odd = odd || (v & 0x7F800000u) == 0x7F800000u;
+                        }
+                }
+            }
+            float mx = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+            if constexpr (U == 2) mx = fmaxf(mx, fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+            mx = fmaxf(m, group_max(mx));
+            const float ref = mx > -INFINITY ? mx : 0.f;
+            if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
+                const float keep = __builtin_amdgcn_exp2f(m - ref);
+                l *= keep;
+#pragma unroll
+                for (int e = 0; e < NT; ++e) acc[e] *= keep;
+                m = mx;
+            }
+            if (__builtin_amdgcn_ballot_w64(!(fabsf(ref) < 65536.f)) == 0) {   // (as above)
+#pragma unroll
+                for (int j = 0; j < J; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], scale2, -ref));
+            } else {
+#pragma unroll
+                for (int j = 0; j < J; ++j) p[j] = __builtin_amdgcn_exp2f(p[j] - ref);
+            }
+            if (masked) {
+#pragma unroll
+                for (int j = 0; j < J; ++j) p[j] = (dead >> j) & 1u ? 0.f : p[j];
+            }
+            if constexpr (U == 2) l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            else l += (p[0] + p[1]) + (p[2] + p[3]);
+            bf16x8 pb[KB ? PARTS : 1];
+            if constexpr (KB) to_parts<PARTS>(p, pb);
+            // o += V^T P, of the values whose bit is set in `of`
+            auto weigh = [&](auto of, int e, f32x4 o) {
+                auto v = [&](int j, int x, int w) -> unsigned {
+                    if constexpr (std::is_same_v<decltype(of), unsigned>) return (of >> j) & 1u ? vr[j][x][w] : 0u;
+                    else return vr[j][x][w];
+                };
+                if constexpr (KB) {
+                    u32x4 w;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[j] = __builtin_amdgcn_perm(v(2 * j + 1, 0, e >> 1), v(2 * j, 0, e >> 1), (e & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                    for (int part = PARTS - 1; part >= 0; --part) o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), pb[part], o, 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < J; ++j) o = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v(j, e >> 2, e & 3)), p[j], o, 0, 0, 0);
+                }
+                return o;
+            };
+            if (__builtin_amdgcn_ballot_w64(odd) == 0) {
+#pragma unroll
+                for (int e = 0; e < NT; ++e) acc[e] = weigh(true, e, acc[e]);
+            } else {
+                for (int r = 0; r < R; ++r) {
+                    const int c = r * group, f_r = __builtin_amdgcn_readlane(first, c), l_r = (in >> c) & 1u ? __builtin_amdgcn_readlane(len, c) : 0;
+                    unsigned of = 0u;                // the keys that row r sees
+#pragma unroll
+                    for (int j = 0; j < J; ++j) {
+                        const int key = t * TK + 16 * (j >> 2) + 4 * g + (j & 3);
+                        of |= key >= f_r && key < l_r ? 1u << j : 0u;
+                    }
+#pragma unroll
+                    for (int e = 0; e < NT; ++e) {
+                        const f32x4 o = weigh(of, e, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[e][i] += rn == r ? o[i] : 0.f;
+                    }
+                }
+            }
+            load_v(t_next, next);
+            t += nw;
+            if (t >= t_end) break;
+            pg = next;
+        }
+    }
+    l = group_sum(l);
+    if (!has) {
+        m = -INFINITY;
+        l = 0.f;
+    }
+    float* sm_m = sm;
+    float* sm_l = sm + nw * 16;
+    float* sm_o = sm + nw * 32;
+    if (lane < 16) {
+        sm_m[wave * 16 + n] = m;
+        sm_l[wave * 16 + n] = l;
+    }
+    __syncthreads();
+    float top = -INFINITY;
+    for (int w = 0; w < nw; ++w) top = fmaxf(top, sm_m[w * 16 + n]);
+    {
+        const float f = part_factor(m, top);
+        float* o = sm_o + (wave * 16 + n) * D;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < NT; e += 4) {
+                f32x4 v = f32x4{acc[e][i], acc[e + 1][i], acc[e + 2][i], acc[e + 3][i]} * f;
+                if (!has) v = f32x4{0.f, 0.f, 0.f, 0.f};
+                *reinterpret_cast<f32x4*>(o + (KB ? NT * (4 * g + i) + e : 64 * (e >> 2) + 4 * (4 * g + i))) = v;
+            }
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < cols * (D / 4); x += blockDim.x) {
+        const int d4 = (x % (D / 4)) * 4, c = x / (D / 4), r = r0 + c / group;
+        if (r >= a.rows || a.lengths[r] < 0) continue;
+        float big = -INFINITY, sum = 0.f;
+        for (int w = 0; w < nw; ++w) big = fmaxf(big, sm_m[w * 16 + c]);
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < nw; ++w) {
+            sum += sm_l[w * 16 + c] * part_factor(sm_m[w * 16 + c], big);
+            o += *reinterpret_cast<const f32x4*>(sm_o + (w * 16 + c) * D + d4);
+        }
+        store_out(a, r, hk * group + c % group, d4, o, sum);
+    }
+}
+
 // a row's few (at most 8) partial results joined in a fixed order, one wave per (row, query head), four to a block
 template <int D>
 __global__ __launch_bounds__(256) void paged_join_few_kernel(PagedAttnArgs a) {
@@ -648,6 +948,27 @@ void launch_attention_p(const PagedAttnArgs& a, unsigned blocks, unsigned thread
     else hipLaunchKernelGGL((paged_attention_kernel<QB, KB, D, TK, 2, PARTS>), grid, block, lds, s, a);
 }
 template <int D>
+void launch_prompt_d(const PagedAttnArgs& a, unsigned blocks, unsigned threads, size_t lds, hipStream_t s) {
+    const dim3 grid(blocks), block(threads);
+    const bool small = a.c.page_shift < a.tile_shift;
+    if (!a.c.bf16) {
+        if (small) hipLaunchKernelGGL((paged_prompt_kernel<false, false, D, 16, true, 1>), grid, block, lds, s, a);
+        else hipLaunchKernelGGL((paged_prompt_kernel<false, false, D, 16, false, 1>), grid, block, lds, s, a);
+    } else if (a.q_bf16 && a.out_bf16) {
+        if (small) hipLaunchKernelGGL((paged_prompt_kernel<true, true, D, 32, true, 1>), grid, block, lds, s, a);
+        else hipLaunchKernelGGL((paged_prompt_kernel<true, true, D, 32, false, 1>), grid, block, lds, s, a);
+    } else if (a.q_bf16) {
+        if (small) hipLaunchKernelGGL((paged_prompt_kernel<true, true, D, 32, true, 3>), grid, block, lds, s, a);
+        else hipLaunchKernelGGL((paged_prompt_kernel<true, true, D, 32, false, 3>), grid, block, lds, s, a);
+    } else if (a.out_bf16) {
+        if (small) hipLaunchKernelGGL((paged_prompt_kernel<false, true, D, 32, true, 1>), grid, block, lds, s, a);
+        else hipLaunchKernelGGL((paged_prompt_kernel<false, true, D, 32, false, 1>), grid, block, lds, s, a);
+    } else {
+        if (small) hipLaunchKernelGGL((paged_prompt_kernel<false, true, D, 32, true, 3>), grid, block, lds, s, a);
+        else hipLaunchKernelGGL((paged_prompt_kernel<false, true, D, 32, false, 3>), grid, block, lds, s, a);
+    }
+}
+template <int D>
 void launch_attention_d(const PagedAttnArgs& a, unsigned blocks, unsigned threads, size_t lds, hipStream_t s) {
     if (!a.c.bf16) launch_attention_p<false, false, D, 16, 1>(a, blocks, threads, lds, s);
     else if (a.q_bf16 && a.out_bf16) launch_attention_p<true, true, D, 32, 1>(a, blocks, threads, lds, s);
@@ -664,7 +985,12 @@ void launch_attention_d(const PagedAttnArgs& a, unsigned blocks, unsigned thread
 // shared memory of a block: maxima and sums, and the weighted sums of its waves
 static size_t attention_lds(const PagedAttnArgs& a) {
     const int group = a.q_heads / a.c.kv_heads;
-    return (size_t)a.waves * (32 + (size_t)(group < 16 ? group : 16) * a.c.head_dim) * 4;
+    return (size_t)a.waves * (32 + (size_t)(group < 16 && !a.prompt ? group : 16) * a.c.head_dim) * 4;
+}
+
+static long long prompt_blocks(const PagedAttnArgs& a) {
+    const int r = 16 / (a.q_heads / a.c.kv_heads);
+    return ((long long)a.rows + r - 1) / r * a.c.kv_heads;
 }
 
 void plan_paged_attention(PagedAttnArgs& a) {
@@ -672,6 +998,15 @@ void plan_paged_attention(PagedAttnArgs& a) {
     a.tile_shift = a.c.bf16 ? 5 : 4;
     const long long tiles = ((long long)a.max_length + (1 << a.tile_shift) - 1) >> a.tile_shift;
     const long long pairs = (long long)a.rows * a.c.kv_heads * ((group + 15) / 16);
+    a.prompt = a.prompt && group <= 8;               // (two rows at least to a tile)
+    if (a.prompt) {
+        const long long blocks = prompt_blocks(a);
+        a.head_waves = 1;
+        a.n_split = 1;
+        a.waves = blocks >= 4096 ? 1 : (blocks >= 2048 ? 2 : 4);
+        a.min_tiles = 1;
+        return;
+    }
     // 128-byte rows that lie beside those of the other heads: blocks of four heads, two waves each, so that a block reads 512 bytes in a
     // row (512 rows of 16 key heads of 64 bf16, 264 keys each: 104 us, a head a block 121; with the heads apart in memory 99).  Up to 24 tiles
     // the row is one block (450 keys: 169 us, in two 210), longer ones, which differ more, are split (128 rows of 60 to 1100 keys: 3 blocks 68 us,
@@ -739,6 +1074,13 @@ hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s) {
     if (a.n_split > 1 && a.ws == nullptr) return hipErrorInvalidValue;
     const size_t lds = attention_lds(a);
     if (lds > 65536) return hipErrorInvalidValue;
+    if (a.prompt) {
+        if (a.n_split != 1 || a.waves > 4 || group > 8) return hipErrorInvalidValue;
+        if (a.c.head_dim == 64) launch_prompt_d<64>(a, (unsigned)prompt_blocks(a), 64u * a.waves, lds, s);
+        else if (a.c.head_dim == 128) launch_prompt_d<128>(a, (unsigned)prompt_blocks(a), 64u * a.waves, lds, s);
+        else return hipErrorInvalidValue;
+        return hipGetLastError();
+    }
     if (a.c.head_dim == 64) launch_attention_d<64>(a, (unsigned)blocks, 64u * a.waves, lds, s);
     else if (a.c.head_dim == 128) launch_attention_d<128>(a, (unsigned)blocks, 64u * a.waves, lds, s);
     else return hipErrorInvalidValue;

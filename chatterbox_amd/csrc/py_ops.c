@@ -307,13 +307,13 @@ fail:
     return NULL;
 }
 
-/* attention(q, k_pages, v_pages, block_table, lengths, seq, starts, scale or None, max_length, out, out_dtype) -> out */
+/* attention(q, k_pages, v_pages, block_table, lengths, seq, starts, scale or None, max_length, out, out_dtype, prompt: 1, 0 or -1) -> out */
 static PyObject* py_attention(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     (void)self;
     t3mi_paged_cache c;
     t3mi_attention_args g = {0};
     Ten kc, q, o;
-    if (wanted("attention", n, 11) || take_cache(a[1], a[2], a[3], &c, &kc) || take("q", a[0], F32 | BF16, 3, kc.device, &q)) return NULL;
+    if (wanted("attention", n, 12) || take_cache(a[1], a[2], a[3], &c, &kc) || take("q", a[0], F32 | BF16, 3, kc.device, &q)) return NULL;
     const int64_t rows = q.shape[0];
     if (rows > INT32_MAX || q.shape[1] > INT32_MAX || q.shape[2] != c.head_dim) {
         PyErr_Format(PyExc_ValueError, "q has head_dim %lld, the cache %d", (long long)q.shape[2], c.head_dim);
@@ -334,6 +334,8 @@ static PyObject* py_attention(PyObject* self, PyObject* const* a, Py_ssize_t n) 
     const long most = PyLong_AsLong(a[8]);
     if (most == -1 && PyErr_Occurred()) return NULL;
     g.max_length = most > INT32_MAX ? INT32_MAX : most < 0 ? -1 : (int32_t)most;
+    g.prompt = (int32_t)PyLong_AsLong(a[11]);
+    if (PyErr_Occurred()) return NULL;
     PyObject *out = NULL, *ws = NULL;
     if (a[9] == Py_None) {
         if (a[10] != Py_None && a[10] != t_f32 && a[10] != t_bf16) {

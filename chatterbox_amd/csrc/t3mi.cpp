@@ -976,6 +976,7 @@ struct GemmCtx {
     const float* pend_bias = nullptr;
     float* qkv = nullptr;      // paged cache: [M][3 d] projections before the append
     void* ws = nullptr;        // and the attention's workspace
+    bool prompt = false;       // the rows are positions of prompts, one after the other
     // bf16 weight storage with fp32 activation rows (exact fp32 products, the arithmetic of the GEMV path): the prefill
     // of sessions that decode with <= 4 rows
     bool act_f32 = false;
@@ -999,14 +1000,14 @@ t3k::PagedCache paged_layer(const t3mi_model* m, const Session* s, int layer) {
     return c;
 }
 // attention of M items (query rows c.q, positions c.posmap) over a layer's pool, as launched and as planned for the workspace
-t3k::PagedAttnArgs paged_attn(const t3mi_model* m, const Session* s, int layer, int M, int out_bf16) {
+t3k::PagedAttnArgs paged_attn(const t3mi_model* m, const Session* s, int layer, int M, int out_bf16, bool prompt) {
     t3k::PagedAttnArgs a;
     a.c = paged_layer(m, s, layer);
     a.qr = a.outr = m->d;
     a.qh = a.outh = 64;
     a.scale = 0.125f;
     a.rows = M; a.q_heads = m->H; a.q_bf16 = 0; a.out_bf16 = out_bf16;
-    a.max_length = s->max_len; a.length_add = 1;
+    a.max_length = s->max_len; a.length_add = 1; a.prompt = prompt ? 1 : 0;
     t3k::plan_paged_attention(a);
     return a;
 }
@@ -1114,7 +1115,7 @@ int run_layers_gemm(t3mi_model* m, Session* s, GemmCtx& c, StepTimer* tm) {
         }
         if (tm) tm->mark(K_QKV);
         if (s->paged) {
-            t3k::PagedAttnArgs t = paged_attn(m, s, l, c.M, abf);
+            t3k::PagedAttnArgs t = paged_attn(m, s, l, c.M, abf, c.prompt);
             t.q = c.q; t.out = c.attn_out; t.lengths = c.posmap; t.seq = c.rowmap; t.ws = static_cast<float*>(c.ws);
             HIPCHK(t3k::launch_paged_attention(t, st));
         } else {
@@ -1382,7 +1383,8 @@ int prefill_rows(t3mi_model* m, Session* s, const std::vector<int>& rows_list, c
         c.posmap = dpos.as<int>(); c.rowmap = drow.as<int>();
         c.act_f32 = pf_act_f32;
         if (s->paged) {
-            HIPCHK(grow(s->pfs[10], t3k::paged_attention_workspace(paged_attn(m, s, 0, c.M, as == 2 ? 1 : 0))));
+            c.prompt = true;
+            HIPCHK(grow(s->pfs[10], t3k::paged_attention_workspace(paged_attn(m, s, 0, c.M, as == 2 ? 1 : 0, c.prompt))));
             c.qkv = s->pfs[9].as<float>();
             c.ws = s->pfs[10].p;
         }
@@ -1763,7 +1765,7 @@ int t3mi_session_begin(t3mi_model* m, int n_utt, int rpu, const float* const* em
         HIPCHK(s->table.alloc(most * 4));
         HIPCHK(hipMemcpy(s->table.p, s->table_h.data(), most * 4, hipMemcpyHostToDevice));
         HIPCHK(s->qkv.alloc(rows * 3 * d * 4));
-        HIPCHK(s->pws.alloc(t3k::paged_attention_workspace(paged_attn(m, s.get(), 0, (int)rows, m->wdtype == T3MI_W_BF16 ? 1 : 0))));
+        HIPCHK(s->pws.alloc(t3k::paged_attention_workspace(paged_attn(m, s.get(), 0, (int)rows, m->wdtype == T3MI_W_BF16 ? 1 : 0, false))));
     }
     HIPCHK(s->kc.alloc(kv));
     HIPCHK(s->vc.alloc(kv));

@@ -53,7 +53,7 @@ def paged_kv_append(k, v, k_pages, v_pages, block_table, positions, *, seq=None,
 
 
 def paged_attention(q, k_pages, v_pages, block_table, lengths, *, seq=None, starts=None, scale: Optional[float] = None,
-                    max_length: Optional[int] = None, out=None, out_dtype=None):
+                    max_length: Optional[int] = None, out=None, out_dtype=None, prompt: Optional[bool] = None):
     """Attention of one new token per row over a paged cache: out[r, h] = sum_j softmax_j(scale q[r, h] . k_j) v_j over the keys
     j in [starts[r], lengths[r]) of sequence seq[r] (None: sequence r; starts None: 0).
 
@@ -62,8 +62,10 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, *, seq=None, star
     scale: 1 / sqrt(head_dim) by default.  max_length: about the longest length, where the host knows it (the call is planned by it;
     rows that are longer come out right too).  A row with no key gives zeros; a row of negative length is left as it was in out.
     out: [rows, heads, head_dim], float32 or bfloat16 (new, in out_dtype or q's type, by default).  Many rows of one sequence
-    (a prompt, causal) are rows with the same seq and lengths 1, 2, 3, ..."""
-    return (_ops or _bind()).attention(q, k_pages, v_pages, block_table, lengths, seq, starts, scale, max_length or 0, out, out_dtype)
+    (a prompt, causal) are rows with the same seq and lengths 1, 2, 3, ...; prompt says that neighbouring rows mostly share a sequence, and
+    then they share the keys they read (None: if there are four rows to a sequence of the table; the results are the same up to rounding)."""
+    return (_ops or _bind()).attention(q, k_pages, v_pages, block_table, lengths, seq, starts, scale, max_length or 0, out, out_dtype,
+                                       0 if prompt is None else 1 if prompt else -1)
 
 
 def process_logits(logits, *, uncond=None, cfg_weight: float = 0.0, tokens=None, n_tokens=None, repetition_penalty=1.0,

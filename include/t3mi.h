@@ -430,7 +430,7 @@ int t3mi_paged_append(const t3mi_paged_cache* cache, const t3mi_append_args* arg
 
 /* Attention of one new token per row: out[r, h] = sum_j softmax_j(scale * q[r, h] . k_j) v_j over the keys j in [starts[r],
  * lengths[r] + length_add) of sequence seq[r], head h reading key head h / (q_heads / kv_heads).  Row r of a prompt's queries attends
- * causally when lengths[r] is its position and length_add 1.  A row with no key is written as zeros, a row whose length is negative is left as it
+ * causally when lengths[r] is its position and length_add 1 (such rows share the keys they read, `prompt`).  A row with no key is written as zeros, a row whose length is negative is left as it
  * was (padding of a batch); lengths beyond the block table end there.  Types: q fp32 over an fp32 or bf16 cache, q bf16 over a bf16
  * cache; out fp32 or bf16, and q itself only with q's type and strides. */
 typedef struct t3mi_attention_args {
@@ -447,6 +447,7 @@ typedef struct t3mi_attention_args {
     int32_t q_dtype, out_dtype;
     int32_t length_add;          /* 0 or 1                                                   */
     int32_t max_length;          /* about the longest length, for planning alone (0: the table's); longer rows are still right */
+    int32_t prompt;              /* for planning alone: 1 if neighbouring rows mostly belong to one sequence (prompts), -1 if not, 0: if there are 4 rows to a sequence */
 } t3mi_attention_args;
 int t3mi_paged_attention_workspace(const t3mi_paged_cache* cache, const t3mi_attention_args* args, size_t* bytes);
 int t3mi_paged_attention(const t3mi_paged_cache* cache, const t3mi_attention_args* args, void* stream);

@@ -292,6 +292,82 @@ def test_attention_extreme_values():
     assert torch.allclose(got[:, 0, 0], want, rtol=8 * U, atol=0), got[:, 0, 0]
 
 
+def prompt_rows(lens, shuffled, seed):
+    """Rows (sequence, length, start) of prompts over sequences of `lens` keys: all positions of the first, the last 40 of each other, causal; padding,
+    rows of no sequence and rows past the end among them; in order or shuffled."""
+    rng = np.random.default_rng(seed)
+    rows = [(0, n, 0) for n in range(1, lens[0] + 1)]
+    for s in range(1, len(lens)):
+        rows += [(s, n, int(rng.integers(0, 30)) if s % 2 else 0) for n in range(max(0, lens[s] - 40), lens[s] + 1)]
+    rows[5] = (0, -1, 0)
+    rows.insert(20, (-4, 9, 0))
+    rows.insert(37, (len(lens) + 3, 50, 0))
+    rows.insert(50, (0, 12, 12))
+    if shuffled:
+        rng.shuffle(rows)
+    return [tuple(int(x) for x in r) for r in rows]
+
+
+@pytest.mark.parametrize("q_t,kv_t,out_t", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,page,order,shuffled", [(16, 16, 64, 16, "slots", False), (8, 2, 128, 64, "heads", False), (15, 5, 64, 1, "pairs", False),
+                                                                    (7, 1, 128, 8, "slots", False), (12, 2, 128, 32, "slots", True), (5, 1, 64, 128, "heads", True),
+                                                                    (2, 2, 64, 4, "pairs", True), (16, 2, 64, 2, "slots", False), (48, 4, 64, 32, "slots", False)])
+def test_attention_of_prompts(q_t, kv_t, out_t, heads, kv_heads, dim, page, order, shuffled):
+    """Rows that share the keys they read, with whatever else the call allows among them, against 64 bits; padding rows stay as they were."""
+    lens = [75, 131, 0, 40, 300]
+    k, v, table, keys, vals = make_cache(lens, page, kv_heads, dim, kv_t, 71, order)
+    rows = prompt_rows(lens, shuffled, heads)
+    seq, n, start = (torch.tensor([r[i] for r in rows], dtype=torch.int32).cuda() for i in range(3))
+    q = (torch.randn(len(rows), heads, dim, generator=torch.Generator().manual_seed(8)) * 2).to(DT[q_t]).cuda()
+    out = torch.full((len(rows), heads, dim), 5.0, dtype=DT[out_t], device="cuda")
+    cb.paged_attention(q, k, v, table, n, seq=seq, starts=start, out=out, prompt=True)
+    lengths = [r[1] if 0 <= r[0] < len(lens) else min(r[1], 0) for r in rows]
+    sq = [r[0] if 0 <= r[0] < len(lens) else 0 for r in rows]
+    check_rows(out, q, keys, vals, [r[2] for r in rows], sq, lengths, dim ** -0.5, out_t, out_t == "bf16")
+    assert bool((out[[i for i, r in enumerate(rows) if r[1] < 0]] == 5).all())
+    if not shuffled:                                       # a prompt without starts: by the sizes' rule, and in place
+        own = [i for i, r in enumerate(rows) if r[0] == 0]
+        qs = q[own].contiguous()
+        want = cb.paged_attention(qs, k, v, table[:1], n[own], seq=seq[own], prompt=True)
+        live = n[own] >= 0                                 # (a padding row of a new tensor holds anything)
+        assert torch.equal(cb.paged_attention(qs, k, v, table[:1], n[own], seq=seq[own])[live], want[live])
+        alone = cb.paged_attention(qs, k, v, table[:1], n[own], seq=seq[own], prompt=False)
+        check_rows(want, qs, keys, vals, None, [0] * len(own), [int(x) for x in n[own]], dim ** -0.5, q_t, q_t == "bf16")
+        check_rows(alone, qs, keys, vals, None, [0] * len(own), [int(x) for x in n[own]], dim ** -0.5, q_t, q_t == "bf16")
+        assert torch.equal(cb.paged_attention(qs, k, v, table[:1], n[own], seq=seq[own], out=qs, prompt=True)[live], want[live])
+
+
+@pytest.mark.parametrize("q_t,kv_t", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_attention_of_prompts_keeps_later_values_out(q_t, kv_t, bad):
+    """A value that is not finite reaches the rows that see its key, in its element, and no other row of the tiles it lies in; keys off the pool likewise."""
+    lens, at = [200], 133
+    k, v, table, keys, vals = make_cache(lens, 16, 4, 64, kv_t, 81)
+    page, slot = int(table[0, at // 16]), at % 16
+    n = torch.arange(1, 201, dtype=torch.int32).cuda()
+    seq = torch.zeros(200, dtype=torch.int32).cuda()
+    q = torch.randn(200, 8, 64, generator=torch.Generator().manual_seed(9)).to(DT[q_t]).cuda()
+    want = cb.paged_attention(q, k, v, table, n, seq=seq, prompt=True)
+    v[page, slot, 2, 11] = bad
+    got = cb.paged_attention(q, k, v, table, n, seq=seq, prompt=True)
+    hit = torch.zeros(200, 8, 64, dtype=torch.bool)
+    hit[at:, 4:6, 11] = True
+    assert not bool(got[hit].isfinite().any())
+    got[hit] = want[hit]                                  # (every other element as if the value were finite; summed in another order, so not bit for bit)
+    check_rows(got, q, keys, vals, None, [0] * 200, list(range(1, 201)), 0.125, q_t, q_t == "bf16")
+    v[page, slot, 2, 11] = 0
+    k[page, slot, 1, 5] = float("nan")
+    got = cb.paged_attention(q, k, v, table, n, seq=seq, prompt=True)
+    assert bool(got[at:, 2:4].isnan().all()) and torch.equal(got[:at], want[:at]) and bool(got[at:, 4:].isfinite().all())
+    k[page, slot, 1, 5] = 0
+    table[0, 6] = -1                                     # keys 96..111 are absent: their values do not matter
+    got = cb.paged_attention(q, k, v, table, n, seq=seq, prompt=True)
+    for r in (95, 96, 111, 112, 199):
+        there = [j for j in range(r + 1) if not 96 <= j < 112]
+        kk, vv = k[table[0].clamp(min=0).long()].flatten(0, 1)[there], v[table[0].clamp(min=0).long()].flatten(0, 1)[there]
+        check_rows(got[r:r + 1], q[r:r + 1], [np64(kk)], [np64(vv)], None, [0], [len(there)], 0.125, q_t, q_t == "bf16")
+
+
 def test_attention_offsets_past_32_bits():
     """A pool of more than 2^31 elements: pages at both ends."""
     page, hk, d = 256, 8, 128

@@ -80,7 +80,7 @@ def test_outputs_that_overlap_are_refused():
 
 
 @pytest.mark.parametrize("kw,word", [(dict(rows=-2), "q_heads"), (dict(q_heads=3), "multiple"), (dict(q_heads=0), "multiple"), (dict(q_dtype=5), "dtypes"),
-                                     (dict(q_dtype=_lib.W_BF16), "bf16 cache"), (dict(length_add=2), "length_add"), (dict(max_length=-1), "max_length"),
+                                     (dict(q_dtype=_lib.W_BF16), "bf16 cache"), (dict(length_add=2), "length_add"), (dict(prompt=2), "prompt"), (dict(prompt=-2), "prompt"), (dict(max_length=-1), "max_length"),
                                      (dict(scale=float("inf")), "finite"), (dict(q=None), "null"), (dict(lengths=None), "null"), (dict(out=P + 4), "16 bytes"),
                                      (dict(out_stride=(256, 63)), "16 bytes"), (dict(rows=4), "sequences"), (dict(rows=1 << 23, seq=P), "pairs"), (dict(out_stride=(512, 64)), "same strides"),
                                      (dict(out_dtype=_lib.W_BF16), "same strides")])
