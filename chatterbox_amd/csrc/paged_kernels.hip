@@ -524,7 +524,8 @@ __global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
 // ---- attention of a prompt's rows -------------------------------------------------------------------------------------------------
 // The same sums where neighbouring rows belong to one sequence: the 16 columns of a tile are 16 / G rows with the G heads of one key head, so a key
 // is read once for all of them (from L2: the blocks that read it are kv_heads apart).  Bound: the matrix and vector work of a tile, a few hundred
-// cycles for 32 keys x 16 columns.  Rows of a block that belong to other sequences are taken in turn (a column that is not in turn has weight
+// cycles for 32 keys x 16 columns (8000 rows of a prompt, 32 heads over 8 of 128, bf16: 2.2 ms, 239 TFLOP/s; row by row the reads take 4 to 10 times
+// as long).  Rows of a block that belong to other sequences are taken in turn (a column that is not in turn has weight
 // zero), so any rows come out right.  A key that some of the rows see and others do not has weight zero for the others; only if such a tile holds a
 // value that is not finite (0 times it is not 0) are its rows summed one by one.
 // SMALL: pages of fewer than TK keys.
@@ -1003,7 +1004,9 @@ void plan_paged_attention(PagedAttnArgs& a) {
         const long long blocks = prompt_blocks(a);
         a.head_waves = 1;
         a.n_split = 1;
-        a.waves = blocks >= 4096 ? 1 : (blocks >= 2048 ? 2 : 4);
+        // one wave to a block where there are enough (2000 rows of two prompts, 8 key heads of 128, bf16: 1 / 2 / 4 waves 310 / 317 / 342 us; 300 rows
+        // of one 18.1 / 14.7 / 19.2; 64 rows 11.2 / 9.3 / 8.7); fp32 products take longer than the waves' joining (2000 rows of 16 heads 143 / 126 / 112)
+        a.waves = a.c.bf16 ? (blocks >= 2000 ? 1 : (blocks >= 512 ? 2 : 4)) : (blocks >= 8192 ? 2 : 4);
         a.min_tiles = 1;
         return;
     }
@@ -1023,8 +1026,8 @@ void plan_paged_attention(PagedAttnArgs& a) {
     // tile) for as many as are useful.
     const bool wide = a.c.bf16 && a.c.head_dim == 128;
     const long long all = pairs * tiles;             // if every row is as long as the longest
-    // rows differ more, the longer they are: so many blocks even out, unless the rows do so by their number (a prompt of 4096 rows, 8 key heads of
-    // 128: 1 block a row 2377 us, 5 3761; 1024 rows of 400 to 2000 keys: 1 912, 3 943)
+    // rows differ more, the longer they are: so many blocks even out, unless the rows do so by their number (1024 rows of 400 to 2000 keys, 8 key heads
+    // of 128: 1 block a row 912 us, 3 943)
     const long long ragged = pairs >= 4096 ? 1 : std::min(tiles / (wide ? 16 : 20), 8LL);
     a.head_waves = 1;
     a.n_split = 1;

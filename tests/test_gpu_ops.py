@@ -368,6 +368,19 @@ def test_attention_of_prompts_keeps_later_values_out(q_t, kv_t, bad):
         check_rows(got[r:r + 1], q[r:r + 1], [np64(kk)], [np64(vv)], None, [0], [len(there)], 0.125, q_t, q_t == "bf16")
 
 
+@pytest.mark.parametrize("q_t,kv_t,heads,kv_heads,dim,prompts", [("bf16", "bf16", 16, 8, 128, [700, 500]), ("bf16", "bf16", 16, 4, 64, [1500, 40, 1460, 1000]),
+                                                                  ("f32", "bf16", 8, 8, 64, [2050, 2000]), ("f32", "f32", 16, 16, 64, [300] * 30), ("f32", "f32", 8, 1, 128, [901])])
+def test_attention_of_long_prompts(q_t, kv_t, heads, kv_heads, dim, prompts):
+    """Enough rows for blocks of one and of two waves; every 61st row and the ends of each prompt against 64 bits."""
+    k, v, table, keys, vals = make_cache(prompts, 64, kv_heads, dim, kv_t, 91)
+    lens = [n for p in prompts for n in range(1, p + 1)]
+    sq = [i for i, p in enumerate(prompts) for _ in range(p)]
+    q = torch.randn(len(lens), heads, dim, generator=torch.Generator().manual_seed(10)).to(DT[q_t]).cuda()
+    got = cb.paged_attention(q, k, v, table, torch.tensor(lens, dtype=torch.int32).cuda(), seq=torch.tensor(sq, dtype=torch.int32).cuda())
+    some = [r for r in range(len(lens)) if r % 61 == 0 or (r % 7 == 0 and lens[r] <= 2) or (r + 1 < len(lens) and sq[r] != sq[r + 1] and sq[r] % 5 == 0)] + [len(lens) - 1]
+    check_rows(got[some], q[some], keys, vals, None, [sq[r] for r in some], [lens[r] for r in some], dim ** -0.5, q_t, q_t == "bf16")
+
+
 def test_attention_offsets_past_32_bits():
     """A pool of more than 2^31 elements: pages at both ends."""
     page, hk, d = 256, 8, 128
