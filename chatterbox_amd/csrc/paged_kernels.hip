@@ -1035,13 +1035,13 @@ void plan_paged_attention(PagedAttnArgs& a) {
         // short rows: one block, no second launch (16 rows of 16 bf16 heads of 64, up to 464 keys: 9.7 us, in four 12.2)
         a.waves = wide ? 2 : 4;
     } else if (all < 65536) {
-        // as many blocks as the card takes well at once (heads of 128, bf16 or long: one to a CU), of two waves, two tiles and more to a wave; where that
+        // as many blocks as the card takes well at once (heads of 128, bf16 or long: one to a CU), of two waves, about two tiles and more to a wave; where that
         // asks for more than 8 partial results of a shortish row, 8 blocks of four waves (2 rows of 16 fp32 heads, up to 4000 keys: 16.0 us, 16 of
         // two 17.4).  (One to a CU: three rows of 60000 bf16 keys, 8 key heads of 128, 10 x 2 131 us, 43 x 4 141; a row of 10397 fp32 keys, 16 heads
         // of 128, 16 x 4 41 us, 40 x 4 48)
         const bool to_cus = wide || (a.c.head_dim == 128 && tiles > 512);
         long long n = to_cus ? std::max(256 / pairs, 1LL) : ((a.c.bf16 ? 384 : 640) + pairs - 1) / pairs;
-        n = std::min(std::max(n, ragged), std::max(tiles / (wide ? 8 : 4), 1LL));
+        n = std::min(std::max(n, ragged), std::max((tiles + 2) / (wide ? 8 : 4), 1LL));
         a.waves = 2;
         if (n > 8 && tiles <= (wide ? 128 : 512)) {
             n = 8;
