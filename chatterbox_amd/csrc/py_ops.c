@@ -23,8 +23,8 @@ static int (*f_attention)(const t3mi_paged_cache*, const t3mi_attention_args*, v
 static int (*f_logits)(const t3mi_logits_args*, void*);
 
 /* of torch, and _lib.check */
-static PyObject *t_f32, *t_bf16, *t_i32, *t_u8, *c_empty, *c_empty_like, *c_stream, *c_grad, *c_check;
-static PyObject *s_data_ptr, *s_dtype, *s_get_device, *s_shape, *s_stride, *s_requires_grad, *s_device, *kw_dtype_device;
+static PyObject *t_f32, *t_bf16, *t_i32, *c_empty, *c_empty_like, *c_stream, *c_grad, *c_check;
+static PyObject *s_data_ptr, *s_dtype, *s_get_device, *s_shape, *s_stride, *s_requires_grad, *s_device, *s_new_empty, *kw_dtype_device;
 
 enum { F32 = 1, BF16 = 2, I32 = 4 };
 #define MAXD 4
@@ -361,14 +361,10 @@ static PyObject* py_attention(PyObject* self, PyObject* const* a, Py_ssize_t n) 
     int rc = f_workspace(&c, &g, &g.workspace_bytes);
     if (rc || rows == 0) return result(rc, out);
     if (g.workspace_bytes) {
-        PyObject* size = PyLong_FromSize_t(g.workspace_bytes);
-        PyObject* dev = size ? PyObject_GetAttr(a[0], s_device) : NULL;
-        if (dev) {
-            PyObject* args[3] = {size, t_u8, dev};
-            ws = PyObject_Vectorcall(c_empty, args, 1, kw_dtype_device);
-        }
+        /* (of q's type and on its device: the cheapest way to ask torch for memory) */
+        PyObject* size = PyLong_FromSize_t((g.workspace_bytes + 3) / (q.dtype == BF16 ? 2 : 4));
+        ws = size ? PyObject_CallMethodOneArg(a[0], s_new_empty, size) : NULL;
         Py_XDECREF(size);
-        Py_XDECREF(dev);
         PyObject* r = ws ? PyObject_CallMethodNoArgs(ws, s_data_ptr) : NULL;
         if (!r) goto fail;
         g.workspace = PyLong_AsVoidPtr(r);
@@ -481,11 +477,11 @@ fail:
     return NULL;
 }
 
-/* bind(4 addresses, float32, bfloat16, int32, uint8, empty, empty_like, raw stream of a device, is_grad_enabled, check, torch.Tensor, its DLPack
+/* bind(4 addresses, float32, bfloat16, int32, empty, empty_like, raw stream of a device, is_grad_enabled, check, torch.Tensor, its DLPack
  * exchange capsule or None) */
 static PyObject* py_bind(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     (void)self;
-    if (wanted("bind", n, 15)) return NULL;
+    if (wanted("bind", n, 14)) return NULL;
     void* p[4];
     for (int i = 0; i < 4; ++i) {
         p[i] = PyLong_AsVoidPtr(a[i]);
@@ -495,18 +491,18 @@ static PyObject* py_bind(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     f_workspace = (int (*)(const t3mi_paged_cache*, const t3mi_attention_args*, size_t*))p[1];
     f_attention = (int (*)(const t3mi_paged_cache*, const t3mi_attention_args*, void*))p[2];
     f_logits = (int (*)(const t3mi_logits_args*, void*))p[3];
-    PyObject** keep[9] = {&t_f32, &t_bf16, &t_i32, &t_u8, &c_empty, &c_empty_like, &c_stream, &c_grad, &c_check};
-    for (int i = 0; i < 9; ++i) {
+    PyObject** keep[8] = {&t_f32, &t_bf16, &t_i32, &c_empty, &c_empty_like, &c_stream, &c_grad, &c_check};
+    for (int i = 0; i < 8; ++i) {
         Py_INCREF(a[4 + i]);
         Py_XSETREF(*keep[i], a[4 + i]);
     }
 #ifdef T3MI_DLPACK
     f_dltensor = NULL;
-    if (PyType_Check(a[13]) && PyCapsule_IsValid(a[14], "dlpack_exchange_api")) {
-        const DLPackExchangeAPI* x = PyCapsule_GetPointer(a[14], "dlpack_exchange_api");
+    if (PyType_Check(a[12]) && PyCapsule_IsValid(a[13], "dlpack_exchange_api")) {
+        const DLPackExchangeAPI* x = PyCapsule_GetPointer(a[13], "dlpack_exchange_api");
         if (x->header.version.major == DLPACK_MAJOR_VERSION) {   /* (the table lives as long as torch does) */
-            Py_INCREF(a[13]);
-            Py_XSETREF(t_tensor, a[13]);
+            Py_INCREF(a[12]);
+            Py_XSETREF(t_tensor, a[12]);
             f_dltensor = x->dltensor_from_py_object_no_sync;
         }
     }
@@ -524,7 +520,7 @@ static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", "tensors to t
 
 PyMODINIT_FUNC PyInit__ops(void) {
     struct { PyObject** o; const char* s; } names[] = {{&s_data_ptr, "data_ptr"}, {&s_dtype, "dtype"}, {&s_get_device, "get_device"}, {&s_shape, "shape"},
-                                                        {&s_stride, "stride"}, {&s_requires_grad, "requires_grad"}, {&s_device, "device"}};
+                                                        {&s_stride, "stride"}, {&s_requires_grad, "requires_grad"}, {&s_device, "device"}, {&s_new_empty, "new_empty"}};
     for (size_t i = 0; i < sizeof(names) / sizeof(names[0]); ++i)
         if (!(*names[i].o = PyUnicode_InternFromString(names[i].s))) return NULL;
     if (!(kw_dtype_device = Py_BuildValue("(ss)", "dtype", "device"))) return NULL;

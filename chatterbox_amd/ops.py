@@ -32,7 +32,7 @@ def _bind():
              for n in ("t3mi_paged_append", "t3mi_paged_attention_workspace", "t3mi_paged_attention", "t3mi_process_logits")]
     # the raw handle of torch's current stream; the spelled-out way where this torch has no short one
     stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
-    ext.bind(*entry, torch.float32, torch.bfloat16, torch.int32, torch.uint8, torch.empty, torch.empty_like, stream, torch.is_grad_enabled, _lib.check,
+    ext.bind(*entry, torch.float32, torch.bfloat16, torch.int32, torch.empty, torch.empty_like, stream, torch.is_grad_enabled, _lib.check,
              torch.Tensor, getattr(torch.Tensor, "__dlpack_c_exchange_api__", None))
     _ops = ext
     return ext
