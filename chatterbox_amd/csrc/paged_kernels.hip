@@ -140,8 +140,9 @@ __device__ __forceinline__ void store_out(const PagedAttnArgs& a, int row, int h
 // product, values after the second, one tile in flight per wave all the time.  Waves of a block take every nw-th tile and meet in LDS;
 // blocks of a row (split) leave (max, sum, weighted sum) in the workspace for paged_join_kernel.
 // Types: bf16 operands go to the bf16 matrix instruction.  An fp32 query over a bf16 cache is cut into three bf16 parts of 8 significant
-// bits each, which hold it exactly, and so are the weights when the result is fp32; a bf16 result rounds each weight to bf16 (the
-// result is rounded as coarsely).  An fp32 cache uses the exact fp32 matrix instruction.  Sums, maxima and products: fp32.
+// bits each, which hold it exactly, and so are the weights when the result is fp32.  Under a bf16 result a weight is two rounded parts, 2^-16 of it off
+// at most: a 256th of what the result's own rounding may be off.  (One part would be off by as much as the result: its error against 64 bits 1.77e-3
+// instead of 1.68e-3 over 3 rows of 100003 to 131071 keys.)  An fp32 cache uses the exact fp32 matrix instruction.  Sums, maxima and products: fp32.
 
 // over the four 16-lane groups of a wave (lanes n, n + 16, n + 32, n + 48), by register swaps
 template <typename F> __device__ __forceinline__ float over_groups(float x, F f) {
@@ -157,11 +158,15 @@ __device__ __forceinline__ float group_sum(float x) { return over_groups(x, [](f
 // the leading 8 significant bits of x; what is left over is x - lead(x), exactly
 __device__ __forceinline__ float lead(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
 
-// eight floats as PARTS bf16 vectors: rounded (1), or cut into three parts that hold them exactly (3)
+// eight floats as bf16 vectors: three parts of 8 significant bits, which hold them exactly, or two rounded ones, off by at most 2^-16 of the value
 template <int PARTS> __device__ __forceinline__ void to_parts(const float (&x)[8], bf16x8 (&o)[PARTS]) {
-    if constexpr (PARTS == 1) {
+    static_assert(PARTS == 2 || PARTS == 3, "two parts or three");
+    if constexpr (PARTS == 2) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[0][j] = (__bf16)x[j];
+        for (int j = 0; j < 8; ++j) {
+            o[0][j] = (__bf16)x[j];
+            o[1][j] = (__bf16)(x[j] - (float)o[0][j]);
+        }
     } else {
         float r[8];
 #pragma unroll
@@ -211,7 +216,7 @@ __device__ __forceinline__ RowPlan plan_row(const PagedAttnArgs& a, int len, int
 }
 
 // QB, KB: bf16 queries, bf16 cache.  TK: keys of a tile, 32 or (fp32 cache) 16.  PAGES 0: pages of TK keys and more (a tile lies in one),
-// 1: smaller ones of 4 keys and more, 2: of 1, 2.  PARTS: bf16 parts of a weight (bf16 cache only).
+// 1: smaller ones of 4 keys and more, 2: of 1, 2.  PARTS: bf16 parts of a weight (bf16 cache only; otherwise 1).
 template <bool QB, bool KB, int D, int TK, int PAGES, int PARTS>
 __global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) float sm[];
@@ -956,14 +961,14 @@ void launch_prompt_d(const PagedAttnArgs& a, unsigned blocks, unsigned threads, 
         if (small) hipLaunchKernelGGL((paged_prompt_kernel<false, false, D, 16, true, 1>), grid, block, lds, s, a);
         else hipLaunchKernelGGL((paged_prompt_kernel<false, false, D, 16, false, 1>), grid, block, lds, s, a);
     } else if (a.q_bf16 && a.out_bf16) {
-        if (small) hipLaunchKernelGGL((paged_prompt_kernel<true, true, D, 32, true, 1>), grid, block, lds, s, a);
-        else hipLaunchKernelGGL((paged_prompt_kernel<true, true, D, 32, false, 1>), grid, block, lds, s, a);
+        if (small) hipLaunchKernelGGL((paged_prompt_kernel<true, true, D, 32, true, 2>), grid, block, lds, s, a);
+        else hipLaunchKernelGGL((paged_prompt_kernel<true, true, D, 32, false, 2>), grid, block, lds, s, a);
     } else if (a.q_bf16) {
         if (small) hipLaunchKernelGGL((paged_prompt_kernel<true, true, D, 32, true, 3>), grid, block, lds, s, a);
         else hipLaunchKernelGGL((paged_prompt_kernel<true, true, D, 32, false, 3>), grid, block, lds, s, a);
     } else if (a.out_bf16) {
-        if (small) hipLaunchKernelGGL((paged_prompt_kernel<false, true, D, 32, true, 1>), grid, block, lds, s, a);
-        else hipLaunchKernelGGL((paged_prompt_kernel<false, true, D, 32, false, 1>), grid, block, lds, s, a);
+        if (small) hipLaunchKernelGGL((paged_prompt_kernel<false, true, D, 32, true, 2>), grid, block, lds, s, a);
+        else hipLaunchKernelGGL((paged_prompt_kernel<false, true, D, 32, false, 2>), grid, block, lds, s, a);
     } else {
         if (small) hipLaunchKernelGGL((paged_prompt_kernel<false, true, D, 32, true, 3>), grid, block, lds, s, a);
         else hipLaunchKernelGGL((paged_prompt_kernel<false, true, D, 32, false, 3>), grid, block, lds, s, a);
@@ -972,9 +977,9 @@ void launch_prompt_d(const PagedAttnArgs& a, unsigned blocks, unsigned threads, 
 template <int D>
 void launch_attention_d(const PagedAttnArgs& a, unsigned blocks, unsigned threads, size_t lds, hipStream_t s) {
     if (!a.c.bf16) launch_attention_p<false, false, D, 16, 1>(a, blocks, threads, lds, s);
-    else if (a.q_bf16 && a.out_bf16) launch_attention_p<true, true, D, 32, 1>(a, blocks, threads, lds, s);
+    else if (a.q_bf16 && a.out_bf16) launch_attention_p<true, true, D, 32, 2>(a, blocks, threads, lds, s);
     else if (a.q_bf16) launch_attention_p<true, true, D, 32, 3>(a, blocks, threads, lds, s);
-    else if (a.out_bf16) launch_attention_p<false, true, D, 32, 1>(a, blocks, threads, lds, s);
+    else if (a.out_bf16) launch_attention_p<false, true, D, 32, 2>(a, blocks, threads, lds, s);
     else launch_attention_p<false, true, D, 32, 3>(a, blocks, threads, lds, s);
     // (96 rows of 32 heads, 3 partial results each: 8.3 us with a block to each, 5.1 with a wave)
     if (a.n_split > 8) hipLaunchKernelGGL((paged_join_kernel<D>), dim3((unsigned)(a.rows * a.q_heads)), dim3(256), 0, s, a);
