@@ -143,6 +143,9 @@ __device__ __forceinline__ void store_out(const PagedAttnArgs& a, int row, int h
 // bits each, which hold it exactly, and so are the weights when the result is fp32.  Under a bf16 result a weight is two rounded parts, 2^-16 of it off
 // at most: a 256th of what the result's own rounding may be off.  (One part would be off by as much as the result: its error against 64 bits 1.77e-3
 // instead of 1.68e-3 over 3 rows of 100003 to 131071 keys.)  An fp32 cache uses the exact fp32 matrix instruction.  Sums, maxima and products: fp32.
+// Parts and infinities: a part of an ordinary number may be 0, and 0 times an infinite key or value is NaN where the number itself gives an infinity.  A wave
+// whose sums end as NaN goes through its keys a second time (whole_pass) and takes the columns concerned from products of whole numbers: NaN that the
+// formula has comes out again, anything else as it should be.  Nothing is looked for on the way: finite keys and values pay for one test at the end.
 
 // over the four 16-lane groups of a wave (lanes n, n + 16, n + 32, n + 48), by register swaps
 template <typename F> __device__ __forceinline__ float over_groups(float x, F f) {
@@ -158,8 +161,9 @@ __device__ __forceinline__ float group_sum(float x) { return over_groups(x, [](f
 // the leading 8 significant bits of x; what is left over is x - lead(x), exactly
 __device__ __forceinline__ float lead(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
 
-// eight floats as bf16 vectors: three parts of 8 significant bits, which hold them exactly, or two rounded ones, off by at most 2^-16 of the value
-template <int PARTS> __device__ __forceinline__ void to_parts(const float (&x)[8], bf16x8 (&o)[PARTS]) {
+// eight floats as bf16 vectors: three parts of 8 significant bits, which hold them exactly, or two rounded ones, off by at most 2^-16 of the value.  INF:
+// there may be infinities among them (which are their first part)
+template <int PARTS, bool INF = false> __device__ __forceinline__ void to_parts(const float (&x)[8], bf16x8 (&o)[PARTS]) {
     static_assert(PARTS == 2 || PARTS == 3, "two parts or three");
     if constexpr (PARTS == 2) {
 #pragma unroll
@@ -178,14 +182,107 @@ template <int PARTS> __device__ __forceinline__ void to_parts(const float (&x)[8
             for (int j = 0; j < 4; ++j) {
                 w[j] = __builtin_amdgcn_perm(__float_as_uint(r[2 * j + 1]), __float_as_uint(r[2 * j]), 0x07060302u);
                 if (s + 1 < PARTS) {
-                    r[2 * j] -= lead(r[2 * j]);
-                    r[2 * j + 1] -= lead(r[2 * j + 1]);
+#pragma unroll
+                    for (int i = 2 * j; i < 2 * j + 2; ++i) r[i] = INF && r[i] == lead(r[i]) ? 0.f : r[i] - lead(r[i]);
                 }
             }
             o[s] = __builtin_bit_cast(bf16x8, w);
         }
     }
 }
+
+__device__ __forceinline__ float bf16_of(unsigned w, int half) { return __uint_as_float(half ? w & 0xFFFF0000u : w << 16); }
+
+// whether a wave's vote is set for this lane's column (lane & 15) in any of its four groups
+__device__ __forceinline__ bool in_column(unsigned long long vote, int n) {
+    vote |= vote >> 32;
+    return ((vote | vote >> 16) >> n) & 1u;
+}
+
+// The sums of a wave over a bf16 cache from whole fp32 numbers: tiles t, t + step, ... below t_end of the sequence whose pages are trow, no key from hi on.
+// Column n (its queries cut into the parts qb, which add up to them) sees the keys [first, len); the columns of a row are `group` neighbours.
+// m, l, acc: maximum, sum and weighted sum so far, laid out as in the kernels below.  Rare, so built for size: a tile at a time, a row at a time.
+template <int QS, int KC, int NT, typename VT>
+__device__ __forceinline__ void whole_pass(const PagedCache& c, const char* kbase, const char* vbase, const int* trow, const bf16x8 (&qb)[QS][KC], float scale2, int t,
+                                           int t_end, int step, int hi, int first, int len, int group, float& m, float& l, f32x4 (&acc)[NT]) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, in_page = (1 << c.page_shift) - 1;
+    for (; t < t_end; t += step) {
+        f32x4 s[2];
+        VT vr[8];
+        unsigned ok = 0u;                            // bit j: key j of this lane's values has a page
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int key = min(t * 32 + 16 * u + n, hi - 1), id = trow[key >> c.page_shift];
+            const char* base = kbase + ((long long)(id >= 0 && id < c.n_pages ? id : 0) * c.kp + (long long)(key & in_page) * c.ks) * 2 + 16 * g;
+            s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < KC; ++x) {
+                const u32x4 kr = *reinterpret_cast<const u32x4*>(base + 64 * x);
+                u32x4 qw[QS];
+#pragma unroll
+                for (int part = 0; part < QS; ++part) {
+                    qw[part] = __builtin_bit_cast(u32x4, qb[part][x]);
+                    asm volatile("" : "+v"(qw[part]));   // (put together here, not kept whole for all tiles: registers)
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float q = bf16_of(qw[QS - 1][j >> 1], j & 1);
+#pragma unroll
+                    for (int part = QS - 2; part >= 0; --part) q += bf16_of(qw[part][j >> 1], j & 1);
+                    s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(bf16_of(kr[j >> 1], j & 1), q, s[u], 0, 0, 0);
+                }
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);           // (values after the scores: registers)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int at = t * 32 + 16 * (j >> 2) + 4 * g + (j & 3), key = min(at, hi - 1), id = trow[key >> c.page_shift];
+            const bool good = id >= 0 && id < c.n_pages;
+            ok |= good && at < hi ? 1u << j : 0u;
+            vr[j] = *reinterpret_cast<const VT*>(vbase + ((long long)(good ? id : 0) * c.vp + (long long)(key & in_page) * c.vs) * 2 + sizeof(VT) * n);
+        }
+        float p[8], mx = m;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int key = t * 32 + 16 * (j >> 2) + 4 * g + (j & 3);
+            p[j] = ((ok >> j) & 1u) && key >= first && key < len ? s[j >> 2][j & 3] * scale2 : -INFINITY;
+            mx = fmaxf(mx, p[j]);
+        }
+        mx = group_max(mx);
+        const float ref = mx > -INFINITY ? mx : 0.f, keep = m == mx ? 1.f : __builtin_amdgcn_exp2f(m - ref);
+        m = mx;
+        l *= keep;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            p[j] = p[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[j] - ref);
+            l += p[j];
+        }
+#pragma unroll
+        for (int e = 0; e < NT; ++e) acc[e] *= keep;
+        for (int r = 0; r * group < 16; ++r) {
+            const int f_r = __builtin_amdgcn_readlane(first, r * group), l_r = __builtin_amdgcn_readlane(len, r * group);
+            unsigned of = 0u;                        // the keys that row r sees
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = t * 32 + 16 * (j >> 2) + 4 * g + (j & 3);
+                of |= key >= f_r && key < l_r ? (ok >> j & 1u) << j : 0u;
+            }
+            if (__builtin_amdgcn_ballot_w64(of != 0u) == 0) continue;
+#pragma unroll
+            for (int e = 0; e < NT; ++e) {
+                f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    o = __builtin_amdgcn_mfma_f32_16x16x4f32((of >> j) & 1u ? bf16_of(vr[j][e >> 1], e & 1) : 0.f, p[j], o, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[e][i] += n / group == r ? o[i] : 0.f;
+            }
+        }
+    }
+}
+
+// from 2^16 up, but finite (a column of an infinite maximum comes out as NaN either way, and does not change how its neighbours are rounded)
+__device__ __forceinline__ bool large(float x) { return (__float_as_uint(x) & 0x7FFFFFFFu) - 0x47800000u < 0x7F800000u - 0x47800000u; }
 
 // what a part's sums count, its maximum being m and that of all parts top.  A part without a maximum saw no key, and its sums are 0, or it saw
 // NaN scores alone, and they are NaN: taken as they are
@@ -218,7 +315,7 @@ __device__ __forceinline__ RowPlan plan_row(const PagedAttnArgs& a, int len, int
 // QB, KB: bf16 queries, bf16 cache.  TK: keys of a tile, 32 or (fp32 cache) 16.  PAGES 0: pages of TK keys and more (a tile lies in one),
 // 1: smaller ones of 4 keys and more, 2: of 1, 2.  PARTS: bf16 parts of a weight (bf16 cache only; otherwise 1).
 template <bool QB, bool KB, int D, int TK, int PAGES, int PARTS>
-__global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(512, QB && D == 128 && PAGES == 1 ? 3 : 2) void paged_attention_kernel(PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) float sm[];
     constexpr int EB = KB ? 2 : 4;                  // bytes of a cache element
     constexpr int KC = KB ? D / 32 : D / 16;        // 16-byte pieces of a key to a lane
@@ -276,7 +373,7 @@ __global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = live ? __uint_as_float(qw[c][j >> 2][j & 3]) : 0.f;
                 bf16x8 o[3];
-                to_parts<3>(x, o);
+                to_parts<3, true>(x, o);
 #pragma unroll
                 for (int s = 0; s < QS; ++s) qb[s][c] = o[s];
             } else {
@@ -438,7 +535,7 @@ __global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
             }
             // Scores of ordinary size: the product with the scale is not rounded before the maximum comes off.  Beyond 2^16 that rounding is what the
             // maximum itself carries, and has to cancel.
-            if (__builtin_amdgcn_ballot_w64(!(fabsf(ref) < 65536.f)) == 0) {
+            if (__builtin_amdgcn_ballot_w64(large(ref)) == 0) {
 #pragma unroll
                 for (int j = 0; j < J; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], scale2, -ref));
                 if (masked) {
@@ -475,6 +572,27 @@ __global__ __launch_bounds__(512) void paged_attention_kernel(PagedAttnArgs a) {
             t += kw;
             if (t >= t_end) break;
             pg = next;
+        }
+    }
+    if constexpr (KB) {
+        bool nan = l != l;
+#pragma unroll
+        for (int e = 0; e < NT; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) nan = nan || acc[e][i] != acc[e][i];
+        if (const unsigned long long vote = __builtin_amdgcn_ballot_w64(nan && n < gn); vote != 0) {
+            f32x4 acc2[NT];
+#pragma unroll
+            for (int e = 0; e < NT; ++e) acc2[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+            float m2 = -INFINITY, l2 = 0.f;
+            whole_pass<QS, KC, NT, VT>(a.c, kbase, vbase, trow, qb, scale2, t_begin + wk, t_end, kw, rp.len, rp.first, rp.len, 16, m2, l2, acc2);
+            const bool redo = in_column(vote, n);
+            m = redo ? m2 : m;
+            l = redo ? l2 : l;
+#pragma unroll
+            for (int e = 0; e < NT; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[e][i] = redo ? acc2[e][i] : acc[e][i];
         }
     }
     l = group_sum(l);
@@ -564,7 +682,7 @@ __global__ __launch_bounds__(256, D == 64 && !(SMALL && KB && !QB) ? 3 : 2) void
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = col ? x[j] : 0.f;
                 bf16x8 o[3];
-                to_parts<3>(x, o);
+                to_parts<3, true>(x, o);
 #pragma unroll
                 for (int s = 0; s < QS; ++s) qb[s][c] = o[s];
             } else {
@@ -592,13 +710,16 @@ __global__ __launch_bounds__(256, D == 64 && !(SMALL && KB && !QB) ? 3 : 2) void
     const float scale2 = a.scale * 1.4426950408889634f;
     const unsigned alive = (unsigned)__builtin_amdgcn_ballot_w64(has) & 0xFFFFu;
     unsigned pending = alive;
-    while (pending != 0u) {
-        // the columns of the first pending one's sequence, and the keys they span: [lo, hi), all of them see [lo_all, hi_all)
-        const int sq = __builtin_amdgcn_readlane(seq, __builtin_ctz(pending));
-        const unsigned in = (unsigned)__builtin_amdgcn_ballot_w64(has && seq == sq) & 0xFFFFu;
+    int sq, lo, hi, lo_all, hi_all;
+    unsigned in;
+    bool mine;
+    // the columns of the first pending one's sequence sq, and the keys they span: [lo, hi), all of them see [lo_all, hi_all)
+    auto next_sequence = [&]() {
+        sq = __builtin_amdgcn_readlane(seq, __builtin_ctz(pending));
+        in = (unsigned)__builtin_amdgcn_ballot_w64(has && seq == sq) & 0xFFFFu;
         pending &= ~in;
-        const bool mine = (in >> n) & 1u;
-        int lo = mine ? first : 0x7FFFFFFF, lo_all = mine ? first : 0, hi = mine ? len : 0, hi_all = mine ? len : 0x7FFFFFFF;
+        mine = (in >> n) & 1u;
+        lo = mine ? first : 0x7FFFFFFF, lo_all = mine ? first : 0, hi = mine ? len : 0, hi_all = mine ? len : 0x7FFFFFFF;
 #pragma unroll
         for (int d = 1; d < 16; d <<= 1) {
             lo = min(lo, __shfl_xor(lo, d, 64));
@@ -610,6 +731,9 @@ __global__ __launch_bounds__(256, D == 64 && !(SMALL && KB && !QB) ? 3 : 2) void
         lo_all = __builtin_amdgcn_readfirstlane(lo_all);
         hi = __builtin_amdgcn_readfirstlane(hi);
         hi_all = __builtin_amdgcn_readfirstlane(hi_all);
+    };
+    while (pending != 0u) {
+        next_sequence();
         const int* trow = a.c.table + (long long)sq * a.c.table_stride;
         const int t_end = (hi + TK - 1) / TK;
         int t = lo / TK + wave;
@@ -726,7 +850,7 @@ __global__ __launch_bounds__(256, D == 64 && !(SMALL && KB && !QB) ? 3 : 2) void
                 for (int e = 0; e < NT; ++e) acc[e] *= keep;
                 m = mx;
             }
-            if (__builtin_amdgcn_ballot_w64(!(fabsf(ref) < 65536.f)) == 0) {   // (as above)
+            if (__builtin_amdgcn_ballot_w64(large(ref)) == 0) {   // (as above)
 #pragma unroll
                 for (int j = 0; j < J; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], scale2, -ref));
             } else {
@@ -783,6 +907,32 @@ __global__ __launch_bounds__(256, D == 64 && !(SMALL && KB && !QB) ? 3 : 2) void
             t += nw;
             if (t >= t_end) break;
             pg = next;
+        }
+    }
+    if constexpr (KB) {
+        bool nan = l != l;
+#pragma unroll
+        for (int e = 0; e < NT; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) nan = nan || acc[e][i] != acc[e][i];
+        if (const unsigned long long vote = __builtin_amdgcn_ballot_w64(nan && has); vote != 0) {
+            f32x4 acc2[NT];
+#pragma unroll
+            for (int e = 0; e < NT; ++e) acc2[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+            float m2 = -INFINITY, l2 = 0.f;
+            pending = alive;
+            while (pending != 0u) {
+                next_sequence();
+                whole_pass<QS, KC, NT, VT>(a.c, kbase, vbase, a.c.table + (long long)sq * a.c.table_stride, qb, scale2, lo / TK + wave, (hi + TK - 1) / TK, nw, hi,
+                                           first, mine ? len : 0, group, m2, l2, acc2);
+            }
+            const bool redo = in_column(vote, n);
+            m = redo ? m2 : m;
+            l = redo ? l2 : l;
+#pragma unroll
+            for (int e = 0; e < NT; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[e][i] = redo ? acc2[e][i] : acc[e][i];
         }
     }
     l = group_sum(l);

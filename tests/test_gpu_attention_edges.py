@@ -32,3 +32,77 @@ def test_weights_under_a_bf16_result_are_not_rounded_to_it(q_t, prompt, heads, k
         tol = (2 * (2 * err * U + 2.0 ** -21 + n * U) + 2.0 ** -16) * mag
         tol += 2.0 ** -8 * (np.abs(ref) + tol)
         assert (np.abs(got[r] - ref) <= tol).all(), (r, n, float((np.abs(got[r] - ref) / tol).max()))
+
+
+def ref_row(q, k, v, scale):
+    """One row and key head: q [G, D], k, v [n, D] in 64 bits -> out [G, D], sum p |v| over the finite values, largest finite score error / U."""
+    with np.errstate(all="ignore"):
+        s = (q[:, None] * k[None]).sum(-1) * scale
+        err = np.where(np.isfinite(s), (q.shape[1] + 2) * (np.abs(q)[:, None] * np.where(np.isfinite(k), np.abs(k), 0)[None]).sum(-1) * abs(scale), 0).max()
+        p = np.exp(s - s.max(1, keepdims=True))
+        p = p / p.sum(1, keepdims=True)
+        return (p[:, :, None] * v[None]).sum(1), (p[:, :, None] * np.where(np.isfinite(v), np.abs(v), 0)[None]).sum(1), err
+
+
+@pytest.mark.parametrize("q_t,kv_t,out_t", [("f32", "bf16", "f32"), ("f32", "bf16", "bf16"), ("bf16", "bf16", "f32"), ("bf16", "bf16", "bf16"), ("f32", "f32", "f32")])
+@pytest.mark.parametrize("prompt,heads,kv_heads,dim,page,most", [(False, 4, 2, 64, 64, 0), (False, 6, 2, 128, 8, 0), (False, 4, 2, 64, 1, 0), (False, 8, 2, 128, 64, 20000),
+                                                                 (False, 40, 2, 64, 32, 0), (True, 4, 2, 64, 64, 0), (True, 6, 2, 128, 8, 0), (True, 2, 2, 64, 16, 0)])
+def test_infinities(q_t, kv_t, out_t, prompt, heads, kv_heads, dim, page, most):
+    """Queries that bf16 holds exactly against keys and values with infinities in them.  A key of -inf score has no weight, one of +inf makes its rows NaN, an
+    infinite value comes out in its element wherever its key is seen (also alone, with weight 1); everything else is as the formula has it, to the
+    tolerance; key heads without infinities keep their bits."""
+    lens = [400, 130, 1, 33, 2000]
+    k, v, table, keys, vals = make_cache(lens, page, kv_heads, dim, kv_t, 17)
+    inf = float("inf")
+
+    def put(which, held, s, j, e, x):
+        which[int(table[s, j // page]), j % page, 0, e] = x
+        held[s][j, 0, e] = x
+
+    g = np.random.default_rng(2)
+    sign = np.sign(g.standard_normal(dim))
+    for s, j in ((0, 7), (0, 333), (1, 129), (4, 1999), (4, 31)):
+        put(k, keys, s, j, 5, -inf * sign[5])               # (every query has this sign there: score -inf)
+    put(k, keys, 3, 20, 9, inf * sign[9])                   # score +inf
+    for s, j, e, x in ((0, 100, 3, inf), (0, 200, 4, -inf), (1, 50, 3, -inf), (2, 0, 6, inf), (4, 1500, 1, inf), (4, 1501, 1, -inf)):
+        put(v, vals, s, j, e, x)
+    seen = [(s, n) for s in range(5) for n in (range(max(1, lens[s] - 12), lens[s] + 1) if prompt else [lens[s]])]
+    q = torch.from_numpy(np.abs(g.standard_normal((len(seen), heads, dim))) * sign + 0.25 * sign).float().bfloat16().to(DT[q_t]).cuda()   # (no zero among them)
+    args = dict(seq=t32([s for s, _ in seen]), out_dtype=DT[out_t], prompt=prompt, max_length=most)
+    n = t32([n for _, n in seen])
+    got = cb.paged_attention(q, k, v, table, n, **args)
+    group = heads // kv_heads
+    for r, (s, m) in enumerate(seen):
+        for h in range(kv_heads):
+            at = slice(h * group, (h + 1) * group)
+            ref, mag, err = ref_row(np64(q[r, at]), keys[s][:m, h], vals[s][:m, h], dim ** -0.5)
+            x = np64(got[r, at])
+            fine = np.isfinite(ref)
+            assert np.array_equal(np.isnan(x), np.isnan(ref)) and np.array_equal(x[np.isinf(ref)], ref[np.isinf(ref)]), (r, s, m, h)
+            tol = 2 * (2 * err * U + 2.0 ** -21 + m * U) * mag
+            if out_t == "bf16":
+                tol = (tol + 2.0 ** -16 * mag) * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(np.where(fine, ref, 0))
+            assert (np.abs(x - ref)[fine] <= tol[fine]).all(), (r, s, m, h)
+    clean = cb.paged_attention(q, torch.nan_to_num(k, posinf=1.0, neginf=1.0), torch.nan_to_num(v, posinf=1.0, neginf=1.0), table, n, **args)
+    assert torch.equal(got[:, group:], clean[:, group:])
+
+
+@pytest.mark.parametrize("q_t,kv_t,out_t", [("f32", "bf16", "f32"), ("f32", "bf16", "bf16"), ("bf16", "bf16", "bf16"), ("f32", "f32", "f32")])
+@pytest.mark.parametrize("prompt", [False, True])
+def test_infinite_queries(q_t, kv_t, out_t, prompt):
+    """An infinite element makes every score +-inf: NaN where one is +inf, nothing seen (zeros) where all are -inf; a NaN element gives NaN; the other rows and
+    heads keep their bits."""
+    lens = [70, 300]
+    k, v, table, _, _ = make_cache(lens, 16, 2, 64, kv_t, 19)
+    k[:, :, 0, 3] = -k[:, :, 0, 3].abs()
+    seq = t32([0, 1, 1, 0, 1])
+    n = t32([70, 300, 299, 69, 298])
+    q = torch.randn(5, 4, 64, generator=torch.Generator().manual_seed(3)).to(DT[q_t]).cuda()
+    args = dict(seq=seq, out_dtype=DT[out_t], prompt=prompt)
+    clean = cb.paged_attention(q, k, v, table, n, **args)
+    q[1, 0, 3], q[2, 1, 3], q[3, 2, 3], q[4, 3, 7] = float("inf"), float("-inf"), float("inf"), float("nan")
+    got = cb.paged_attention(q, k, v, table, n, **args)
+    assert bool((got[1, 0] == 0).all()) and bool(got[2, 1].isnan().all()) and bool(got[3, 2].isnan().all()) and bool(got[4, 3].isnan().all())
+    for r, h in ((1, 0), (2, 1), (3, 2), (4, 3)):
+        got[r, h] = clean[r, h]
+    assert torch.equal(got, clean)
