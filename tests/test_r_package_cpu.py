@@ -48,3 +48,11 @@ cp {CSRC}/"${{name%.*}}".o "$out"
                           cwd=pkg / "src")
     names = subprocess.run(["nm", "-D", "--defined-only", "chatterbox.so"], cwd=pkg / "src", check=True, capture_output=True, text=True).stdout
     assert "t3mi_paged_attention" in names and "t3mi_hift_inference" in names
+
+
+def test_the_library_builds_without_python_headers():
+    """A C or R user needs no Python.h: the library is made, the Python side left out and named."""
+    plan = lambda *a: subprocess.run(["make", "-n", "-B", "-C", CSRC, *a], check=True, capture_output=True, text=True).stdout  # noqa: E731
+    assert "py_ops.c" in plan()
+    out = plan("PYINC=/nonexistent")
+    assert "py_ops.c" not in out and "-o ../libt3mi.so" in out and "no Python.h" in out
