@@ -1403,10 +1403,14 @@ int prefill_rows(t3mi_model* m, Session* s, const std::vector<int>& rows_list, c
 }
 
 // ---- pages of the slots ---------------------------------------------------------------------------------------------------------
-// pages one row of an utterance needs: its prompt and every token up to its limit, never more than the cache rows have room for
+// pages one row of an utterance needs: its prompt and every token up to its limit, never more than a cache row of `room` positions takes
+int pages_of(int page_size, int room, int s0, int limit) {
+    const long long n = std::min<long long>((long long)s0 + limit, room);
+    return (int)((n + page_size - 1) / page_size);
+}
+// (under max_cache_len the sampler ends an utterance there, before the row's own end, which is rounded up)
 int pages_of(const Session* s, int s0, int limit) {
-    const long long n = std::min<long long>((long long)s0 + limit, s->max_len);
-    return (int)((n + s->page_size - 1) / s->page_size);
+    return pages_of(s->page_size, s->prm.max_cache_len > 0 ? std::min(s->prm.max_cache_len, s->max_len) : s->max_len, s0, limit);
 }
 void release_pages(Session* s, int u) {
     s->free_pages.insert(s->free_pages.end(), s->held[u].begin(), s->held[u].end());
@@ -2547,6 +2551,7 @@ struct ContinuousJob {
     std::vector<int32_t> mx;                 // token limit of each utterance (without Turbo's extra first token)
     std::vector<int32_t> order;              // the queue: utterance indices in the order they are started
     std::vector<int32_t> s0;                 // prompt lengths
+    int cache_len = 0;                       // the session's max_cache_len
     std::function<int(const std::vector<int32_t>& items)> begin;                                          // session whose slot u holds utterance items[u]
     std::function<int(const std::vector<int32_t>& slots, const std::vector<int32_t>& items)> refill;      // slots[i] takes utterance items[i]
 };
@@ -2555,8 +2560,8 @@ int run_continuous(t3mi_model* m, ContinuousJob& job, int32_t* out, int32_t cap,
     const int extra = m->variant == T3MI_VARIANT_TURBO ? 1 : 0;
     if (m->paged_size > 0 && m->paged_pages > 0) {
         // Every utterance has to fit an empty pool; and no more slots than it serves from the start (an utterance holds the pages of its
-        // prompt and its own limit)
-        const auto pages = [&](int i) { return (long long)job.rows * ((job.s0[i] + job.mx[i] + extra + m->paged_size - 1) / m->paged_size); };
+        // prompt and its own limit, as the session counts them: continuous_setup has set max_cache_len)
+        const auto pages = [&](int i) { return (long long)job.rows * pages_of(m->paged_size, job.cache_len, job.s0[i], std::min(job.mx[i], m->max_pos - 1) + extra); };
         for (int i = 0; i < job.n_utt; ++i)
             if (pages(i) > m->paged_pages)
                 return fail(T3MI_ERR_ARG, "t3mi_generate_continuous: utterance " + std::to_string(i) + " needs " + std::to_string(pages(i)) + " pages, the pool has " +
@@ -2691,6 +2696,7 @@ int continuous_setup(t3mi_model* m, int n_utt, const int32_t* s0, const int32_t*
     sp = *p;
     sp.max_new_tokens = top;
     if (sp.max_cache_len <= 0) sp.max_cache_len = need + 2 + extra;   // long enough that the per-row clamp of R/t3.R:996 never binds
+    job.cache_len = sp.max_cache_len;
     return T3MI_OK;
 }
 }  // namespace
