@@ -86,8 +86,12 @@ struct DevBuf {
         release();
         if (n == 0) n = 16;
         hipError_t e = hipMalloc(&p, n);
-        if (e == hipSuccess) bytes = n;
-        else p = nullptr;
+        if (e == hipSuccess) {
+            bytes = n;
+        } else {
+            p = nullptr;
+            (void)hipGetLastError();   // (the caller reports it; the next launch's check is not to find it)
+        }
         return e;
     }
     template <typename T>
@@ -1478,34 +1482,49 @@ constexpr int kRuleTokens = 1048575;   // (process_logits counts a token's occur
 const char* const kRuleTokensText = "logit rules: a session under rules may have at most 1048575 tokens an utterance";
 
 // the rules of slots `utts` change (the stream is idle).  The first rules of a session, and more biases than its buffers hold, change what a
-// step launches: the captured graph is dropped and the next step captures another.
+// step launches: the captured graph is dropped and the next step captures another.  A call that fails leaves every slot its rules.
 int set_slot_rules(t3mi_model* m, Session* s, const std::vector<int>& utts, const LogitRules& r) {
     if (!s->rules && !r.any()) return T3MI_OK;
     if (s->cap > kRuleTokens) return fail(T3MI_ERR_ARG, kRuleTokensText);
-    s->slot_rules.resize(s->n_utt);
-    for (int u : utts) s->slot_rules[u] = r;
-    int rc;
+    std::vector<LogitRules> slots = s->slot_rules;
+    slots.resize(s->n_utt);
+    for (int u : utts) slots[u] = r;
+    int rc = T3MI_OK;
     if (s->rules && (int)r.ids.size() <= s->rule_cap) {
-        for (int u : utts)
-            if ((rc = upload_rules(m, s, u))) return rc;
-        return T3MI_OK;
+        s->slot_rules.swap(slots);
+        for (size_t i = 0; i < utts.size() && !rc; ++i) rc = upload_rules(m, s, utts[i]);
+        if (rc) s->slot_rules.swap(slots);
+        return rc;
+    }
+    int cap = (int)((std::max<size_t>(r.ids.size(), 1) + 63) / 64 * 64);
+    const size_t U = s->n_utt;
+    DevBuf ids, vals, allowed, fre, pre, out;
+    HIPCHK(ids.alloc(U * cap * 4));
+    HIPCHK(vals.alloc(U * cap * 4));
+    HIPCHK(allowed.alloc(U * ((m->V + 31) / 32) * 4));
+    HIPCHK(fre.alloc(U * 4));
+    HIPCHK(pre.alloc(U * 4));
+    HIPCHK(out.alloc(U * (size_t)m->V * 4));
+    const auto change = [&]() {                 // (and back)
+        const std::pair<DevBuf*, DevBuf*> each[] = {{&ids, &s->lr_ids}, {&vals, &s->lr_vals}, {&allowed, &s->lr_allowed}, {&fre, &s->lr_fre}, {&pre, &s->lr_pre}, {&out, &s->lr_out}};
+        for (const auto& b : each) {
+            std::swap(b.first->p, b.second->p);
+            std::swap(b.first->bytes, b.second->bytes);
+        }
+        std::swap(cap, s->rule_cap);
+        s->slot_rules.swap(slots);
+    };
+    change();
+    for (int u = 0; u < s->n_utt && !rc; ++u) rc = upload_rules(m, s, u);
+    if (rc) {
+        change();
+        return rc;
     }
     if (s->gexec) (void)hipGraphExecDestroy(s->gexec);
     if (s->graph) (void)hipGraphDestroy(s->graph);
     s->gexec = nullptr;
     s->graph = nullptr;
     s->graph_tried = false;
-    s->rules = false;
-    s->rule_cap = (int)((std::max<size_t>(r.ids.size(), 1) + 63) / 64 * 64);
-    const size_t U = s->n_utt, cap = s->rule_cap;
-    HIPCHK(s->lr_ids.alloc(U * cap * 4));
-    HIPCHK(s->lr_vals.alloc(U * cap * 4));
-    HIPCHK(s->lr_allowed.alloc(U * ((m->V + 31) / 32) * 4));
-    HIPCHK(s->lr_fre.alloc(U * 4));
-    HIPCHK(s->lr_pre.alloc(U * 4));
-    HIPCHK(s->lr_out.alloc(U * (size_t)m->V * 4));
-    for (int u = 0; u < s->n_utt; ++u)
-        if ((rc = upload_rules(m, s, u))) return rc;
     s->rules = true;
     return T3MI_OK;
 }
@@ -2454,9 +2473,9 @@ int t3mi_session_refill(t3mi_model* m, int n, const int32_t* utts, const float* 
     hipStream_t st = m->stream;
     HIPCHK(hipStreamSynchronize(st));   // the steps enqueued so far are over: the slots' tokens were the caller's to read before this call
     if ((s->rules || m->rules.any()) && s->cap > kRuleTokens) return fail(T3MI_ERR_ARG, kRuleTokensText);   // (before anything is given up)
+    std::vector<int32_t> over(s->n_utt);
     if (s->paged) {
         // the pages of the slots that are refilled, and of every other slot whose utterance has ended, go back to the pool first
-        std::vector<int32_t> over(s->n_utt);
         HIPCHK(hipMemcpy(over.data(), s->done.p, (size_t)s->n_utt * 4, hipMemcpyDeviceToHost));
         size_t want = 0, have = s->free_pages.size();
         for (int u = 0; u < s->n_utt; ++u)
@@ -2465,13 +2484,15 @@ int t3mi_session_refill(t3mi_model* m, int n, const int32_t* utts, const float* 
         if (want > have)
             return fail(T3MI_ERR_STATE, "t3mi_session_refill: " + std::to_string(want) + " pages are needed, " + std::to_string(have) + " of " +
                                             std::to_string(s->n_pages) + " are free");
+    }
+    if (s->rules || m->rules.any()) {   // a slot's rules are its utterance's: the new one starts with the model's
+        if ((rc = set_slot_rules(m, s, std::vector<int>(utts, utts + n), m->rules))) return rc;
+    }
+    if (s->paged) {
         for (int u = 0; u < s->n_utt; ++u)
             if (taken[u] || over[u]) release_pages(s, u);
         for (int i = 0; i < n; ++i) take_pages(s, utts[i], pages_of(s, s0[i], mn[i]));
         HIPCHK(hipMemcpy(s->table.p, s->table_h.data(), s->table_h.size() * 4, hipMemcpyHostToDevice));
-    }
-    if (s->rules || m->rules.any()) {   // a slot's rules are its utterance's: the new one starts with the model's
-        if ((rc = set_slot_rules(m, s, std::vector<int>(utts, utts + n), m->rules))) return rc;
     }
     // prompts to the device
     DevBuf stage;

@@ -1,0 +1,82 @@
+"""What sessions do on the host -- pages, rules, allocations, refusals -- on a stand-in for the HIP runtime, without a GPU."""
+from tests.host_runtime import run
+
+# a step's launches go out one by one, and the arguments of the last logits-rules launch can be read: "device" memory is the process's own
+RULES = """
+import os
+os.environ["T3MI_GRAPH"] = "0"
+
+class LogitsArgs(C.Structure):   # t3k::LogitsArgs
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "uncond", "out")] + [(n, C.c_int64) for n in ("lr", "ur", "outr")] + \\
+               [(n, C.c_int) for n in ("bf16", "rows", "vocab")] + [("cfg", C.c_float), ("tokens", C.c_void_p), ("n_tokens", C.c_void_p), ("tr", C.c_int64), ("cap", C.c_int)] + \\
+               [(n, C.c_void_p) for n in ("repetition", "frequency", "presence")] + [(n, C.c_float) for n in ("rep", "fre", "pre")] + \\
+               [("ids", C.c_void_p), ("values", C.c_void_p), ("br", C.c_int64), ("bvr", C.c_int64), ("n_bias", C.c_int), ("allowed", C.c_void_p), ("ar", C.c_int64)]
+
+def step(s):
+    # the biases, penalties and numbers of allowed tokens of every slot in the next step; None: no rules
+    rt.hostrt_forget()
+    s.decode(1)
+    if not rt.hostrt_launches(b"process_logits"):
+        return None
+    a = LogitsArgs()
+    assert rt.hostrt_last(b"process_logits", C.byref(a), C.c_size_t(C.sizeof(a)))
+    got = []
+    for u in range(a.rows):
+        ids = np.ctypeslib.as_array((C.c_int32 * a.n_bias).from_address(a.ids + u * a.br * 4))
+        vals = np.ctypeslib.as_array((C.c_float * a.n_bias).from_address(a.values + u * a.bvr * 4))
+        words = np.ctypeslib.as_array((C.c_uint32 * ((a.vocab + 31) // 32)).from_address(a.allowed + u * a.ar * 4))
+        got.append(({int(i): float(v) for i, v in zip(ids, vals) if i >= 0}, C.c_float.from_address(a.frequency + 4 * u).value,
+                    int(np.unpackbits(words.view(np.uint8), bitorder="little")[:a.vocab].sum())))
+    return got
+"""
+
+
+def test_rules_that_find_no_memory_leave_the_old_ones():
+    """Each allocation of a growing rule set fails in turn: the error comes back, every slot keeps its rules, and nothing is lost or kept."""
+    run(RULES + """
+m = model()
+with cb.Session(m, [prompt(9), prompt(5)], max_new_tokens=20, top_p=0.0) as s:
+    assert step(s) is None
+    wide = {t: 0.5 for t in range(100)}
+    for first in (True, False):
+        held, failed = rt.hostrt_held(), 0
+        before = step(s)
+        for k in range(20):
+            rt.hostrt_fail_malloc(k)
+            try:
+                s.logit_rules(1, bias={7: 2.0} if first else wide, frequency_penalty=0.25)
+                break
+            except _lib.T3miError as e:
+                assert "memory" in str(e)
+                failed += 1
+            rt.hostrt_fail_malloc(-1)
+            assert rt.hostrt_held() == held and step(s) == before, (first, k, step(s), before)
+        rt.hostrt_fail_malloc(-1)
+        assert failed >= 5
+        s.logit_rules(0, bias={3: 1.0}, allowed=[1, 2, 3])
+    assert step(s) == [({3: 1.0}, 0.0, 3), (wide, 0.25, m.vocab)]
+m.close()
+""")
+
+
+def test_a_refill_that_finds_no_memory_for_rules_changes_nothing():
+    run(RULES + """
+m = model()
+m.set_paged_kv(8, 14)
+with cb.Session(m, [prompt(9), prompt(5)], max_new_tokens=16, top_p=0.0) as s:
+    m.set_logit_rules(bias={t: 0.5 for t in range(70)})
+    pages, held = s.pages(), rt.hostrt_held()
+    assert pages == (14, 14 - 2 * 4 - 2 * 3)
+    for k in range(6):
+        rt.hostrt_fail_malloc(k)
+        try:
+            s.refill([0], [prompt(3)], max_new_tokens=[4])
+            raise SystemExit("no error")
+        except _lib.T3miError as e:
+            assert "memory" in str(e)
+        rt.hostrt_fail_malloc(-1)
+        assert s.pages() == pages and rt.hostrt_held() == held and step(s) is None, (k, s.pages(), pages)
+    s.refill([0], [prompt(3)], max_new_tokens=[4])
+    assert s.pages() == (14, 6) and [len(r[0]) for r in step(s)] == [70, 0]
+m.close()
+""")
