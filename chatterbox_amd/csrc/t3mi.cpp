@@ -1701,7 +1701,7 @@ int t3mi_session_end(t3mi_model* m) {
     return T3MI_OK;
 }
 
-int t3mi_session_begin(t3mi_model* m, int n_utt, int rpu, const float* const* embeds, const int32_t* s0,
+static int session_begin(t3mi_model* m, int n_utt, int rpu, const float* const* embeds, const int32_t* s0,
                        const t3mi_params* p, int embeds_on_device) {
     if (!m || !embeds || !s0 || !p) return fail(T3MI_ERR_ARG, "t3mi_session_begin: null argument");
     if (n_utt <= 0) return fail(T3MI_ERR_ARG, "t3mi_session_begin: n_utt must be positive");
@@ -1938,6 +1938,11 @@ int t3mi_session_begin(t3mi_model* m, int n_utt, int rpu, const float* const* em
     }
     m->sess = std::move(s);
     return T3MI_OK;
+}
+
+int t3mi_session_begin(t3mi_model* m, int n_utt, int rpu, const float* const* embeds, const int32_t* s0,
+                       const t3mi_params* p, int embeds_on_device) {
+    return guarded([&] { return session_begin(m, n_utt, rpu, embeds, s0, p, embeds_on_device); });
 }
 
 int t3mi_set_paged_kv(t3mi_model* m, int page_size, int n_pages) {
@@ -2424,7 +2429,7 @@ int t3mi_prepare_input_embeds_static(t3mi_model* m, const t3mi_cond* cond, const
     return T3MI_OK;
 }
 
-int t3mi_session_begin_tokens(t3mi_model* m, int n_utt, const t3mi_cond* conds, const int32_t* const* text_tokens,
+static int session_begin_tokens(t3mi_model* m, int n_utt, const t3mi_cond* conds, const int32_t* const* text_tokens,
                               const int32_t* n_text, const t3mi_params* p) {
     if (!p) return fail(T3MI_ERR_ARG, "t3mi_session_begin_tokens: null params");
     std::vector<const float*> ptrs;
@@ -2435,11 +2440,16 @@ int t3mi_session_begin_tokens(t3mi_model* m, int n_utt, const t3mi_cond* conds, 
     return t3mi_session_begin(m, n_utt, rpu, ptrs.data(), s0.data(), p, 1);
 }
 
+int t3mi_session_begin_tokens(t3mi_model* m, int n_utt, const t3mi_cond* conds, const int32_t* const* text_tokens,
+                              const int32_t* n_text, const t3mi_params* p) {
+    return guarded([&] { return session_begin_tokens(m, n_utt, conds, text_tokens, n_text, p); });
+}
+
 // Continuous batching: slots of the running session whose utterance has ended (or any slot) take new utterances while the others keep
 // their state.  Their prompts are prefilled together (the same kernels as t3mi_session_begin), their cache rows are simply
 // overwritten from position 0 (attention never reads a slot beyond the row's position), the per-slot state restarts, and the first
 // logits of ALL rows are re-evaluated from the resident hidden states (bit-identical for the untouched rows).
-int t3mi_session_refill(t3mi_model* m, int n, const int32_t* utts, const float* const* embeds, const int32_t* s0,
+static int session_refill(t3mi_model* m, int n, const int32_t* utts, const float* const* embeds, const int32_t* s0,
                         const int32_t* max_new_tokens, const int64_t* utterance_ids, int embeds_on_device) {
     int rc = need_session(m);
     if (rc) return rc;
@@ -2551,7 +2561,12 @@ int t3mi_session_refill(t3mi_model* m, int n, const int32_t* utts, const float* 
     return T3MI_OK;
 }
 
-int t3mi_session_refill_tokens(t3mi_model* m, int n, const int32_t* utts, const t3mi_cond* conds, const int32_t* const* text_tokens,
+int t3mi_session_refill(t3mi_model* m, int n, const int32_t* utts, const float* const* embeds, const int32_t* s0,
+                        const int32_t* max_new_tokens, const int64_t* utterance_ids, int embeds_on_device) {
+    return guarded([&] { return session_refill(m, n, utts, embeds, s0, max_new_tokens, utterance_ids, embeds_on_device); });
+}
+
+static int session_refill_tokens(t3mi_model* m, int n, const int32_t* utts, const t3mi_cond* conds, const int32_t* const* text_tokens,
                                const int32_t* n_text, const int32_t* max_new_tokens, const int64_t* utterance_ids) {
     int rc = need_session(m);
     if (rc) return rc;
@@ -2563,6 +2578,11 @@ int t3mi_session_refill_tokens(t3mi_model* m, int n, const int32_t* utts, const 
     if (rc) return rc;
     if (rpu != s->rpu) return fail(T3MI_ERR_ARG, "t3mi_session_refill_tokens: the prompt has another number of rows than the session's utterances");
     return t3mi_session_refill(m, n, utts, ptrs.data(), s0.data(), max_new_tokens, utterance_ids, 1);
+}
+
+int t3mi_session_refill_tokens(t3mi_model* m, int n, const int32_t* utts, const t3mi_cond* conds, const int32_t* const* text_tokens,
+                               const int32_t* n_text, const int32_t* max_new_tokens, const int64_t* utterance_ids) {
+    return guarded([&] { return session_refill_tokens(m, n, utts, conds, text_tokens, n_text, max_new_tokens, utterance_ids); });
 }
 
 // ---- continuous batching driver: n_utt utterances through `slots` session slots (t3mi_session_refill between polls) ---------------
@@ -2593,11 +2613,23 @@ int run_continuous(t3mi_model* m, ContinuousJob& job, int32_t* out, int32_t cap,
         job.slots = fit;
     }
     std::vector<int32_t> owner(job.order.begin(), job.order.begin() + job.slots);
-    m->begin_limits.resize(job.slots);
-    for (int u = 0; u < job.slots; ++u) m->begin_limits[u] = job.mx[owner[u]] + extra;
-    int rc = job.begin(owner);
-    m->begin_limits.clear();
+    struct Limits {                             // (for this begin alone, however it ends)
+        t3mi_model* m;
+        ~Limits() { m->begin_limits.clear(); }
+    };
+    int rc;
+    {
+        const Limits limits{m};
+        m->begin_limits.resize(job.slots);
+        for (int u = 0; u < job.slots; ++u) m->begin_limits[u] = job.mx[owner[u]] + extra;
+        rc = job.begin(owner);
+    }
     if (rc) return rc;
+    struct End {                                // (and the session for this job)
+        t3mi_model* m;
+        ~End() { t3mi_session_end(m); }
+    };
+    const End end{m};
     Session* s = m->sess.get();
     {   // t3mi_session_begin numbered the slots first_utterance_id + slot and gave all of them the session's limit: each slot gets
         // its utterance's global index (random stream) and own limit, as t3mi_session_refill sets them
@@ -2722,7 +2754,7 @@ int continuous_setup(t3mi_model* m, int n_utt, const int32_t* s0, const int32_t*
 }
 }  // namespace
 
-int t3mi_generate_continuous(t3mi_model* m, int n_utt, int rows_per_utt, const float* const* embeds, const int32_t* s0,
+static int generate_continuous(t3mi_model* m, int n_utt, int rows_per_utt, const float* const* embeds, const int32_t* s0,
                              const int32_t* max_new_each, int slots, int poll_steps, int flags, const t3mi_params* p, int32_t* out,
                              int32_t cap, int32_t* n_out, int32_t* stats) {
     if (!embeds || !s0 || !out || !n_out) return fail(T3MI_ERR_ARG, "t3mi_generate_continuous: null argument");
@@ -2750,7 +2782,13 @@ int t3mi_generate_continuous(t3mi_model* m, int n_utt, int rows_per_utt, const f
     return run_continuous(m, job, out, cap, n_out, stats);
 }
 
-int t3mi_generate_continuous_tokens(t3mi_model* m, int n_utt, const t3mi_cond* conds, const int32_t* const* text_tokens,
+int t3mi_generate_continuous(t3mi_model* m, int n_utt, int rows_per_utt, const float* const* embeds, const int32_t* s0,
+                             const int32_t* max_new_each, int slots, int poll_steps, int flags, const t3mi_params* p, int32_t* out,
+                             int32_t cap, int32_t* n_out, int32_t* stats) {
+    return guarded([&] { return generate_continuous(m, n_utt, rows_per_utt, embeds, s0, max_new_each, slots, poll_steps, flags, p, out, cap, n_out, stats); });
+}
+
+static int generate_continuous_tokens(t3mi_model* m, int n_utt, const t3mi_cond* conds, const int32_t* const* text_tokens,
                                     const int32_t* n_text, const int32_t* max_new_each, int slots, int poll_steps, int flags,
                                     const t3mi_params* p, int32_t* out, int32_t cap, int32_t* n_out, int32_t* stats) {
     if (!m || !p || !conds || !text_tokens || !n_text || !out || !n_out || n_utt <= 0)
@@ -2788,6 +2826,12 @@ int t3mi_generate_continuous_tokens(t3mi_model* m, int n_utt, const t3mi_cond* c
         return t3mi_session_refill_tokens(m, (int)it.size(), sl.data(), c.data(), t.data(), nt.data(), mn.data(), id.data());
     };
     return run_continuous(m, job, out, cap, n_out, stats);
+}
+
+int t3mi_generate_continuous_tokens(t3mi_model* m, int n_utt, const t3mi_cond* conds, const int32_t* const* text_tokens,
+                                    const int32_t* n_text, const int32_t* max_new_each, int slots, int poll_steps, int flags,
+                                    const t3mi_params* p, int32_t* out, int32_t cap, int32_t* n_out, int32_t* stats) {
+    return guarded([&] { return generate_continuous_tokens(m, n_utt, conds, text_tokens, n_text, max_new_each, slots, poll_steps, flags, p, out, cap, n_out, stats); });
 }
 
 int t3mi_generate_batch_tokens(t3mi_model* m, int n_utt, const t3mi_cond* conds, const int32_t* const* text_tokens,

@@ -1,5 +1,5 @@
 // A stand-in for the HIP runtime on a machine without a GPU, for tests of what the library does on the host: device memory is host memory, copies copy,
-// kernels do nothing.  Allocations (hipMalloc and operator new) can be told to fail; launches are counted by name, with their first argument kept.
+// kernels do nothing.  Allocations (hipMalloc and operator new) and copies can be told to fail; launches are counted by name, with their first argument kept.
 #include <cstdlib>
 #include <cstring>
 #include <map>
@@ -17,7 +17,7 @@ std::vector<size_t>& sizes() { static std::vector<size_t> v; return v; }
 Dim3 grid, block;
 size_t shared;
 void* stream;
-long fail_malloc = -1, fail_new = -1;   // how many succeed before one fails; -1: all do
+long fail_malloc = -1, fail_new = -1, fail_copy = -1;   // how many succeed before one fails; -1: all do
 int capturing = 0, last_error = 0;
 bool due(long& n) { return n >= 0 && n-- == 0; }
 int handle;
@@ -37,6 +37,7 @@ extern "C" {
 // what the tests call
 void hostrt_fail_malloc(long after) { fail_malloc = after; }
 void hostrt_fail_new(long after) { fail_new = after; }
+void hostrt_fail_copy(long after) { fail_copy = after; }
 void hostrt_forget() { launches().clear(); sizes().clear(); }
 long hostrt_launches(const char* part) {
     long n = 0;
@@ -91,8 +92,12 @@ int hipFree(void* p) {
     std::free(p);
     return 0;
 }
-int hipMemcpy(void* d, const void* s, size_t n, int) { std::memmove(d, s, n); return 0; }
-int hipMemcpyAsync(void* d, const void* s, size_t n, int, void*) { std::memmove(d, s, n); return 0; }
+int hipMemcpy(void* d, const void* s, size_t n, int) {
+    if (due(fail_copy)) return last_error = 1;
+    std::memmove(d, s, n);
+    return 0;
+}
+int hipMemcpyAsync(void* d, const void* s, size_t n, int kind, void*) { return hipMemcpy(d, s, n, kind); }
 int hipMemset(void* d, int v, size_t n) { std::memset(d, v, n); return 0; }
 int hipMemsetAsync(void* d, int v, size_t n, void*) { std::memset(d, v, n); return 0; }
 int hipMemsetD32Async(void* d, int v, size_t n, void*) { for (size_t i = 0; i < n; ++i) static_cast<int*>(d)[i] = v; return 0; }

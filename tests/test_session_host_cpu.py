@@ -80,3 +80,58 @@ with cb.Session(m, [prompt(9), prompt(5)], max_new_tokens=16, top_p=0.0) as s:
     assert s.pages() == (14, 6) and [len(r[0]) for r in step(s)] == [70, 0]
 m.close()
 """)
+
+
+def test_no_exception_leaves_the_session_calls():
+    """Every allocation of a begin, a refill and a continuous job fails in turn with std::bad_alloc: an error comes back, and what follows is a session like any
+    other (its own pages, no limits of the job that failed)."""
+    run("""
+m = model()
+m.set_paged_kv(8, 60)
+kw = dict(max_new_tokens=40, top_p=0.0)
+embs = [prompt(9), prompt(5), prompt(7)]
+
+def fails(call, limit=4000):
+    n = 0
+    for k in range(limit):
+        rt.hostrt_fail_new(C.c_long(k))
+        try:
+            call()
+        except _lib.T3miError as e:
+            rt.hostrt_fail_new(C.c_long(-1))
+            if "memory" not in str(e):
+                return n                        # (the job's own end)
+            n += 1
+            continue
+        rt.hostrt_fail_new(C.c_long(-1))
+        return n
+    raise SystemExit("no end")
+
+def begin():
+    cb.Session(m, embs, **kw).__enter__().__exit__(None, None, None)
+
+def plain():
+    with cb.Session(m, embs, **kw) as s:
+        assert s.pages() == (42, 42 - 2 * (7 + 6 + 6)), s.pages()   # (never more than the worst case)
+
+assert fails(begin) > 10
+plain()
+s = cb.Session(m, embs, **kw)
+assert fails(lambda: s.refill([1], [prompt(6)], max_new_tokens=[5])) > 5
+total, free = s.pages()
+assert (total, free) == (42, 42 - 2 * (7 + 2 + 6))
+s.close() if hasattr(s, "close") else s.__exit__(None, None, None)
+
+def job():
+    rt.hostrt_fail_copy(C.c_long(200))           # (no token is ever drawn here: the job ends with this error)
+    try:
+        cb.t3_inference_continuous(m, embs + [prompt(4)], slots=3, poll_steps=3, max_new_tokens=[2, 3, 4, 5], top_p=0.0)
+    finally:
+        rt.hostrt_fail_copy(C.c_long(-1))
+        rt.hostrt_fail_new(C.c_long(-1))
+        plain()
+
+assert fails(job) > 10
+plain()
+m.close()
+""")
