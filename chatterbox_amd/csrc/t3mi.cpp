@@ -1016,6 +1016,9 @@ t3k::PagedAttnArgs paged_attn(const t3mi_model* m, const Session* s, int layer, 
     return a;
 }
 
+// bytes of the projections that M rows of a session on pages need between the qkv product and the append: none where the product writes into the pages
+size_t qkv_bytes(const t3mi_model* m, size_t M) { return t3k::gemm_takes_pages((int)M, m->d, m->wdtype) ? 0 : M * 3 * m->d * 4; }
+
 int run_layers_gemm(t3mi_model* m, Session* s, GemmCtx& c, StepTimer* tm) {
     const int d = m->d, F = m->F, H = m->H;
     const int abf = (m->wdtype == T3MI_W_BF16 && !c.act_f32) ? 1 : 0;
@@ -1335,13 +1338,14 @@ int prefill_rows(t3mi_model* m, Session* s, const std::vector<int>& rows_list, c
     hipStream_t st = m->stream;
     const int nr = (int)rows_list.size();
     std::vector<std::pair<int, int>> groups;   // [begin, end) into rows_list
-    size_t max_items = 0;
+    size_t max_items = 0, max_qkv = 0;
     for (int i0 = 0; i0 < nr;) {
         size_t n = 0;
         int i1 = i0;
         while (i1 < nr && (i1 == i0 || n + (size_t)s->s0[rows_list[i1] / rpu] <= kPrefillItems)) n += (size_t)s->s0[rows_list[i1++] / rpu];
         groups.emplace_back(i0, i1);
         max_items = std::max(max_items, n);
+        if (s->paged) max_qkv = std::max(max_qkv, qkv_bytes(m, n));
         i0 = i1;
     }
     // scratch of the prefill: kept in the session and only ever grown (t3mi_session_refill prefills again and again; hipFree
@@ -1359,7 +1363,7 @@ int prefill_rows(t3mi_model* m, Session* s, const std::vector<int>& rows_list, c
     HIPCHK(grow(dpos, max_items * 4));
     HIPCHK(grow(drow, max_items * 4));
     HIPCHK(grow(dlast, (size_t)nr * sizeof(void*)));
-    if (s->paged) HIPCHK(grow(s->pfs[9], max_items * 3 * d * 4));
+    if (max_qkv > 0) HIPCHK(grow(s->pfs[9], max_qkv));
     std::vector<const float*> isrc, last;
     std::vector<int32_t> ipos, irow;
     int rc;
@@ -1388,7 +1392,8 @@ int prefill_rows(t3mi_model* m, Session* s, const std::vector<int>& rows_list, c
         c.act_f32 = pf_act_f32;
         if (s->paged) {
             c.prompt = true;
-            HIPCHK(grow(s->pfs[10], t3k::paged_attention_workspace(paged_attn(m, s, 0, c.M, as == 2 ? 1 : 0, c.prompt))));
+            const size_t ws = t3k::paged_attention_workspace(paged_attn(m, s, 0, c.M, as == 2 ? 1 : 0, c.prompt));
+            if (ws > 0) HIPCHK(grow(s->pfs[10], ws));
             c.qkv = s->pfs[9].as<float>();
             c.ws = s->pfs[10].p;
         }
@@ -1787,7 +1792,7 @@ static int session_begin(t3mi_model* m, int n_utt, int rpu, const float* const* 
         kv = (size_t)m->n_layers * s->n_pages * m->H * s->page_size * 64 * (s->kv_bf16 ? 2 : 4);
         HIPCHK(s->table.alloc(most * 4));
         HIPCHK(hipMemcpy(s->table.p, s->table_h.data(), most * 4, hipMemcpyHostToDevice));
-        HIPCHK(s->qkv.alloc(rows * 3 * d * 4));
+        if (const size_t bytes = qkv_bytes(m, rows); bytes > 0) HIPCHK(s->qkv.alloc(bytes));
         HIPCHK(s->pws.alloc(t3k::paged_attention_workspace(paged_attn(m, s.get(), 0, (int)rows, m->wdtype == T3MI_W_BF16 ? 1 : 0, false))));
     }
     HIPCHK(s->kc.alloc(kv));

@@ -135,3 +135,21 @@ assert fails(job) > 10
 plain()
 m.close()
 """)
+
+
+def test_projections_take_memory_only_where_they_are_read():
+    """The qkv product writes into the pages itself in bf16 and from 64 fp32 rows on: no buffer for its projections then (402 MB for the largest prefill of
+    the full-size model), and one for the few rows that need it."""
+    run("""
+d = synth.TINY.hidden_size
+for dtype, lens, decode_rows, prefill_rows in (("bf16", [40] * 5, 0, 0), ("bf16", [5], 0, 0), ("f32", [9, 20], 4, 58), ("f32", [200] * 2, 4, 0), ("f32", [200] * 40, 0, 0)):
+    m = model(dtype=dtype)
+    m.set_paged_kv(16)
+    rt.hostrt_forget()
+    with cb.Session(m, [prompt(n) for n in lens], max_new_tokens=11, top_p=0.0) as s:
+        s.decode(1)
+        got = sizes()
+        for rows, needed in ((2 * len(lens), decode_rows), (2 * sum(lens), prefill_rows)):
+            assert got.count(rows * 3 * d * 4) == (1 if needed else 0), (dtype, lens, rows, got)
+    m.close()
+""")
