@@ -116,7 +116,8 @@ int take_attention(const char* where, const t3mi_paged_cache* cache, const t3mi_
     o.max_length = (int)(a->max_length > 0 && a->max_length < most ? a->max_length : most);
     o.length_add = a->length_add;
     if (a->prompt < -1 || a->prompt > 1) return bad(where, "prompt must be -1, 0 or 1");
-    o.prompt = a->prompt > 0 || (a->prompt == 0 && a->seq && (int64_t)a->rows >= 4LL * cache->n_seqs);
+    // (of one sequence any rows are neighbours)
+    o.prompt = a->prompt > 0 ? 1 : (a->prompt == 0 && a->seq && (int64_t)a->rows >= 4LL * cache->n_seqs ? (cache->n_seqs == 1 ? 1 : 2) : 0);
     return T3MI_OK;
 }
 

@@ -46,7 +46,7 @@ struct PagedAttnArgs {
     const int* seq = nullptr;     // [rows] block-table row, or nullptr: identity
     float scale = 1.f;
     int rows = 0, q_heads = 0, q_bf16 = 0, out_bf16 = 0, max_length = 0, length_add = 0;
-    int prompt = 0;               // neighbouring rows mostly share a sequence (plan_paged_attention clears it where that is of no use)
+    int prompt = 0;               // 1: neighbouring rows mostly share a sequence; 2: in the mean four rows or more do, in any order (plan_paged_attention clears it where that is of no use)
     // filled by plan_paged_attention
     int n_split = 1;              // blocks a row's keys are shared by at most
     int tile_shift = 5;           // keys of a tile: 32, or 16 (fp32 cache)

@@ -1154,7 +1154,15 @@ void plan_paged_attention(PagedAttnArgs& a) {
     a.tile_shift = a.c.bf16 ? 5 : 4;
     const long long tiles = ((long long)a.max_length + (1 << a.tile_shift) - 1) >> a.tile_shift;
     const long long pairs = (long long)a.rows * a.c.kv_heads * ((group + 15) / 16);
-    a.prompt = a.prompt && group <= 8;               // (two rows at least to a tile)
+    // Rows that share their keys read them once, but no block of theirs is split: it goes through the whole length with its few waves.  A tile takes a block
+    // of theirs 0.16 to 0.31 us, a (row, key head) pair on its own 1.2 (heads of 64) to 2.6 ns, so sharing pays from some 190 pairs on at any length (32 / 8
+    // heads of 128, bf16, 131071 keys of one sequence: 4 rows 1527 us shared, 369 row by row; 16 rows 1312, 1210; 32 rows 1283, 2520; 8 / 1 heads 4 rows
+    // 1096, 48; 256 rows 1110, 1151; 16 fp32 heads of 64 8 rows 1851, 1414; 16 rows 1853, 2653).  Where the rows' order is not known, a block may hold as
+    // many sequences as rows and take them in turn: sharing then gains so many times in one order what it loses in the other only from sqrt(turns) times the
+    // pairs on.  (4 sequences of 131071 keys, 32 / 8 heads, rows sequence by sequence, in turn, and either row by row: 16 rows 1576, 7522, 1350 us; 64 rows
+    // 1371, 7505, 4900; 128 rows 1340, 7517, 9700.)
+    const long long turns = a.prompt == 2 ? std::min(16 / std::min(group, 16), a.c.n_seqs) : 1;
+    a.prompt = a.prompt && group <= 8 && pairs * pairs >= 192LL * 192LL * turns;   // (group: two rows at least to a tile)
     if (a.prompt) {
         const long long blocks = prompt_blocks(a);
         a.head_waves = 1;

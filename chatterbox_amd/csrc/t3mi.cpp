@@ -980,7 +980,7 @@ struct GemmCtx {
     const float* pend_bias = nullptr;
     float* qkv = nullptr;      // paged cache: [M][3 d] projections before the append
     void* ws = nullptr;        // and the attention's workspace
-    bool prompt = false;       // the rows are positions of prompts, one after the other
+    int prompt = 0;            // > 0: the rows are positions of prompts, one after the other, the longest of this length
     // bf16 weight storage with fp32 activation rows (exact fp32 products, the arithmetic of the GEMV path): the prefill
     // of sessions that decode with <= 4 rows
     bool act_f32 = false;
@@ -1003,15 +1003,16 @@ t3k::PagedCache paged_layer(const t3mi_model* m, const Session* s, int layer) {
     c.kv_heads = m->H; c.head_dim = 64; c.bf16 = s->kv_bf16 ? 1 : 0;
     return c;
 }
-// attention of M items (query rows c.q, positions c.posmap) over a layer's pool, as launched and as planned for the workspace
-t3k::PagedAttnArgs paged_attn(const t3mi_model* m, const Session* s, int layer, int M, int out_bf16, bool prompt) {
+// attention of M items (query rows c.q, positions c.posmap) over a layer's pool, as launched and as planned for the workspace; prompt: the rows
+// are positions of prompts of this length at most (0: one new token of every row)
+t3k::PagedAttnArgs paged_attn(const t3mi_model* m, const Session* s, int layer, int M, int out_bf16, int prompt) {
     t3k::PagedAttnArgs a;
     a.c = paged_layer(m, s, layer);
     a.qr = a.outr = m->d;
     a.qh = a.outh = 64;
     a.scale = 0.125f;
     a.rows = M; a.q_heads = m->H; a.q_bf16 = 0; a.out_bf16 = out_bf16;
-    a.max_length = s->max_len; a.length_add = 1; a.prompt = prompt ? 1 : 0;
+    a.max_length = prompt > 0 ? prompt : s->max_len; a.length_add = 1; a.prompt = prompt > 0 ? 1 : 0;
     t3k::plan_paged_attention(a);
     return a;
 }
@@ -1391,7 +1392,7 @@ int prefill_rows(t3mi_model* m, Session* s, const std::vector<int>& rows_list, c
         c.posmap = dpos.as<int>(); c.rowmap = drow.as<int>();
         c.act_f32 = pf_act_f32;
         if (s->paged) {
-            c.prompt = true;
+            c.prompt = 1 + *std::max_element(ipos.begin(), ipos.end());
             const size_t ws = t3k::paged_attention_workspace(paged_attn(m, s, 0, c.M, as == 2 ? 1 : 0, c.prompt));
             if (ws > 0) HIPCHK(grow(s->pfs[10], ws));
             c.qkv = s->pfs[9].as<float>();
@@ -1793,7 +1794,7 @@ static int session_begin(t3mi_model* m, int n_utt, int rpu, const float* const* 
         HIPCHK(s->table.alloc(most * 4));
         HIPCHK(hipMemcpy(s->table.p, s->table_h.data(), most * 4, hipMemcpyHostToDevice));
         if (const size_t bytes = qkv_bytes(m, rows); bytes > 0) HIPCHK(s->qkv.alloc(bytes));
-        HIPCHK(s->pws.alloc(t3k::paged_attention_workspace(paged_attn(m, s.get(), 0, (int)rows, m->wdtype == T3MI_W_BF16 ? 1 : 0, false))));
+        HIPCHK(s->pws.alloc(t3k::paged_attention_workspace(paged_attn(m, s.get(), 0, (int)rows, m->wdtype == T3MI_W_BF16 ? 1 : 0, 0))));
     }
     HIPCHK(s->kc.alloc(kv));
     HIPCHK(s->vc.alloc(kv));

@@ -62,8 +62,9 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, *, seq=None, star
     scale: 1 / sqrt(head_dim) by default.  max_length: about the longest length, where the host knows it (the call is planned by it;
     rows that are longer come out right too).  A row with no key gives zeros; a row of negative length is left as it was in out.
     out: [rows, heads, head_dim], float32 or bfloat16 (new, in out_dtype or q's type, by default).  Many rows of one sequence
-    (a prompt, causal) are rows with the same seq and lengths 1, 2, 3, ...; prompt says that neighbouring rows mostly share a sequence, and
-    then they share the keys they read (None: if there are four rows to a sequence of the table; the results are the same up to rounding)."""
+    (a prompt, causal) are rows with the same seq and lengths 1, 2, 3, ...; prompt says whether neighbouring rows mostly share a sequence: such rows share
+    the keys they read where there are enough of them for that to pay (None: four rows to a sequence of the table, and more of
+    them, since their order is not known; the results are the same up to rounding)."""
     return (_ops or _bind()).attention(q, k_pages, v_pages, block_table, lengths, seq, starts, scale, max_length or 0, out, out_dtype,
                                        0 if prompt is None else 1 if prompt else -1)
 

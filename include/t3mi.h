@@ -447,7 +447,8 @@ typedef struct t3mi_attention_args {
     int32_t q_dtype, out_dtype;
     int32_t length_add;          /* 0 or 1                                                   */
     int32_t max_length;          /* about the longest length, for planning alone (0: the table's); longer rows are still right */
-    int32_t prompt;              /* for planning alone: 1 if neighbouring rows mostly belong to one sequence (prompts), -1 if not, 0: if there are 4 rows to a sequence */
+    int32_t prompt;              /* for planning alone: 1 if neighbouring rows mostly belong to one sequence (prompts), -1 if not, 0: unknown.  Rows then share
+                                  * the keys they read where there are enough of them for that to pay (0: more are needed, and 4 to a sequence; their order is not known) */
 } t3mi_attention_args;
 int t3mi_paged_attention_workspace(const t3mi_paged_cache* cache, const t3mi_attention_args* args, size_t* bytes);
 int t3mi_paged_attention(const t3mi_paged_cache* cache, const t3mi_attention_args* args, void* stream);

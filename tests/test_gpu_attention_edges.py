@@ -17,7 +17,8 @@ def t32(x):
 
 
 @pytest.mark.parametrize("q_t", ["f32", "bf16"])
-@pytest.mark.parametrize("prompt,heads,kv_heads,dim,page", [(False, 16, 16, 64, 64), (False, 32, 8, 128, 16), (False, 6, 2, 64, 2), (True, 8, 2, 128, 64), (True, 4, 4, 64, 8)])
+@pytest.mark.parametrize("prompt,heads,kv_heads,dim,page", [(False, 16, 16, 64, 64), (False, 32, 8, 128, 16), (False, 6, 2, 64, 2), (True, 8, 2, 128, 64), (True, 4, 4, 64, 8),
+                                                               (True, 24, 8, 128, 64), (True, 12, 12, 64, 8)])
 def test_weights_under_a_bf16_result_are_not_rounded_to_it(q_t, prompt, heads, kv_heads, dim, page):
     """A bf16 result is off by its own rounding, 2^-8 of itself, and by next to nothing else: a weight held in two bf16 parts, each rounded to the nearest,
     is off by at most 2^-8 2^-8 of itself, a 256th of what one part would be.  Sums of many keys are small against sum p |v|, which one part's error goes with."""
@@ -46,7 +47,8 @@ def ref_row(q, k, v, scale):
 
 @pytest.mark.parametrize("q_t,kv_t,out_t", [("f32", "bf16", "f32"), ("f32", "bf16", "bf16"), ("bf16", "bf16", "f32"), ("bf16", "bf16", "bf16"), ("f32", "f32", "f32")])
 @pytest.mark.parametrize("prompt,heads,kv_heads,dim,page,most", [(False, 4, 2, 64, 64, 0), (False, 6, 2, 128, 8, 0), (False, 4, 2, 64, 1, 0), (False, 8, 2, 128, 64, 20000),
-                                                                 (False, 40, 2, 64, 32, 0), (True, 4, 2, 64, 64, 0), (True, 6, 2, 128, 8, 0), (True, 2, 2, 64, 16, 0)])
+                                                                 (False, 40, 2, 64, 32, 0), (True, 4, 2, 64, 64, 0), (True, 6, 2, 128, 8, 0), (True, 2, 2, 64, 16, 0),
+                                                                 (True, 16, 8, 64, 64, 0), (True, 24, 8, 128, 8, 0), (True, 6, 6, 64, 16, 0), (True, 32, 8, 128, 32, 0)])
 def test_infinities(q_t, kv_t, out_t, prompt, heads, kv_heads, dim, page, most):
     """Queries that bf16 holds exactly against keys and values with infinities in them.  A key of -inf score has no weight, one of +inf makes its rows NaN, an
     infinite value comes out in its element wherever its key is seen (also alone, with weight 1); everything else is as the formula has it, to the
@@ -106,3 +108,26 @@ def test_infinite_queries(q_t, kv_t, out_t, prompt):
     for r, h in ((1, 0), (2, 1), (3, 2), (4, 3)):
         got[r, h] = clean[r, h]
     assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("q_t,kv_t,out_t", [("f32", "f32", "f32"), ("f32", "bf16", "bf16"), ("bf16", "bf16", "bf16")])
+@pytest.mark.parametrize("rows,heads,kv_heads,dim", [(4, 8, 2, 128), (12, 4, 4, 64), (40, 8, 2, 128), (64, 6, 6, 64), (96, 4, 2, 64)])
+def test_rows_of_long_sequences_in_any_order(q_t, kv_t, out_t, rows, heads, kv_heads, dim):
+    """Few and many rows of one and of four long sequences, one sequence after the other and in turn: the same values however they are planned."""
+    lens = [5000, 3001, 4100, 4999]
+    k, v, table, keys, vals = make_cache(lens, 64, kv_heads, dim, kv_t, 23)
+    q = torch.randn(rows, heads, dim, generator=torch.Generator().manual_seed(4)).to(DT[q_t]).cuda()
+    for seqs, order in ((1, "after"), (4, "after"), (4, "turn")):
+        each = rows // seqs
+        at = [(s, lens[s] - each + 1 + i) for s in range(seqs) for i in range(each)]
+        if order == "turn":
+            at = [at[s * each + i] for i in range(each) for s in range(seqs)]
+        some = [r for r in range(rows) if r % 7 == 0 or r == rows - 1]
+        want = [ref_attention(np64(q[r]), keys[s][:n], vals[s][:n], 0, dim ** -0.5) for r, (s, n) in ((r, at[r]) for r in some)]
+        for prompt in (None, True, False):
+            got = np64(cb.paged_attention(q, k, v, table[:seqs], t32([n for _, n in at]), seq=t32([s for s, _ in at]), out_dtype=DT[out_t], prompt=prompt))
+            for r, (ref, mag, err) in zip(some, want):
+                tol = 2 * (2 * err * U + 2.0 ** -21 + at[r][1] * U) * mag
+                if out_t == "bf16":
+                    tol = (tol + 2.0 ** -16 * mag) * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(ref)
+                assert (np.abs(got[r] - ref) <= tol).all(), (seqs, order, prompt, r)
