@@ -67,6 +67,38 @@ template <int N> bool disjoint(const int64_t (&stride)[N], const int64_t (&count
     return true;
 }
 
+// [rows, heads] runs of `inner` elements of `bytes` each
+struct Runs {
+    const void* p;
+    int64_t stride[2], count[2];
+    int64_t inner;
+    int bytes;
+};
+// whether two tensors share no memory: apart as a whole, or woven into each other with the same strides and a distance that keeps them apart
+// (anything else is taken to share)
+bool apart(const Runs& a, const Runs& b) {
+    if (!a.p || !b.p || a.count[0] <= 0 || a.count[1] <= 0 || b.count[0] <= 0 || b.count[1] <= 0) return true;
+    typedef __int128 wide;
+    const auto from = [](const Runs& t) { return (wide)reinterpret_cast<uintptr_t>(t.p); };
+    const auto to = [&](const Runs& t) { return from(t) + ((wide)(t.count[0] - 1) * t.stride[0] + (wide)(t.count[1] - 1) * t.stride[1] + t.inner) * t.bytes; };
+    if (to(a) <= from(b) || to(b) <= from(a)) return true;
+    int64_t stride[2];                               // common to both; 0: neither takes a second step, or has one to take
+    for (int d = 0; d < 2; ++d) {
+        if (a.count[d] > 1 && b.count[d] > 1 && a.stride[d] != b.stride[d]) return false;
+        stride[d] = a.count[d] > 1 ? a.stride[d] : b.count[d] > 1 ? b.stride[d] : 0;
+    }
+    const wide off = from(b) - from(a);
+    if (a.bytes != b.bytes || off % a.bytes) return false;
+    const auto place = [&](int64_t step) { const wide r = off / a.bytes % step; return r < 0 ? r + step : r; };   // of b's first run after one of a's
+    const int big = stride[0] >= stride[1] ? 0 : 1, small = 1 - big;
+    const auto extent = [&](const Runs& t) { return (wide)(t.count[small] - 1) * stride[small] + t.inner; };
+    if (stride[big] > 0 && place(stride[big]) >= extent(a) && place(stride[big]) + extent(b) <= stride[big]) return true;
+    return stride[small] > 0 && stride[big] % stride[small] == 0 && place(stride[small]) >= a.inner && place(stride[small]) + b.inner <= stride[small];
+}
+Runs runs(const void* p, const int64_t (&stride)[2], int64_t rows, int64_t heads, int64_t inner, int dtype) {
+    return {p, {stride[0], stride[1]}, {rows, heads}, inner, dtype == T3MI_W_BF16 ? 2 : 4};
+}
+
 int take_cache(const char* where, const t3mi_paged_cache* c, t3k::PagedCache& o) {
     if (!c) return bad(where, "null cache");
     if (!c->k || !c->v || !c->block_table) return bad(where, "the cache has a null pointer");
@@ -107,6 +139,9 @@ int take_attention(const char* where, const t3mi_paged_cache* cache, const t3mi_
     if (a->q == a->out && (a->q_dtype != a->out_dtype || a->q_stride[0] != a->out_stride[0] || a->q_stride[1] != a->out_stride[1]))
         if (a->rows) return bad(where, "out may be q only with the same strides and type");
     if (!disjoint<2>(a->out_stride, {a->rows, a->q_heads}, cache->head_dim)) return bad(where, "the rows and heads of out must not overlap");
+    if (a->q != a->out && !apart(runs(a->q, a->q_stride, a->rows, a->q_heads, cache->head_dim, a->q_dtype),
+                                 runs(a->out, a->out_stride, a->rows, a->q_heads, cache->head_dim, a->out_dtype)))
+        return bad(where, "out must not share memory with q (but be q)");
     o.q = a->q; o.out = a->out;
     o.qr = a->q_stride[0]; o.qh = a->q_stride[1]; o.outr = a->out_stride[0]; o.outh = a->out_stride[1];
     o.lengths = a->lengths; o.starts = a->starts; o.seq = a->seq;
@@ -151,6 +186,13 @@ int t3mi_paged_append(const t3mi_paged_cache* cache, const t3mi_append_args* a, 
     if (!disjoint<3>(cache->k_stride, {cache->n_pages, cache->page_size, cache->kv_heads}, cache->head_dim) ||
         !disjoint<3>(cache->v_stride, {cache->n_pages, cache->page_size, cache->kv_heads}, cache->head_dim) || cache->k == cache->v)
         return bad(me, "the pages, slots and heads of the cache must not overlap");
+    if (a->q) {
+        const Runs out = runs(a->q_out, a->q_out_stride, a->rows, a->q_heads, cache->head_dim, a->dtype);
+        if ((a->q != a->q_out && !apart(runs(a->q, a->q_stride, a->rows, a->q_heads, cache->head_dim, a->dtype), out)) ||
+            !apart(runs(a->k, a->k_stride, a->rows, cache->kv_heads, cache->head_dim, a->dtype), out) ||
+            !apart(runs(a->v, a->v_stride, a->rows, cache->kv_heads, cache->head_dim, a->dtype), out))
+            return bad(me, "q_out must not share memory with q (but be q), k or v");
+    }
     o.k = a->k; o.v = a->v; o.q = a->q; o.q_out = a->q_out;
     o.kr = a->k_stride[0]; o.kh = a->k_stride[1]; o.vr = a->v_stride[0]; o.vh = a->v_stride[1];
     o.qr = a->q_stride[0]; o.qh = a->q_stride[1]; o.qor = a->q_out_stride[0]; o.qoh = a->q_out_stride[1];
@@ -210,6 +252,10 @@ int t3mi_process_logits(const t3mi_logits_args* a, void* stream) {
         !at4(a->frequency_each) || !at4(a->presence_each))
         return bad(me, "arrays must be aligned to 4 bytes");
     if (a->rows == 0) return T3MI_OK;
+    const Runs out = runs(a->out, {a->out_stride, 0}, a->rows, 1, a->vocab, a->dtype);
+    if ((a->out != a->logits && !apart(runs(a->logits, {a->logits_stride, 0}, a->rows, 1, a->vocab, a->dtype), out)) ||
+        !apart(runs(a->uncond, {a->uncond_stride, 0}, a->rows, 1, a->vocab, a->dtype), out))
+        return bad(me, "out must not share memory with logits (but be logits) or uncond");
     t3k::LogitsArgs o;
     o.logits = a->logits; o.uncond = a->uncond; o.out = a->out;
     o.lr = a->logits_stride; o.ur = a->uncond_stride; o.outr = a->out_stride;

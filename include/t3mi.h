@@ -409,7 +409,7 @@ typedef struct t3mi_paged_cache {
 /* Append: row r's key and value go to position positions[r] of sequence seq[r] (NULL: sequence r).  With cos / sin ([rope_len, >=
  * head_dim / 2] fp32, 4-byte aligned) keys and queries are rotated by their position's angle on the way, element i with element
  * i + head_dim / 2 (apply_rotary_pos_emb, R/llama.R:155-188): (a, b) -> (a cos - b sin, b cos + a sin); the rotated queries go to
- * q_out (may be q itself, with the same strides).  A row whose position is negative, beyond the tables or on no page is skipped: neither
+ * q_out (may be q itself, with the same strides; it shares no memory with q otherwise, nor with k or v).  A row whose position is negative, beyond the tables or on no page is skipped: neither
  * the cache nor its q_out row is written.  No two rows of a call may name the same place, and no two elements of the cache or of q_out may be
  * the same memory. */
 typedef struct t3mi_append_args {
@@ -432,7 +432,7 @@ int t3mi_paged_append(const t3mi_paged_cache* cache, const t3mi_append_args* arg
  * lengths[r] + length_add) of sequence seq[r], head h reading key head h / (q_heads / kv_heads).  Row r of a prompt's queries attends
  * causally when lengths[r] is its position and length_add 1 (such rows share the keys they read, `prompt`).  A row with no key is written as zeros, a row whose length is negative is left as it
  * was (padding of a batch); lengths beyond the block table end there.  Types: q fp32 over an fp32 or bf16 cache, q bf16 over a bf16
- * cache; out fp32 or bf16, and q itself only with q's type and strides. */
+ * cache; out fp32 or bf16, and q itself only with q's type and strides; it shares no memory with q otherwise. */
 typedef struct t3mi_attention_args {
     const void* q;               /* [rows, q_heads, head_dim]; strides (row, head)           */
     void* out;

@@ -4,6 +4,7 @@ import ctypes as C
 import pytest
 
 from chatterbox_amd import _lib
+from tests.host_runtime import run
 from tests.test_ops_cpu import P, attention, cache
 
 
@@ -37,3 +38,84 @@ def test_rows_in_unknown_order_share_keys_where_that_gains_more_than_it_may_lose
     kw = dict(q_heads=4, seq=P, q_stride=(256, 64), out_stride=(256, 64))
     assert split(c, rows=64, prompt=0, **kw) and not split(c, rows=64, prompt=1, **kw) and split(c, rows=64, prompt=-1, **kw)
     assert not split(c, rows=512, prompt=0, **kw)
+
+
+# (everything on a stand-in for the HIP runtime: calls that pass the checks launch nothing there)
+CALLS = """
+P = 1 << 24
+def attend(q, out, qs, os, rows=3, heads=4, qd=0, od=0, dim=64):
+    c = _lib.PagedCache(k=P << 8, v=P << 9, block_table=P << 10, table_stride=4, n_seqs=rows, max_pages=4, n_pages=9, page_size=16, kv_heads=2, head_dim=dim, dtype=qd, device=0)
+    c.k_stride[:] = c.v_stride[:] = (16 * 2 * dim, 2 * dim, dim)
+    a = _lib.AttentionArgs(q=q, out=out, lengths=P << 10, workspace=P << 11, workspace_bytes=1 << 40, scale=0.125, rows=rows, q_heads=heads, q_dtype=qd, out_dtype=od)
+    a.q_stride[:], a.out_stride[:] = qs, os
+    return L.t3mi_paged_attention(C.byref(c), C.byref(a), None)
+
+def append(k, v, q, out, ks, vs, qs, os, rows=3, heads=4):
+    c = _lib.PagedCache(k=P << 8, v=P << 9, block_table=P << 10, table_stride=4, n_seqs=rows, max_pages=4, n_pages=9, page_size=16, kv_heads=2, head_dim=64, dtype=0, device=0)
+    c.k_stride[:] = c.v_stride[:] = (16 * 2 * 64, 2 * 64, 64)
+    a = _lib.AppendArgs(k=k, v=v, q=q, q_out=out, positions=P << 10, rows=rows, q_heads=heads, dtype=0)
+    a.k_stride[:], a.v_stride[:], a.q_stride[:], a.q_out_stride[:] = ks, vs, qs, os
+    return L.t3mi_paged_append(C.byref(c), C.byref(a), None)
+
+def rules(logits, out, ls, os, uncond=None, us=0, rows=3, vocab=100, dtype=0):
+    a = _lib.LogitsArgs(logits=logits, out=out, uncond=uncond, logits_stride=ls, uncond_stride=us, out_stride=os, repetition=1.0, rows=rows, vocab=vocab, dtype=dtype, device=0)
+    return L.t3mi_process_logits(C.byref(a), None)
+
+def refused(rc):
+    assert rc == _lib.ERR_ARG and b"share memory" in L.t3mi_last_error(), (rc, L.t3mi_last_error())
+
+def taken(rc):
+    assert rc == _lib.OK, (rc, L.t3mi_last_error())
+"""
+
+
+def test_outputs_that_share_memory_with_inputs_are_refused():
+    """At another address, that is: a row later, half a head further, in other steps, in the other type.  Woven views of one buffer are taken."""
+    run(CALLS + """
+row, F = 4 * 64, 4                                      # elements of a row of q, bytes of one
+s = (row, 64)
+taken(attend(P, P, s, s))
+taken(attend(P, P + 3 * row * F, s, s))
+for off in (16, 64 * F, row * F, 2 * row * F, 3 * row * F - 16):
+    refused(attend(P, P + off, s, s))
+    refused(attend(P + off, P, s, s))
+wide = (3 * row, 64)
+taken(attend(P, P + row * F, wide, wide))               # q and out beside each other in one buffer, either way round, and rows later
+taken(attend(P + 2 * row * F, P, wide, wide))
+taken(attend(P, P + 7 * row * F, wide, wide))
+refused(attend(P, P + row * F // 2, wide, wide))
+refused(attend(P, P + 3 * row * F, wide, wide))
+refused(attend(P, P + row * F, wide, (3 * row, 128)))   # (other steps in the same place)
+taken(attend(P, P + 64 * F, (2 * row, 128), (2 * row, 128)))    # heads in turn
+taken(attend(P, P + 5 * 64 * F, (4 * row, 128), (4 * row, 128)))
+refused(attend(P, P + 4 * 64 * F, (4 * row, 128), (4 * row, 128)))
+taken(attend(P, P + 64 * F, (64 * 2, 64 * 8), (64 * 2, 64 * 8)))  # heads outside, rows inside
+refused(attend(P, P + 64 * 2 * F, (64 * 2, 64 * 8), (64 * 2, 64 * 8)))
+taken(attend(P, P + row * F, (0, 64), (0, 64), rows=1))
+refused(attend(P, P + 64 * F, (0, 64), (0, 64), rows=1))
+refused(attend(P, P + 2 * row, s, s, qd=1, od=0))       # a bf16 row later, in fp32
+taken(attend(P, P + 3 * row * 2, s, s, qd=1, od=0))
+
+kv = (2 * 64, 64)
+k, v, q, o = P, P << 1, P << 2, P << 3
+taken(append(k, v, q, o, kv, kv, s, s))
+taken(append(k, v, q, q, kv, kv, s, s))
+packed = (8 * 64, 64)                                   # q, k and v of a row beside each other, q_out in q's place
+taken(append(P + row * F, P + (row + 128) * F, P, P, packed, packed, packed, packed))
+refused(append(P + row * F, P + (row + 128) * F, P, P + 64 * F, packed, packed, packed, packed))
+refused(append(k, v, q, k, kv, kv, s, s))
+refused(append(k, v, q, v + 128 * F, kv, kv, s, s))
+refused(append(k, v, q, q + row * F, kv, kv, s, s))
+
+taken(rules(P, P, 100, 100))
+taken(rules(P, P + 300 * F, 100, 100))
+taken(rules(P, P + 100 * F, 200, 200))
+for off in (F, 100 * F, 299 * F):
+    refused(rules(P, P + off, 100, 100))
+refused(rules(P, P + 100 * F, 200, 100))
+refused(rules(P << 1, P, 100, 100, P + F, 100))
+refused(rules(P << 1, P, 100, 100, P, 100))
+taken(rules(P << 1, P, 100, 100, P << 2, 100))
+taken(rules(P, P + 100 * F, 0, 100, P, 0))              # (a broadcast row before it)
+refused(rules(P + 100 * F, P, 0, 100))
+""")
