@@ -23,8 +23,8 @@ static int (*f_attention)(const t3mi_paged_cache*, const t3mi_attention_args*, v
 static int (*f_logits)(const t3mi_logits_args*, void*);
 
 /* of torch, and _lib.check */
-static PyObject *t_f32, *t_bf16, *t_i32, *c_empty, *c_empty_like, *c_stream, *c_grad, *c_check;
-static PyObject *s_data_ptr, *s_dtype, *s_get_device, *s_shape, *s_stride, *s_requires_grad, *s_device, *s_new_empty, *kw_dtype_device;
+static PyObject *t_f32, *t_bf16, *t_i32, *c_empty, *c_empty_like, *c_stream, *c_grad, *c_check, *c_forward, *c_unpack;
+static PyObject *s_data_ptr, *s_dtype, *s_get_device, *s_shape, *s_stride, *s_requires_grad, *s_device, *s_new_empty, *s_level, *s_tangent, *kw_dtype_device;
 
 enum { F32 = 1, BF16 = 2, I32 = 4 };
 #define MAXD 4
@@ -56,17 +56,35 @@ static int need_gpu(const char* name, int device, int wanted_device) {
     return -1;
 }
 
+/* forward mode: whether t carries a tangent of the level that is open, if one is */
+static int wants_no_tangent(const char* name, PyObject* t) {
+    PyObject* r = PyObject_GetAttr(c_forward, s_level);
+    if (!r) return -1;
+    const long level = PyLong_AsLong(r);
+    Py_DECREF(r);
+    if (level < 0) return PyErr_Occurred() ? -1 : 0;
+    if (!(r = PyObject_CallOneArg(c_unpack, t))) return -1;
+    PyObject* d = PyObject_GetAttr(r, s_tangent);
+    Py_DECREF(r);
+    if (!d) return -1;
+    const int none = d == Py_None;
+    Py_DECREF(d);
+    if (!none) PyErr_Format(PyExc_ValueError, "%s carries a forward-mode gradient: this operator has none", name);
+    return none ? 0 : -1;
+}
+
 static int wants_no_gradient(const char* name, PyObject* t) {
     PyObject* r = PyObject_GetAttr(t, s_requires_grad);
     if (!r) return -1;
     const int grad = PyObject_IsTrue(r);
     Py_DECREF(r);
-    if (grad <= 0) return grad;
+    if (grad < 0) return grad;
+    if (!grad) return wants_no_tangent(name, t);
     if (!(r = PyObject_CallNoArgs(c_grad))) return -1;
     const int on = PyObject_IsTrue(r);
     Py_DECREF(r);
     if (on > 0) PyErr_Format(PyExc_ValueError, "%s requires gradients: this operator has no backward pass", name);
-    return on ? -1 : 0;
+    return on ? -1 : wants_no_tangent(name, t);
 }
 
 #ifdef T3MI_DLPACK
@@ -477,11 +495,11 @@ fail:
     return NULL;
 }
 
-/* bind(4 addresses, float32, bfloat16, int32, empty, empty_like, raw stream of a device, is_grad_enabled, check, torch.Tensor, its DLPack
- * exchange capsule or None) */
+/* bind(4 addresses, float32, bfloat16, int32, empty, empty_like, raw stream of a device, is_grad_enabled, check, torch.autograd.forward_ad, its
+ * unpack_dual, torch.Tensor, its DLPack exchange capsule or None) */
 static PyObject* py_bind(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     (void)self;
-    if (wanted("bind", n, 14)) return NULL;
+    if (wanted("bind", n, 16)) return NULL;
     void* p[4];
     for (int i = 0; i < 4; ++i) {
         p[i] = PyLong_AsVoidPtr(a[i]);
@@ -491,18 +509,18 @@ static PyObject* py_bind(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     f_workspace = (int (*)(const t3mi_paged_cache*, const t3mi_attention_args*, size_t*))p[1];
     f_attention = (int (*)(const t3mi_paged_cache*, const t3mi_attention_args*, void*))p[2];
     f_logits = (int (*)(const t3mi_logits_args*, void*))p[3];
-    PyObject** keep[8] = {&t_f32, &t_bf16, &t_i32, &c_empty, &c_empty_like, &c_stream, &c_grad, &c_check};
-    for (int i = 0; i < 8; ++i) {
+    PyObject** keep[10] = {&t_f32, &t_bf16, &t_i32, &c_empty, &c_empty_like, &c_stream, &c_grad, &c_check, &c_forward, &c_unpack};
+    for (int i = 0; i < 10; ++i) {
         Py_INCREF(a[4 + i]);
         Py_XSETREF(*keep[i], a[4 + i]);
     }
 #ifdef T3MI_DLPACK
     f_dltensor = NULL;
-    if (PyType_Check(a[12]) && PyCapsule_IsValid(a[13], "dlpack_exchange_api")) {
-        const DLPackExchangeAPI* x = PyCapsule_GetPointer(a[13], "dlpack_exchange_api");
+    if (PyType_Check(a[14]) && PyCapsule_IsValid(a[15], "dlpack_exchange_api")) {
+        const DLPackExchangeAPI* x = PyCapsule_GetPointer(a[15], "dlpack_exchange_api");
         if (x->header.version.major == DLPACK_MAJOR_VERSION) {   /* (the table lives as long as torch does) */
-            Py_INCREF(a[12]);
-            Py_XSETREF(t_tensor, a[12]);
+            Py_INCREF(a[14]);
+            Py_XSETREF(t_tensor, a[14]);
             f_dltensor = x->dltensor_from_py_object_no_sync;
         }
     }
@@ -520,7 +538,8 @@ static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", "tensors to t
 
 PyMODINIT_FUNC PyInit__ops(void) {
     struct { PyObject** o; const char* s; } names[] = {{&s_data_ptr, "data_ptr"}, {&s_dtype, "dtype"}, {&s_get_device, "get_device"}, {&s_shape, "shape"},
-                                                        {&s_stride, "stride"}, {&s_requires_grad, "requires_grad"}, {&s_device, "device"}, {&s_new_empty, "new_empty"}};
+                                                        {&s_stride, "stride"}, {&s_requires_grad, "requires_grad"}, {&s_device, "device"}, {&s_new_empty, "new_empty"},
+                                                        {&s_level, "_current_level"}, {&s_tangent, "tangent"}};
     for (size_t i = 0; i < sizeof(names) / sizeof(names[0]); ++i)
         if (!(*names[i].o = PyUnicode_InternFromString(names[i].s))) return NULL;
     if (!(kw_dtype_device = Py_BuildValue("(ss)", "dtype", "device"))) return NULL;

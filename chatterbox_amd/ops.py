@@ -5,7 +5,7 @@ t3mi_process_logits (include/t3mi.h), for serving loops of one's own; the sessio
 (R/llama_traced.R:274-297) and its sampling tail knows the repetition penalty alone (R/t3.R:529-537).
 
 The calls enqueue on torch's current stream of the tensors' device and return; they may be captured into a graph.  Results and
-workspaces are torch allocations of that stream.  There is no backward pass: inputs that require gradients are refused.
+workspaces are torch allocations of that stream.  There is no backward pass and no forward-mode gradient: inputs that ask for either are refused.
 torch is imported by the first call, not with the package."""
 from __future__ import annotations
 
@@ -23,6 +23,7 @@ def _bind():
     """The compiled half of this module (csrc/py_ops.c: tensors to structs), bound to the library and to torch at the first call."""
     global _ops
     import torch
+    from torch.autograd import forward_ad
     try:
         from . import _ops as ext
     except ImportError as e:
@@ -33,7 +34,7 @@ def _bind():
     # the raw handle of torch's current stream; the spelled-out way where this torch has no short one
     stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
     ext.bind(*entry, torch.float32, torch.bfloat16, torch.int32, torch.empty, torch.empty_like, stream, torch.is_grad_enabled, _lib.check,
-             torch.Tensor, getattr(torch.Tensor, "__dlpack_c_exchange_api__", None))
+             forward_ad, forward_ad.unpack_dual, torch.Tensor, getattr(torch.Tensor, "__dlpack_c_exchange_api__", None))
     _ops = ext
     return ext
 
