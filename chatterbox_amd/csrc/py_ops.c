@@ -407,7 +407,7 @@ static int take_each(const char* name, PyObject* x, int64_t rows, int device, fl
     Ten t;
     *each = NULL;
     *number = 1.f;
-    if (PyFloat_Check(x) || PyLong_Check(x)) {
+    if (PyFloat_Check(x) || PyLong_Check(x) || !PyObject_HasAttr(x, s_get_device)) {   /* (numbers of other libraries, too) */
         *number = (float)PyFloat_AsDouble(x);
         return PyErr_Occurred() ? -1 : 0;
     }

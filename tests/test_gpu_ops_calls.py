@@ -50,3 +50,15 @@ def test_reverse_mode_gradients_are_refused_where_they_are_recorded():
                 call(leaf)
             with torch.no_grad():
                 assert torch.equal(call(leaf), want), (name, which)
+
+
+def test_a_penalty_is_a_number_of_any_kind():
+    """numpy's fp32 scalars are no Python floats; what is no number is named."""
+    np = pytest.importorskip("numpy")
+    l, tok, n = torch.randn(3, 50, device="cuda"), torch.arange(12, dtype=torch.int32, device="cuda").view(3, 4), torch.full((3,), 4, dtype=torch.int32, device="cuda")
+    for name, x in (("repetition_penalty", 1.25), ("frequency_penalty", 0.5), ("presence_penalty", 2.0)):
+        want = cb.process_logits(l, tokens=tok, n_tokens=n, **{name: x})
+        for kind in (np.float32, np.float64, np.float16):
+            assert torch.equal(cb.process_logits(l, tokens=tok, n_tokens=n, **{name: kind(x)}), want)
+        with pytest.raises(TypeError):
+            cb.process_logits(l, tokens=tok, n_tokens=n, **{name: "1.25"})
