@@ -1457,6 +1457,7 @@ int take_rules(const t3mi_model* m, const t3mi_logit_rules* r, LogitRules& o) {
         for (int t = 0; t < m->V && !some; ++t) some = (r->allowed[t >> 5] >> (t & 31)) & 1u;
         if (!some) return fail(T3MI_ERR_ARG, "logit rules: no token is allowed");
         o.allowed.assign(r->allowed, r->allowed + (m->V + 31) / 32);
+        if (m->V % 32) o.allowed.back() &= (1u << (m->V % 32)) - 1u;   // (bits past the vocabulary name no token)
     }
     if (r->n_bias > 0) {
         o.ids.assign(r->bias_ids, r->bias_ids + r->n_bias);
@@ -1466,6 +1467,17 @@ int take_rules(const t3mi_model* m, const t3mi_logit_rules* r, LogitRules& o) {
     o.pre = r->presence_penalty;
     return T3MI_OK;
 }
+
+// under mask_stop the stop token is never drawn: rules that allow it alone leave nothing
+bool leaves_a_token(const LogitRules& r, const t3mi_params& p) {
+    if (r.allowed.empty() || !p.mask_stop) return true;
+    for (size_t w = 0; w < r.allowed.size(); ++w) {
+        const uint32_t stop = (size_t)p.stop_token / 32 == w ? 1u << (p.stop_token & 31) : 0u;
+        if (r.allowed[w] & ~stop) return true;
+    }
+    return false;
+}
+const char* const kNoTokenText = "logit rules: the stop token alone is allowed, and mask_stop rules it out";
 
 // slot u's rules to the device (the stream is idle)
 int upload_rules(t3mi_model* m, Session* s, int u) {
@@ -1492,6 +1504,7 @@ const char* const kRuleTokensText = "logit rules: a session under rules may have
 int set_slot_rules(t3mi_model* m, Session* s, const std::vector<int>& utts, const LogitRules& r) {
     if (!s->rules && !r.any()) return T3MI_OK;
     if (s->cap > kRuleTokens) return fail(T3MI_ERR_ARG, kRuleTokensText);
+    if (!leaves_a_token(r, s->prm)) return fail(T3MI_ERR_ARG, kNoTokenText);
     std::vector<LogitRules> slots = s->slot_rules;
     slots.resize(s->n_utt);
     for (int u : utts) slots[u] = r;
@@ -1729,6 +1742,7 @@ static int session_begin(t3mi_model* m, int n_utt, int rpu, const float* const* 
     if (!(p->repetition_penalty > 0.f)) return fail(T3MI_ERR_ARG, "repetition_penalty must be > 0");
     if (p->stop_token < 0 || p->stop_token >= m->V) return fail(T3MI_ERR_ARG, "stop_token outside the vocabulary");
     if (p->drop_invalid_from < 0) return fail(T3MI_ERR_ARG, "drop_invalid_from must be >= 0");
+    if (!leaves_a_token(m->rules, *p)) return fail(T3MI_ERR_ARG, kNoTokenText);
     HIPCHK(hipSetDevice(m->device));
     if (m->sess) t3mi_session_end(m);
 

@@ -69,7 +69,7 @@ class T3Model:
 
     def set_logit_rules(self, bias=None, allowed=None, frequency_penalty: float = 0.0, presence_penalty: float = 0.0) -> None:
         """What every utterance to come is sampled under, until changed (t3mi_set_logit_rules; no argument: no rules).  bias: {token: value added
-        to its logit}; allowed: the tokens that may be drawn (ids, or a bool array [vocab]); frequency_penalty is subtracted
+        to its logit}; allowed: the tokens that may be drawn (ids, or a bool array [vocab]; under mask_stop one beside the stop token); frequency_penalty is subtracted
         once for every time a token has been drawn, presence_penalty if it has been.  Applied after guidance, before the sampler's own
         repetition penalty, temperature, min-p and top-p."""
         _lib.check(self._lib.t3mi_set_logit_rules(self._h, _logit_rules(self, bias, allowed, frequency_penalty, presence_penalty)))

@@ -209,7 +209,8 @@ int t3mi_session_pages(t3mi_model* m, int32_t* total, int32_t* free_pages);
 typedef struct t3mi_logit_rules {
     const int32_t* bias_ids;     /* [n_bias] token ids and the finite values added to their logits (an id named twice: the last)  */
     const float* bias_values;
-    const uint32_t* allowed;     /* [ceil(vocab / 32)] bits, token t's is bit t & 31 of word t >> 5; NULL: every token.  Some token must be allowed */
+    const uint32_t* allowed;     /* [ceil(vocab / 32)] bits, token t's is bit t & 31 of word t >> 5; NULL: every token.  Some token must be allowed
+                                  * (under mask_stop, which a session refuses otherwise, one beside the stop token) */
     int32_t n_bias;              /* at most 4094                                             */
     float frequency_penalty;     /* subtracted once for every time the token has been drawn  */
     float presence_penalty;      /* subtracted if it has been drawn                          */

@@ -153,3 +153,47 @@ for dtype, lens, decode_rows, prefill_rows in (("bf16", [40] * 5, 0, 0), ("bf16"
             assert got.count(rows * 3 * d * 4) == (1 if needed else 0), (dtype, lens, rows, got)
     m.close()
 """)
+
+
+def test_rules_that_leave_no_token_under_mask_stop_are_refused():
+    """The stop token alone allowed, and mask_stop: nothing could be drawn, and the sampler would have emitted the stop token all the same.  Refused where both are
+    known: at begin, at a slot's rules, at a refill; the session goes on as it was."""
+    run(RULES + """
+m = model()
+stop = m.stop_speech_token
+kw = dict(max_new_tokens=20, top_p=0.0)
+
+def refused(call):
+    try:
+        call()
+    except _lib.T3miError as e:
+        assert e.code == _lib.ERR_ARG and "mask_stop" in str(e), e
+        return
+    raise SystemExit("taken")
+
+with cb.Session(m, [prompt(9), prompt(5)], mask_stop=True, **kw) as s:
+    s.logit_rules(0, allowed=[5, stop])
+    before = step(s)
+    refused(lambda: s.logit_rules(1, allowed=[stop]))
+    assert step(s) == before
+    m.set_logit_rules(allowed=[stop])
+    refused(lambda: s.refill([1], [prompt(4)]))
+    assert step(s) == before
+    refused(lambda: cb.Session(m, [prompt(9)], mask_stop=True, **kw).__enter__())
+    assert step(s) == before                     # (refused before the running session is given up)
+    refused(lambda: cb.t3_inference_batch(m, [prompt(9)], mask_stop=True, **kw))
+refused(lambda: cb.t3_inference_continuous(m, [prompt(9)], mask_stop=True, **kw))
+with cb.Session(m, [prompt(9)], **kw) as s:      # without mask_stop the stop token may be all there is
+    assert step(s)[0][2] == 1
+m.set_logit_rules(allowed=[5])
+with cb.Session(m, [prompt(9)], mask_stop=True, **kw) as s:
+    assert step(s)[0][2] == 1
+# bits of the last word past the vocabulary are no tokens
+words = (C.c_uint32 * ((m.vocab + 31) // 32))()
+words[stop // 32] = 1 << (stop % 32)
+words[len(words) - 1] |= 0xFFFFFFFF << (m.vocab % 32) & 0xFFFFFFFF
+r = _lib.LogitRules(allowed=words)
+_lib.check(L.t3mi_set_logit_rules(m._h, C.byref(r)))
+refused(lambda: cb.Session(m, [prompt(9)], mask_stop=True, **kw).__enter__())
+m.close()
+""")
