@@ -18,6 +18,7 @@ Two call forms, told apart by the second argument:
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -91,10 +92,15 @@ def _logit_rules(model: T3Model, bias, allowed, frequency_penalty, presence_pena
     r = _lib.LogitRules(frequency_penalty=float(frequency_penalty), presence_penalty=float(presence_penalty))
     if bias:
         r.n_bias = len(bias)
-        r.bias_ids = (C.c_int32 * len(bias))(*[int(t) for t in bias])
+        ids = [operator.index(t) for t in bias]
+        if min(ids) < -2 ** 31 or max(ids) >= 2 ** 31:   # (what an int32 holds, the library checks against the vocabulary)
+            raise ValueError("bias: a token id is outside the vocabulary")
+        r.bias_ids = (C.c_int32 * len(bias))(*ids)
         r.bias_values = (C.c_float * len(bias))(*[float(v) for v in bias.values()])
     if allowed is not None:
-        a = np.asarray(allowed)
+        a = np.asarray(list(allowed) if isinstance(allowed, (set, frozenset)) else allowed)
+        if a.size and a.dtype != bool and a.dtype.kind not in "iu":
+            raise ValueError(f"allowed: token ids or bools wanted, got {a.dtype}")
         if a.dtype == bool:
             if a.shape != (model.vocab,):
                 raise ValueError(f"allowed: a bool array must be [{model.vocab}], got {a.shape}")

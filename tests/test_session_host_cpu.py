@@ -197,3 +197,25 @@ _lib.check(L.t3mi_set_logit_rules(m._h, C.byref(r)))
 refused(lambda: cb.Session(m, [prompt(9)], mask_stop=True, **kw).__enter__())
 m.close()
 """)
+
+
+def test_token_ids_of_rules_are_taken_as_they_are():
+    """An id past 32 bits used to wrap round to another token, a fractional one to be cut."""
+    run("""
+m = model()
+for bad in ({2 ** 32 + 3: 1.0}, {-2 ** 32 + 5: 1.0}, {m.vocab: 1.0}, {3.7: 1.0}, {"3": 1.0}):
+    try:
+        m.set_logit_rules(bias=bad)
+        raise SystemExit(f"taken: {bad}")
+    except (ValueError, TypeError, _lib.T3miError):
+        pass
+for bad in ([1.7], np.array([1.0, 2.0]), ["3"], [m.vocab], [-1], [2 ** 70], [True, False]):
+    try:
+        m.set_logit_rules(allowed=bad)
+        raise SystemExit(f"taken: {bad}")
+    except (ValueError, OverflowError):
+        pass
+for good in ([3, 5], (3, 5), {3, 5}, np.array([3, 5], np.uint8), range(3, 6), np.arange(m.vocab) < 4):
+    m.set_logit_rules(allowed=good, bias={np.int64(7): np.float32(1.0)})
+m.close()
+""")
