@@ -56,16 +56,22 @@ static int need_gpu(const char* name, int device, int wanted_device) {
     return -1;
 }
 
-/* forward mode: whether t carries a tangent of the level that is open, if one is */
-static int wants_no_tangent(const char* name, PyObject* t) {
+/* forward mode: whether a level is open (asked once a call), and whether t carries a tangent of it */
+static int level_open;
+static int look_for_level(void) {
     PyObject* r = PyObject_GetAttr(c_forward, s_level);
     if (!r) return -1;
     const long level = PyLong_AsLong(r);
     Py_DECREF(r);
-    if (level < 0) return PyErr_Occurred() ? -1 : 0;
-    if (!(r = PyObject_CallOneArg(c_unpack, t))) return -1;
-    PyObject* d = PyObject_GetAttr(r, s_tangent);
-    Py_DECREF(r);
+    if (level == -1 && PyErr_Occurred()) return -1;
+    level_open = level >= 0;
+    return 0;
+}
+static int wants_no_tangent(const char* name, PyObject* t) {
+    if (!level_open) return 0;
+    PyObject* r = PyObject_CallOneArg(c_unpack, t);
+    PyObject* d = r ? PyObject_GetAttr(r, s_tangent) : NULL;
+    Py_XDECREF(r);
     if (!d) return -1;
     const int none = d == Py_None;
     Py_DECREF(d);
@@ -266,7 +272,7 @@ static PyObject* py_append(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     t3mi_paged_cache c;
     t3mi_append_args g = {0};
     Ten kc, k, v, q, o, cs, sn;
-    if (wanted("append", n, 11) || take_cache(a[2], a[3], a[4], &c, &kc)) return NULL;
+    if (wanted("append", n, 11) || look_for_level() || take_cache(a[2], a[3], a[4], &c, &kc)) return NULL;
     if (take("k", a[0], F32 | BF16, 3, kc.device, &k) || take("v", a[1], k.dtype, 3, kc.device, &v)) return NULL;
     const int64_t rows = k.shape[0];
     if (rows > INT32_MAX || v.shape[0] != rows || k.shape[1] != c.kv_heads || v.shape[1] != c.kv_heads || k.shape[2] != c.head_dim || v.shape[2] != c.head_dim) {
@@ -331,7 +337,7 @@ static PyObject* py_attention(PyObject* self, PyObject* const* a, Py_ssize_t n) 
     t3mi_paged_cache c;
     t3mi_attention_args g = {0};
     Ten kc, q, o;
-    if (wanted("attention", n, 12) || take_cache(a[1], a[2], a[3], &c, &kc) || take("q", a[0], F32 | BF16, 3, kc.device, &q)) return NULL;
+    if (wanted("attention", n, 12) || look_for_level() || take_cache(a[1], a[2], a[3], &c, &kc) || take("q", a[0], F32 | BF16, 3, kc.device, &q)) return NULL;
     const int64_t rows = q.shape[0];
     if (rows > INT32_MAX || q.shape[1] > INT32_MAX || q.shape[2] != c.head_dim) {
         PyErr_Format(PyExc_ValueError, "q has head_dim %lld, the cache %d", (long long)q.shape[2], c.head_dim);
@@ -422,7 +428,7 @@ static PyObject* py_logits(PyObject* self, PyObject* const* a, Py_ssize_t n) {
     (void)self;
     t3mi_logits_args g = {0};
     Ten l, u, t, x, y, o;
-    if (wanted("logits", n, 12) || take("logits", a[0], F32 | BF16, 2, -1, &l)) return NULL;
+    if (wanted("logits", n, 12) || look_for_level() || take("logits", a[0], F32 | BF16, 2, -1, &l)) return NULL;
     const int64_t rows = l.shape[0], vocab = l.shape[1];
     if (rows > INT32_MAX || vocab > INT32_MAX) {
         PyErr_SetString(PyExc_ValueError, "logits has too many rows or entries");
