@@ -284,6 +284,14 @@ __device__ __forceinline__ void whole_pass(const PagedCache& c, const char* kbas
 // from 2^16 up, but finite (a column of an infinite maximum comes out as NaN either way, and does not change how its neighbours are rounded)
 __device__ __forceinline__ bool large(float x) { return (__float_as_uint(x) & 0x7FFFFFFFu) - 0x47800000u < 0x7F800000u - 0x47800000u; }
 
+// the kernel's arguments, read again: what only a rare path needs of them is not kept in registers for it (the scalar registers that took cost every
+// launch 0.6 us: the arguments' loads waited for each other)
+__device__ __forceinline__ const PagedAttnArgs& arguments_again() {
+    auto p = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const PagedAttnArgs*)p;
+}
+
 // what a part's sums count, its maximum being m and that of all parts top.  A part without a maximum saw no key, and its sums are 0, or it saw
 // NaN scores alone, and they are NaN: taken as they are
 __device__ __forceinline__ float part_factor(float m, float top) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 1.f; }
@@ -315,7 +323,7 @@ __device__ __forceinline__ RowPlan plan_row(const PagedAttnArgs& a, int len, int
 // QB, KB: bf16 queries, bf16 cache.  TK: keys of a tile, 32 or (fp32 cache) 16.  PAGES 0: pages of TK keys and more (a tile lies in one),
 // 1: smaller ones of 4 keys and more, 2: of 1, 2.  PARTS: bf16 parts of a weight (bf16 cache only; otherwise 1).
 template <bool QB, bool KB, int D, int TK, int PAGES, int PARTS>
-__global__ __launch_bounds__(512, QB && D == 128 && PAGES == 1 ? 3 : 2) void paged_attention_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(512, D == 64 ? (PAGES == 2 && KB && !QB ? 3 : 4) : (QB && PAGES == 1 ? 3 : 2)) void paged_attention_kernel(PagedAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) float sm[];
     constexpr int EB = KB ? 2 : 4;                  // bytes of a cache element
     constexpr int KC = KB ? D / 32 : D / 16;        // 16-byte pieces of a key to a lane
@@ -360,28 +368,6 @@ __global__ __launch_bounds__(512, QB && D == 128 && PAGES == 1 ? 3 : 2) void pag
     const RowPlan rp = plan_row(a, row_len, row_first, seq);
     if ((int)split >= rp.active) return;
     const int t_begin = rp.t0 + (int)split * rp.per, t_end = idle ? t_begin : min(rp.t1, t_begin + rp.per);
-    bf16x8 qb[KB ? QS : 1][KB ? KC : 1];
-    f32x4 qf[KB ? 1 : KC];
-    {
-        const bool live = n < gn;
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            if constexpr (QB) {
-                qb[0][c] = __builtin_bit_cast(bf16x8, live ? qw[c][0] : u32x4{0u, 0u, 0u, 0u});
-            } else if constexpr (KB) {
-                float x[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = live ? __uint_as_float(qw[c][j >> 2][j & 3]) : 0.f;
-                bf16x8 o[3];
-                to_parts<3, true>(x, o);
-#pragma unroll
-                for (int s = 0; s < QS; ++s) qb[s][c] = o[s];
-            } else {
-                qf[c] = live ? __builtin_bit_cast(f32x4, qw[c][0]) : f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-        }
-    }
-
     // byte offsets of this lane inside a tile: keys 16 t + n, piece g; values of keys 16 t + 4 g + i, elements D / 16 * n (or 4 n)
     const unsigned ksb = (unsigned)a.c.ks * EB, vsb = (unsigned)a.c.vs * EB;
     const char* kbase = static_cast<const char*>(a.c.k) + (long long)hk * a.c.kh * EB;
@@ -466,6 +452,28 @@ __global__ __launch_bounds__(512, QB && D == 128 && PAGES == 1 ? 3 : 2) void pag
         ask(min(t + kw, t_end - 1));
         load_k(t, pg);
         load_v(t, pg);
+        __builtin_amdgcn_sched_barrier(0);           // (the queries are cut while the first keys come)
+        bf16x8 qb[KB ? QS : 1][KB ? KC : 1];
+        f32x4 qf[KB ? 1 : KC];
+        {
+            const bool live = n < gn;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                if constexpr (QB) {
+                    qb[0][c] = __builtin_bit_cast(bf16x8, live ? qw[c][0] : u32x4{0u, 0u, 0u, 0u});
+                } else if constexpr (KB) {
+                    float x[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = live ? __uint_as_float(qw[c][j >> 2][j & 3]) : 0.f;
+                    bf16x8 o[3];
+                    to_parts<3, true>(x, o);
+#pragma unroll
+                    for (int s = 0; s < QS; ++s) qb[s][c] = o[s];
+                } else {
+                    qf[c] = live ? __builtin_bit_cast(f32x4, qw[c][0]) : f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+            }
+        }
         while (true) {
             const int t_next = min(t + kw, t_end - 1);   // (past the end: a tile that is asked for again, from L2, and not used)
             f32x4 s[U];
@@ -573,26 +581,32 @@ __global__ __launch_bounds__(512, QB && D == 128 && PAGES == 1 ? 3 : 2) void pag
             if (t >= t_end) break;
             pg = next;
         }
-    }
-    if constexpr (KB) {
-        bool nan = l != l;
+        if constexpr (KB) {
+            f32x4 all = acc[0];                      // (its sum is NaN if any of them is; opposite infinities only cost the second pass)
 #pragma unroll
-        for (int e = 0; e < NT; ++e)
+            for (int e = 1; e < NT; ++e) all += acc[e];
+            const float one = ((all[0] + all[1]) + (all[2] + all[3])) + l;
+            const bool nan = one != one;
+            if (const unsigned long long vote = __builtin_amdgcn_ballot_w64(nan && n < gn); __builtin_expect(vote != 0, 0)) {
+                f32x4 acc2[NT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) nan = nan || acc[e][i] != acc[e][i];
-        if (const unsigned long long vote = __builtin_amdgcn_ballot_w64(nan && n < gn); vote != 0) {
-            f32x4 acc2[NT];
+                for (int e = 0; e < NT; ++e) acc2[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+                float m2 = -INFINITY, l2 = 0.f;
+                const PagedAttnArgs& b = arguments_again();
+                const int seq2 = b.seq ? b.seq[row] : row;
+                const RowPlan r = plan_row(b, b.lengths[row], b.starts ? b.starts[row] : 0, seq2);
+                const int begin = r.t0 + (int)split * r.per;
+                whole_pass<QS, KC, NT, VT>(b.c, static_cast<const char*>(b.c.k) + (long long)hk * b.c.kh * EB, static_cast<const char*>(b.c.v) + (long long)hk * b.c.vh * EB,
+                                           b.c.table + (long long)seq2 * b.c.table_stride, qb, b.scale * 1.4426950408889634f, begin + wk, min(r.t1, begin + r.per), kw, r.len,
+                                           r.first, r.len, 16, m2, l2, acc2);
+                const bool redo = in_column(vote, n);
+                m = redo ? m2 : m;
+                l = redo ? l2 : l;
 #pragma unroll
-            for (int e = 0; e < NT; ++e) acc2[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-            float m2 = -INFINITY, l2 = 0.f;
-            whole_pass<QS, KC, NT, VT>(a.c, kbase, vbase, trow, qb, scale2, t_begin + wk, t_end, kw, rp.len, rp.first, rp.len, 16, m2, l2, acc2);
-            const bool redo = in_column(vote, n);
-            m = redo ? m2 : m;
-            l = redo ? l2 : l;
+                for (int e = 0; e < NT; ++e)
 #pragma unroll
-            for (int e = 0; e < NT; ++e)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[e][i] = redo ? acc2[e][i] : acc[e][i];
+                    for (int i = 0; i < 4; ++i) acc[e][i] = redo ? acc2[e][i] : acc[e][i];
+            }
         }
     }
     l = group_sum(l);
@@ -910,12 +924,12 @@ __global__ __launch_bounds__(256, D == 64 && !(SMALL && KB && !QB) ? 3 : 2) void
         }
     }
     if constexpr (KB) {
-        bool nan = l != l;
+        f32x4 all = acc[0];                          // (as above)
 #pragma unroll
-        for (int e = 0; e < NT; ++e)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) nan = nan || acc[e][i] != acc[e][i];
-        if (const unsigned long long vote = __builtin_amdgcn_ballot_w64(nan && has); vote != 0) {
+        for (int e = 1; e < NT; ++e) all += acc[e];
+        const float one = ((all[0] + all[1]) + (all[2] + all[3])) + l;
+        const bool nan = one != one;
+        if (const unsigned long long vote = __builtin_amdgcn_ballot_w64(nan && has); __builtin_expect(vote != 0, 0)) {
             f32x4 acc2[NT];
 #pragma unroll
             for (int e = 0; e < NT; ++e) acc2[e] = f32x4{0.f, 0.f, 0.f, 0.f};
