@@ -98,7 +98,7 @@ template <int TH, bool HOLD> struct IdList {
 };
 
 // Chunks [c0, c1) of CH entries of one row, one after the other, TH threads.  Bound: the logits are read and written once (256 rows of 131072
-// fp32 entries in 60 us: 4.6 TB/s); everything else is kept off that stream.  The entries go to LDS as they arrive, the next
+// fp32 entries with 2000 tokens, 300 biases and a mask each: 54.7 us in the kernel, 5.0 TB/s); everything else is kept off that stream.  The entries go to LDS as they arrive, the next
 // chunk's already asked for.  How often each entry occurs among the row's tokens and which bias names it is noted in LDS (integer atomics: the
 // result does not depend on their order; of two biases with one id the later counts).  Few entries have a note: a second walk over the
 // tokens and biases lets the first thread that comes to one take the note (which leaves it clear for the next chunk) and change the
@@ -168,7 +168,7 @@ __device__ __forceinline__ void process_chunks(const LogitsArgs& a, const Logits
         for (int i = 0; i < CH / (TH * 4); ++i) *reinterpret_cast<uint4*>(&note[(i * TH + tid) * 4]) = uint4{0u, 0u, 0u, 0u};
     }
     // a block of several chunks sorts the tokens by chunk first: each chunk then walks its own few, not the whole list (the call in
-    // launch_logits: 78 us without it, 49 with)
+    // launch_logits: 79 us without it, 53 with)
     const bool sorted = MANY && n_tok > 0 && n_tok <= kListed;
     if (sorted) {
         if (tid < kMaxRun) fill[tid] = 0;
@@ -311,8 +311,8 @@ __global__ __launch_bounds__(TH) void process_logits_kernel(LogitsArgs a, int ru
 template <typename T> void launch_logits(const LogitsArgs& a, hipStream_t s) {
     constexpr int CH = 4096, TH = 512;
     // Blocks of a row: two blocks fit a CU at a time (LDS), 512 the chip; the time goes as the rounds they make times the chunks of one,
-    // and a block starts for about three chunks' time (it sorts the row's tokens).  256 rows of 131072 fp32 entries with 2000 tokens and
-    // 300 biases each, in a loop over four inputs, 1 / 2 / 3 / 4 blocks a row: 75 / 49 / 63 / 62 us; a block for every chunk, unsorted: 78 us.
+    // and a block starts for about three chunks' time (it sorts the row's tokens).  256 rows of 131072 fp32 entries with 2000 tokens,
+    // 300 biases and a mask each, 20 calls in a row over four inputs, 1 / 2 / 3 / 4 blocks a row: 75 / 53 / 64 / 64 us; a block for every chunk, unsorted: 79.
     const int whole = a.vocab / CH;
     int run = 1;
     if ((long long)whole * a.rows > 512) {

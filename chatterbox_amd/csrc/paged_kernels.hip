@@ -661,7 +661,7 @@ __global__ __launch_bounds__(512, D == 64 ? (PAGES == 2 && KB && !QB ? 3 : 4) : 
 // ---- attention of a prompt's rows -------------------------------------------------------------------------------------------------
 // The same sums where neighbouring rows belong to one sequence: the 16 columns of a tile are 16 / G rows with the G heads of one key head, so a key
 // is read once for all of them (from L2: the blocks that read it are kv_heads apart).  Bound: the matrix and vector work of a tile, a few hundred
-// cycles for 32 keys x 16 columns (8000 rows of a prompt, 32 heads over 8 of 128, bf16: 2.2 ms, 239 TFLOP/s; row by row the reads take 4 to 10 times
+// cycles for 32 keys x 16 columns (8000 rows of a prompt, 32 heads over 8 of 128, bf16: 2.2 ms, 237 TFLOP/s; row by row the reads take 4 to 10 times
 // as long).  Rows of a block that belong to other sequences are taken in turn (a column that is not in turn has weight
 // zero), so any rows come out right.  A key that some of the rows see and others do not has weight zero for the others; only if such a tile holds a
 // value that is not finite (0 times it is not 0) are its rows summed one by one.
@@ -1198,8 +1198,8 @@ void plan_paged_attention(PagedAttnArgs& a) {
         a.n_split = tiles <= 24 || pairs >= 4096 ? 1 : (int)std::min((tiles + 6) / 12, 8LL);
         return;
     }
-    // Otherwise a block works on one key head.  Measured over 230 shapes (1 to 600 rows, 5 to 4096 tiles), this is within 4 % of the best of 60 plans
-    // on average.  `wide`: the kernel of 128 bf16 elements has registers for two waves to a SIMD, the others for four or (fp32, half the work to a
+    // Otherwise a block works on one key head.  Over 236 shapes (1 to 600 rows, 5 to 4096 tiles) this is 3.2 to 4.0 % above the best of the plans that were
+    // timed on average, by type and head_dim (profiles/paged_attention_plans.txt).  `wide`: the kernel of 128 bf16 elements has registers for two waves to a SIMD, the others for four or (fp32, half the work to a
     // tile) for as many as are useful.
     const bool wide = a.c.bf16 && a.c.head_dim == 128;
     const long long all = pairs * tiles;             // if every row is as long as the longest

@@ -47,8 +47,8 @@ def paged_kv_append(k, v, k_pages, v_pages, block_table, positions, *, seq=None,
     [sequences, pages of a sequence].  Row r goes to position positions[r] (int32) of sequence seq[r] (None: sequence r); a row whose
     position is negative, past the tables, or on no page of the pool is skipped.  rope = (cos, sin), float32 [positions,
     >= head_dim / 2]: keys and queries are rotated by halves, (a, b) -> (a cos - b sin, b cos + a sin); None: not rotated.  q:
-    [rows, heads, head_dim] of k's type; the rotated queries are returned (in q_out, which may be q and shares no memory with q, k or v otherwise), rows that were skipped are
-    left as they were in q_out.  No two rows may name the same place of the cache."""
+    [rows, heads, head_dim] of k's type; the rotated queries are returned (in q_out, which may be q and shares no memory with q, k or v
+    otherwise), rows that were skipped are left as they were in q_out.  No two rows may name the same place of the cache."""
     cos, sin = (None, None) if rope is None else rope
     return (_ops or _bind()).append(k, v, k_pages, v_pages, block_table, positions, seq, q, q_out, cos, sin)
 
@@ -61,11 +61,12 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, *, seq=None, star
     q: [rows, heads, head_dim], float32 (cache float32 or bfloat16) or bfloat16 (cache bfloat16); heads a multiple of the cache's,
     head h reads key head h // (heads // kv_heads).  Cache and block_table as in paged_kv_append; lengths, starts, seq: int32 [rows].
     scale: 1 / sqrt(head_dim) by default.  max_length: about the longest length, where the host knows it (the call is planned by it;
-    rows that are longer come out right too).  A row with no key gives zeros; a row of negative length is left as it was in out.
-    out: [rows, heads, head_dim], float32 or bfloat16 (new, in out_dtype or q's type, by default; may be q, and shares no memory with it otherwise).  Many rows of one sequence
-    (a prompt, causal) are rows with the same seq and lengths 1, 2, 3, ...; prompt says whether neighbouring rows mostly share a sequence: such rows share
-    the keys they read where there are enough of them for that to pay (None: four rows to a sequence of the table, and more of
-    them, since their order is not known; the results are the same up to rounding)."""
+    rows that are longer come out right too; with starts, about the most keys a row sees).  A row with no key, or whose scores are all
+    -inf, gives zeros; a row of negative length is left as it was in out.
+    out: [rows, heads, head_dim], float32 or bfloat16 (new, in out_dtype or q's type, by default; may be q, and shares no memory with it
+    otherwise).  Many rows of one sequence (a prompt, causal) are rows with the same seq and lengths 1, 2, 3, ...; prompt says whether
+    neighbouring rows mostly share a sequence: such rows share the keys they read where there are enough of them for that to pay (None:
+    four rows to a sequence of the table, and more of them, since their order is not known; the results are the same up to rounding)."""
     return (_ops or _bind()).attention(q, k_pages, v_pages, block_table, lengths, seq, starts, scale, max_length or 0, out, out_dtype,
                                        0 if prompt is None else 1 if prompt else -1)
 

@@ -65,7 +65,8 @@ class T3Model:
     def set_paged_kv(self, page_size: int = 64, pages: int = 0) -> None:
         """Sessions begun from now on keep keys and values in pages of `page_size` positions out of one pool of `pages` pages (0: the worst
         case); page_size 0: contiguous slabs again.  An utterance holds the pages of its prompt and its own token limit, so ragged
-        batches run in the memory they need (t3mi_set_paged_kv)."""
+        batches run in the memory they need.  A bf16 model's sessions of up to 4 rows then hold activations and cache in bf16, as larger ones do
+        (t3mi_set_paged_kv)."""
         _lib.check(self._lib.t3mi_set_paged_kv(self._h, int(page_size), int(pages)))
 
     def set_logit_rules(self, bias=None, allowed=None, frequency_penalty: float = 0.0, presence_penalty: float = 0.0) -> None:

@@ -198,7 +198,8 @@ int t3mi_session_begin_tokens(t3mi_model* m, int n_utt, const t3mi_cond* conds, 
  * or another is refilled, instead of a slab as long as the longest utterance may get: with n_pages below the worst case, a batch of
  * ragged utterances runs in the memory it needs.  t3mi_session_begin refuses (T3MI_ERR_ARG) what does not fit the pool, t3mi_session_refill
  * likewise (T3MI_ERR_STATE, the session is as it was); t3mi_generate_continuous opens as many slots as the pool serves and starts a
- * waiting utterance when enough pages are free.  Arithmetic is the batched path's (whatever the number of rows); keys and values are written
+ * waiting utterance when enough pages are free.  Arithmetic is the batched path's whatever the number of rows: bf16 models hold activations
+ * and cache in bf16 also in sessions of up to 4 rows, which compute in fp32 on slabs.  Keys and values are written
  * by the qkv product itself (fp32 weights below 64 rows: by t3mi_paged_append's kernel) and read by t3mi_paged_attention's. */
 int t3mi_set_paged_kv(t3mi_model* m, int page_size, int n_pages);
 /* pages of the running session's pool, and how many no utterance holds (0, 0 without pages) */
@@ -431,7 +432,8 @@ int t3mi_paged_append(const t3mi_paged_cache* cache, const t3mi_append_args* arg
 
 /* Attention of one new token per row: out[r, h] = sum_j softmax_j(scale * q[r, h] . k_j) v_j over the keys j in [starts[r],
  * lengths[r] + length_add) of sequence seq[r], head h reading key head h / (q_heads / kv_heads).  Row r of a prompt's queries attends
- * causally when lengths[r] is its position and length_add 1 (such rows share the keys they read, `prompt`).  A row with no key is written as zeros, a row whose length is negative is left as it
+ * causally when lengths[r] is its position and length_add 1 (such rows share the keys they read, `prompt`).  A row with no key, or whose scores
+ * are all -inf, is written as zeros, a row whose length is negative is left as it
  * was (padding of a batch); lengths beyond the block table end there.  Types: q fp32 over an fp32 or bf16 cache, q bf16 over a bf16
  * cache; out fp32 or bf16, and q itself only with q's type and strides; it shares no memory with q otherwise. */
 typedef struct t3mi_attention_args {
