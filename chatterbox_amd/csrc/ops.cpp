@@ -67,36 +67,58 @@ template <int N> bool disjoint(const int64_t (&stride)[N], const int64_t (&count
     return true;
 }
 
-// [rows, heads] runs of `inner` elements of `bytes` each
+// runs of `inner` elements of `bytes` each, in up to three dimensions
 struct Runs {
     const void* p;
-    int64_t stride[2], count[2];
+    int64_t stride[3], count[3];
     int64_t inner;
     int bytes;
 };
 // whether two tensors share no memory: apart as a whole, or woven into each other with the same strides and a distance that keeps them apart
 // (anything else is taken to share)
 bool apart(const Runs& a, const Runs& b) {
-    if (!a.p || !b.p || a.count[0] <= 0 || a.count[1] <= 0 || b.count[0] <= 0 || b.count[1] <= 0) return true;
+    if (!a.p || !b.p) return true;
     typedef __int128 wide;
     const auto from = [](const Runs& t) { return (wide)reinterpret_cast<uintptr_t>(t.p); };
-    const auto to = [&](const Runs& t) { return from(t) + ((wide)(t.count[0] - 1) * t.stride[0] + (wide)(t.count[1] - 1) * t.stride[1] + t.inner) * t.bytes; };
+    const auto to = [&](const Runs& t) {
+        wide n = t.inner;
+        for (int d = 0; d < 3; ++d) n += (wide)(t.count[d] - 1) * t.stride[d];
+        return from(t) + n * t.bytes;
+    };
+    for (int d = 0; d < 3; ++d)
+        if (a.count[d] <= 0 || b.count[d] <= 0) return true;
     if (to(a) <= from(b) || to(b) <= from(a)) return true;
-    int64_t stride[2];                               // common to both; 0: neither takes a second step, or has one to take
-    for (int d = 0; d < 2; ++d) {
+    int64_t stride[3];                               // common to both; 0: neither takes a second step, or has one to take
+    int by[3];                                       // dimensions, the largest step first
+    for (int d = 0; d < 3; ++d) {
         if (a.count[d] > 1 && b.count[d] > 1 && a.stride[d] != b.stride[d]) return false;
         stride[d] = a.count[d] > 1 ? a.stride[d] : b.count[d] > 1 ? b.stride[d] : 0;
+        int j = d;
+        for (; j > 0 && stride[by[j - 1]] < stride[d]; --j) by[j] = by[j - 1];
+        by[j] = d;
     }
     const wide off = from(b) - from(a);
     if (a.bytes != b.bytes || off % a.bytes) return false;
-    const auto place = [&](int64_t step) { const wide r = off / a.bytes % step; return r < 0 ? r + step : r; };   // of b's first run after one of a's
-    const int big = stride[0] >= stride[1] ? 0 : 1, small = 1 - big;
-    const auto extent = [&](const Runs& t) { return (wide)(t.count[small] - 1) * stride[small] + t.inner; };
-    if (stride[big] > 0 && place(stride[big]) >= extent(a) && place(stride[big]) + extent(b) <= stride[big]) return true;
-    return stride[small] > 0 && stride[big] % stride[small] == 0 && place(stride[small]) >= a.inner && place(stride[small]) + b.inner <= stride[small];
+    // within one step of a dimension that every larger step is a multiple of: what lies in the smaller dimensions, side by side
+    for (int i = 0; i < 3 && stride[by[i]] > 0; ++i) {
+        const int64_t step = stride[by[i]];
+        bool whole = true;
+        for (int j = 0; j < i; ++j) whole = whole && stride[by[j]] % step == 0;
+        wide at = off / a.bytes % step, in_a = a.inner, in_b = b.inner;
+        if (at < 0) at += step;
+        for (int j = i + 1; j < 3; ++j) {
+            in_a += (wide)(a.count[by[j]] - 1) * stride[by[j]];
+            in_b += (wide)(b.count[by[j]] - 1) * stride[by[j]];
+        }
+        if (whole && at >= in_a && at + in_b <= step) return true;
+    }
+    return false;
 }
 Runs runs(const void* p, const int64_t (&stride)[2], int64_t rows, int64_t heads, int64_t inner, int dtype) {
-    return {p, {stride[0], stride[1]}, {rows, heads}, inner, dtype == T3MI_W_BF16 ? 2 : 4};
+    return {p, {stride[0], stride[1], 0}, {rows, heads, 1}, inner, dtype == T3MI_W_BF16 ? 2 : 4};
+}
+Runs pages(const t3mi_paged_cache* c, const void* p, const int64_t (&s)[3]) {
+    return {p, {s[0], s[1], s[2]}, {c->n_pages, c->page_size, c->kv_heads}, c->head_dim, c->dtype == T3MI_W_BF16 ? 2 : 4};
 }
 
 int take_cache(const char* where, const t3mi_paged_cache* c, t3k::PagedCache& o) {
@@ -184,7 +206,8 @@ int t3mi_paged_append(const t3mi_paged_cache* cache, const t3mi_append_args* a, 
     if (a->rows == 0) return T3MI_OK;
     if (a->q && !disjoint<2>(a->q_out_stride, {a->rows, a->q_heads}, cache->head_dim)) return bad(me, "the rows and heads of q_out must not overlap");
     if (!disjoint<3>(cache->k_stride, {cache->n_pages, cache->page_size, cache->kv_heads}, cache->head_dim) ||
-        !disjoint<3>(cache->v_stride, {cache->n_pages, cache->page_size, cache->kv_heads}, cache->head_dim) || cache->k == cache->v)
+        !disjoint<3>(cache->v_stride, {cache->n_pages, cache->page_size, cache->kv_heads}, cache->head_dim) ||
+        !apart(pages(cache, cache->k, cache->k_stride), pages(cache, cache->v, cache->v_stride)))
         return bad(me, "the pages, slots and heads of the cache must not overlap");
     if (a->q) {
         const Runs out = runs(a->q_out, a->q_out_stride, a->rows, a->q_heads, cache->head_dim, a->dtype);

@@ -119,3 +119,33 @@ taken(rules(P << 1, P, 100, 100, P << 2, 100))
 taken(rules(P, P + 100 * F, 0, 100, P, 0))              # (a broadcast row before it)
 refused(rules(P + 100 * F, P, 0, 100))
 """)
+
+
+def test_keys_and_values_of_a_cache_that_share_memory_are_refused_by_the_append():
+    """Equal addresses alone were compared.  Keys and values of a page side by side, heads of both in turn, or one pool cut in two are taken."""
+    run(CALLS + """
+def put(k, v, strides, n_pages=9, page=16, heads=2, vs=None):
+    c = _lib.PagedCache(k=k, v=v, block_table=P << 10, table_stride=4, n_seqs=3, max_pages=4, n_pages=n_pages, page_size=page, kv_heads=heads, head_dim=64, dtype=0, device=0)
+    c.k_stride[:], c.v_stride[:] = strides, vs or strides
+    a = _lib.AppendArgs(k=P << 5, v=P << 6, positions=P << 10, rows=3, dtype=0)
+    a.k_stride[:] = a.v_stride[:] = (128, 64)
+    return L.t3mi_paged_append(C.byref(c), C.byref(a), None)
+
+def no(rc):
+    assert rc == _lib.ERR_ARG and b"must not overlap" in L.t3mi_last_error(), (rc, L.t3mi_last_error())
+
+page, F = 16 * 2 * 64, 4
+plain, side = (page, 128, 64), (2 * page, 128, 64)
+taken(put(P, P + 9 * page * F, plain))
+taken(put(P + 9 * page * F, P, plain))
+taken(put(P, P + page * F, side))                        # [pages, 2, slots, heads, 64]
+taken(put(P + page * F, P, side))
+taken(put(P, P + 2 * 64 * F, (2 * page, 256, 64)))       # [pages, slots, 2, heads, 64]
+taken(put(P, P + 64 * F, (2 * page, 256, 128)))          # [pages, slots, heads, 2, 64]
+taken(put(P, P + 16 * 64 * F, (2 * page, 64, 2 * 16 * 64)))   # [pages, heads, 2, slots, 64]
+for off in (0, 16, 64 * F, 128 * F, page * F, 8 * page * F, 9 * page * F - 16):
+    no(put(P, P + off, plain))
+for off in (0, 64 * F, page * F // 2, page * F + 128 * F, 2 * page * F):
+    no(put(P, P + off, side))
+no(put(P, P + page * F, side, vs=(2 * page, 64, 16 * 64)))    # (another order in the same place)
+""")
