@@ -157,6 +157,7 @@ int take_attention(const char* where, const t3mi_paged_cache* cache, const t3mi_
     if (a->rows && (!a->q || !a->out || !a->lengths)) return bad(where, "null pointer");
     if (!at16(a->q) || !at16(a->out) || !steps16(a->q_stride, a->q_dtype) || !steps16(a->out_stride, a->out_dtype))
         return bad(where, "q and out: addresses and strides must be multiples of 16 bytes");
+    if (!at4(a->lengths) || !at4(a->starts) || !at4(a->seq)) return bad(where, "lengths, starts and seq must be aligned to 4 bytes");
     if (!a->seq && a->rows > cache->n_seqs) return bad(where, "more rows than sequences (seq says which row belongs to which)");
     if (a->q == a->out && (a->q_dtype != a->out_dtype || a->q_stride[0] != a->out_stride[0] || a->q_stride[1] != a->out_stride[1]))
         if (a->rows) return bad(where, "out may be q only with the same strides and type");
@@ -199,6 +200,7 @@ int t3mi_paged_append(const t3mi_paged_cache* cache, const t3mi_append_args* a, 
         (a->q && (!steps16(a->q_stride, a->dtype) || !steps16(a->q_out_stride, a->dtype))))
         return bad(me, "k, v, q and q_out: addresses and strides must be multiples of 16 bytes");
     if (!at4(a->cos) || !at4(a->sin)) return bad(me, "rotation tables must be aligned to 4 bytes");
+    if (!at4(a->positions) || !at4(a->seq)) return bad(me, "positions and seq must be aligned to 4 bytes");
     if (a->q && a->q == a->q_out && (a->q_stride[0] != a->q_out_stride[0] || a->q_stride[1] != a->q_out_stride[1]))
         return bad(me, "q_out may be q only with the same strides");
     if (!a->seq && a->rows > cache->n_seqs) return bad(me, "more rows than sequences (seq says which row belongs to which)");

@@ -5,7 +5,7 @@ import pytest
 
 from chatterbox_amd import _lib
 from tests.host_runtime import run
-from tests.test_ops_cpu import P, attention, cache
+from tests.test_ops_cpu import P, append, attention, cache, refused
 
 
 def split(c, **kw):
@@ -149,3 +149,14 @@ for off in (0, 64 * F, page * F // 2, page * F + 128 * F, 2 * page * F):
     no(put(P, P + off, side))
 no(put(P, P + page * F, side, vs=(2 * page, 64, 16 * 64)))    # (another order in the same place)
 """)
+
+
+@pytest.mark.parametrize("which", ["lengths", "starts", "seq", "positions"])
+def test_misaligned_lists_are_refused(which):
+    """(a scalar load would drop the low bits of the address and read a neighbour)"""
+    L, kw = _lib.load(), {which: P + 2}
+    if which != "positions":
+        n = C.c_size_t(0)
+        refused(L.t3mi_paged_attention_workspace(cache(), attention(**kw), n), "4 bytes")
+    if which in ("positions", "seq"):
+        refused(L.t3mi_paged_append(cache(v=2 * P), append(q_out=P, **kw), None), "4 bytes")
