@@ -131,3 +131,46 @@ def test_rows_of_long_sequences_in_any_order(q_t, kv_t, out_t, rows, heads, kv_h
                 if out_t == "bf16":
                     tol = (tol + 2.0 ** -16 * mag) * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(ref)
                 assert (np.abs(got[r] - ref) <= tol).all(), (seqs, order, prompt, r)
+
+
+@pytest.mark.parametrize("q_t,out_t", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("order", ["slots", "heads"])
+def test_infinities_in_one_of_neighbouring_heads(q_t, out_t, order):
+    """Enough rows that blocks take four neighbouring key heads (heads beside each other) or one (heads apart), in a graph that is replayed as the values come and
+    go: head 2 sees an infinite value and a key of -inf score, the others keep their bits."""
+    lens = [70, 33, 90]
+    k, v, table, keys, vals = make_cache(lens, 16, 16, 64, "bf16", 29, order)
+    rows = [(i % 3, lens[i % 3]) for i in range(120)]
+    q = torch.randn(120, 16, 64, generator=torch.Generator().manual_seed(5)).bfloat16().abs().to(DT[q_t]).cuda() + 0.5
+    seq, n = t32([s for s, _ in rows]), t32([m for _, m in rows])
+    call = lambda: cb.paged_attention(q, k, v, table, n, seq=seq, out_dtype=DT[out_t], prompt=False)  # noqa: E731
+    clean = call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    at = [(s, lens[s] - 5) for s in range(3)]
+    places = [(int(table[s, j // 16]), j % 16) for s, j in at]
+    held = [(k[p, i, 2, 3].clone(), v[p, i, 2, 7].clone()) for p, i in places]
+    for turn in range(4):
+        for (p, i), (hk, hv), (s, j) in zip(places, held, at):
+            k[p, i, 2, 3] = float("-inf") if turn == 1 else hk
+            v[p, i, 2, 7] = float("inf") if turn == 2 else hv
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call())
+        rest = [h for h in range(16) if h != 2]
+        assert torch.equal(out[:, rest], clean[:, rest])
+        if turn == 1:
+            assert bool(out.isfinite().all())
+            for r in (0, 1, 2, 119):
+                s, m = rows[r]
+                keep = [x for x in range(m) if x != at[s][1]]
+                ref, mag, err = ref_attention(np64(q[r, 2:3]), keys[s][keep, 2:3], vals[s][keep, 2:3], 0, 0.125)
+                tol = 2 * (2 * err * U + 2.0 ** -21 + m * U) * mag
+                if out_t == "bf16":
+                    tol = (tol + 2.0 ** -16 * mag) * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(ref)
+                assert (np.abs(np64(out[r, 2:3]) - ref) <= tol).all(), r
+        elif turn == 2:
+            assert bool((out[:, 2, 7] == float("inf")).all()) and bool(out[:, 2, :7].isfinite().all()) and bool(out[:, 2, 8:].isfinite().all())
+        else:
+            assert torch.equal(out, clean)
